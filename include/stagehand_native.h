@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define SH_ABI_VERSION 8
+#define SH_ABI_VERSION 9
 
 enum sh_status {
   SH_OK = 0,
@@ -708,6 +708,115 @@ int sh_dl_free(sh_dl_managed_tensor* t);
  * 64-bit multiplicative inverse stored in sh_unpack_desc.div_magic), exported
  * so the index arithmetic can be checked on a CPU. No reference counterpart. */
 int sh_index_div(uint32_t d, const uint32_t* n, uint32_t* q, size_t count);
+
+/* ── Operators on SquareQ weights and attention heads ──────────────────────
+ *
+ * Device operators beside the streaming path (no reference counterpart: the
+ * reference leaves them to torch, on dequantised weights). Device pointers and
+ * a stream, as everywhere; each call only queues kernels on `stream` (of the
+ * current device), allocates nothing and may be captured into a graph once the
+ * operator has run on the device (its first call loads the kernels). */
+enum sh_dtype { SH_DTYPE_BF16 = 1, SH_DTYPE_F16 = 2, SH_DTYPE_F32 = 3 };
+
+/* A SquareQ weight as it lies in device memory: `rows` output features of
+ * `cols` int8 values, `ld` bytes apart, W[n][k] = (q[n][k] - zero_point[n]) *
+ * scale[n]. q is 16-byte aligned, ld a multiple of 16 and at least cols; all
+ * rows * ld bytes are readable (what lies between cols and ld does not
+ * matter). zero_point may be NULL (zeros), bias too (none); both are fp32. */
+typedef struct sh_i8_weight {
+  const void* q;
+  uint64_t ld;
+  uint32_t rows;
+  uint32_t cols; /* 1 .. SH_I8_MAX_COLS */
+  const float* scale;
+  const float* zero_point;
+  const float* bias;
+} sh_i8_weight;
+
+/* int32 sums of 8-bit products stay exact up to here (128 * 128 * 131071 < 2^31). */
+#define SH_I8_MAX_COLS 131071u
+/* Quantised tokens lie in rows of a multiple of this many bytes, zero-filled past cols. */
+#define SH_I8_TOKEN_ALIGN 128u
+
+/* Quantises `tokens` rows of `cols` values (`dtype`, x_ld elements apart) to
+ * int8 with one scale each: a = max |x|, q = rint(x * (127 / a)), scale = a /
+ * 127, sums = sum q. A token whose largest magnitude is under 2^-120 counts as
+ * zero (q = 0, scale = 0). A token with an infinity or a NaN gets q = 0 and
+ * scale = NaN: all outputs of that token are NaN, no other token's are. q is
+ * 16-byte aligned, q_ld a multiple of SH_I8_TOKEN_ALIGN and at least cols;
+ * the bytes from cols to q_ld are set to 0. sums may be NULL. */
+int sh_quantize_tokens(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, uint32_t cols, void* q,
+                       uint64_t q_ld, float* scale, int32_t* sums, void* stream);
+/* out[t][n] = scale[t] * w.scale[n] * (sum_k q[t][k] w.q[n][k] - w.zero_point[n] sums[t]) + w.bias[n],
+ * rounded once to out_dtype; rows of out are out_ld elements apart. The int8
+ * products are summed exactly, in 32 bits. q, scale and sums as
+ * sh_quantize_tokens writes them for w.cols columns (sums is read only where w
+ * has zero points). out must not overlap the inputs. */
+int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, const int32_t* sums, uint32_t tokens,
+                 const sh_i8_weight* w, void* out, uint32_t out_dtype, uint64_t out_ld, void* stream);
+/* Both: out = quantised(x) * W^T + bias, in the type of x. The results are
+ * those of the two calls above. The workspace (16-byte aligned device memory,
+ * in use until the call's kernels have run) holds at least
+ * sh_linear_i8_workspace bytes, which is 0 for a few tokens. */
+int sh_linear_i8_workspace(uint32_t tokens, uint32_t cols, uint64_t* bytes);
+int sh_linear_i8(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, const sh_i8_weight* w, void* out,
+                 uint64_t out_ld, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Heads of a (batch, heads, seq, dim) tensor with strides in elements; the
+ * values of one head are contiguous. */
+typedef struct sh_heads {
+  void* data;
+  uint64_t batch_stride;
+  uint64_t head_stride;
+  uint64_t seq_stride;
+} sh_heads;
+
+/* RMS norm of every head of the queries and keys, then the position rotation:
+ *   n = x * weight * (mean(x^2) + eps)^(-1/2)            over the dim values of a head
+ *   out[a] = n[a] c - n[b] s,  out[b] = n[b] c + n[a] s  for the rot / 2 pairs (a, b)
+ * with (a, b) = (p, p + rot / 2), or (2p, 2p + 1) when `interleaved`, and c, s
+ * = cos, sin[position][p], rows of table_ld floats. Values past rot are not
+ * rotated; rot = 0 only norms. A token's position is positions[b *
+ * position_batch_stride + s] (int32 or int64), or start + s when positions is
+ * NULL; a position outside the table_rows rows of the tables gives NaN for
+ * that token. Statistics and products are fp32, outputs are rounded once.
+ *
+ * sh_qk_norm_rope reads q and k and writes q_out and k_out.
+ * sh_qk_norm_rope_backward reads q, k and the gradients of the outputs (in
+ * q_out and k_out) and writes, of dq, dk, dq_weight and dk_weight, those that
+ * are not NULL (the weights' in weight_dtype; a sum over all tokens and heads
+ * in a fixed order). Outputs may not overlap inputs, save q_out = q and k_out = k with
+ * equal strides. */
+typedef struct sh_qk_norm_rope_args {
+  sh_heads q, k;
+  sh_heads q_out, k_out;
+  sh_heads dq, dk;
+  const void* q_weight; /* dim values of weight_dtype, or NULL: ones */
+  const void* k_weight;
+  void* dq_weight;
+  void* dk_weight;
+  const float* cos;
+  const float* sin;
+  const void* positions;
+  uint64_t table_ld;
+  uint64_t position_batch_stride;
+  int64_t start;
+  uint32_t table_rows;
+  uint32_t position_bytes; /* 4 or 8 */
+  uint32_t batch, seq, q_heads, k_heads;
+  uint32_t dim; /* even, 2 .. SH_QK_MAX_DIM */
+  uint32_t rot; /* even, 0 .. dim */
+  uint32_t dtype, weight_dtype;
+  uint32_t interleaved;
+  float eps;
+} sh_qk_norm_rope_args;
+#define SH_QK_MAX_DIM 512u
+int sh_qk_norm_rope(const sh_qk_norm_rope_args* args, void* stream);
+/* Bytes of workspace that the backward pass needs (0 when neither weight's
+ * gradient is wanted); 16-byte aligned device memory. */
+int sh_qk_norm_rope_workspace(const sh_qk_norm_rope_args* args, uint64_t* bytes);
+int sh_qk_norm_rope_backward(const sh_qk_norm_rope_args* args, void* workspace, uint64_t workspace_bytes,
+                             void* stream);
 
 #ifdef __cplusplus
 }

@@ -224,6 +224,13 @@ _SIGNATURES: dict[str, list] = {
     "sh_turbo_block_times": [_vp, _u32, _vp, _vp],
     "sh_turbo_trace_spans": [_vp, _vp, _u32, _vp],
     "sh_turbo_set_writeback_chunks": [_vp, _u32],
+    "sh_quantize_tokens": [_vp, _u32, ctypes.c_uint64, _u32, _u32, _vp, ctypes.c_uint64, _vp, _vp, _vp],
+    "sh_matmul_i8": [_vp, ctypes.c_uint64, _vp, _vp, _u32, _vp, _vp, _u32, ctypes.c_uint64, _vp],
+    "sh_linear_i8_workspace": [_u32, _u32, ctypes.POINTER(ctypes.c_uint64)],
+    "sh_linear_i8": [_vp, _u32, ctypes.c_uint64, _u32, _vp, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp],
+    "sh_qk_norm_rope": [_vp, _vp],
+    "sh_qk_norm_rope_workspace": [_vp, ctypes.POINTER(ctypes.c_uint64)],
+    "sh_qk_norm_rope_backward": [_vp, _vp, ctypes.c_uint64, _vp],
 }
 
 # Mirror of `struct sh_chunk_region`.
@@ -263,7 +270,7 @@ TURBO_SPAN_DTYPE = np.dtype([("block", "<u4"), ("kind", "<u4"), ("start_ns", "<u
                              ("bytes", "<u8")])
 TURBO_SPAN_WRITEBACK, TURBO_SPAN_HOST_WAIT = 0, 1
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,154 @@
+// Linear layers on SquareQ weights that stay in int8 (no reference counterpart: the reference
+// dequantises them, src/stagehand/scheduler.py:285-308, and multiplies in bf16).
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sh_int8_args.h"
+#include "sh_internal.h"
+#include "stagehand_native.h"
+
+namespace {
+
+bool known_dtype(uint32_t d) { return d == SH_DTYPE_BF16 || d == SH_DTYPE_F16 || d == SH_DTYPE_F32; }
+uint32_t dtype_bytes(uint32_t d) { return d == SH_DTYPE_F32 ? 4 : 2; }
+bool misaligned(const void* p, uint32_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+
+uint64_t token_ld(uint32_t cols) {
+  return ((uint64_t)cols + SH_I8_TOKEN_ALIGN - 1) / SH_I8_TOKEN_ALIGN * SH_I8_TOKEN_ALIGN;
+}
+
+int check_weight(const sh_i8_weight* w, const char* who) {
+  if (w == nullptr) return sh::fail(SH_ERR_INVALID, "%s: w is NULL", who);
+  if (w->cols == 0 || w->cols > SH_I8_MAX_COLS)
+    return sh::fail(SH_ERR_INVALID, "%s: cols %u is not in 1 .. %u", who, w->cols, SH_I8_MAX_COLS);
+  if (w->ld % 16 != 0 || w->ld < w->cols || w->ld > (1u << 20))
+    return sh::fail(SH_ERR_INVALID, "%s: ld %llu of the weight is not a multiple of 16 in %u .. %u", who,
+                    (unsigned long long)w->ld, w->cols, 1u << 20);
+  if (w->rows > 0 && (w->q == nullptr || w->scale == nullptr))
+    return sh::fail(SH_ERR_INVALID, "%s: the weight's q or scale is NULL", who);
+  if (misaligned(w->q, 16)) return sh::fail(SH_ERR_INVALID, "%s: the weight's q is not 16-byte aligned", who);
+  if (misaligned(w->scale, 4) || misaligned(w->zero_point, 4) || misaligned(w->bias, 4))
+    return sh::fail(SH_ERR_INVALID, "%s: the weight's scale, zero_point or bias is not 4-byte aligned", who);
+  return SH_OK;
+}
+
+int check_x(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, uint32_t cols, const char* who) {
+  if (!known_dtype(dtype)) return sh::fail(SH_ERR_INVALID, "%s: unknown dtype %u", who, dtype);
+  if (cols == 0 || cols > SH_I8_MAX_COLS)
+    return sh::fail(SH_ERR_INVALID, "%s: cols %u is not in 1 .. %u", who, cols, SH_I8_MAX_COLS);
+  if (tokens == 0) return SH_OK;
+  if (x == nullptr) return sh::fail(SH_ERR_INVALID, "%s: x is NULL", who);
+  if (misaligned(x, dtype_bytes(dtype))) return sh::fail(SH_ERR_INVALID, "%s: x is not aligned to its type", who);
+  (void)x_ld;  // any stride: rows of x may overlap, they are only read
+  return SH_OK;
+}
+
+int check_out(const void* out, uint32_t dtype, uint64_t out_ld, uint32_t tokens, uint32_t rows, const char* who) {
+  if (!known_dtype(dtype)) return sh::fail(SH_ERR_INVALID, "%s: unknown out dtype %u", who, dtype);
+  if (tokens == 0 || rows == 0) return SH_OK;
+  if (out == nullptr) return sh::fail(SH_ERR_INVALID, "%s: out is NULL", who);
+  if (misaligned(out, dtype_bytes(dtype))) return sh::fail(SH_ERR_INVALID, "%s: out is not aligned to its type", who);
+  if (tokens > 1 && out_ld < rows)
+    return sh::fail(SH_ERR_INVALID, "%s: out_ld %llu is less than the weight's %u rows", who,
+                    (unsigned long long)out_ld, rows);
+  return SH_OK;
+}
+
+int check_tokens(const void* q, uint64_t q_ld, const float* scale, const int32_t* sums, uint32_t tokens, uint32_t cols,
+                 const char* who) {
+  if (q_ld % SH_I8_TOKEN_ALIGN != 0 || q_ld < cols || q_ld > (1u << 20))
+    return sh::fail(SH_ERR_INVALID, "%s: q_ld %llu is not a multiple of %u in %u .. %u", who, (unsigned long long)q_ld,
+                    SH_I8_TOKEN_ALIGN, cols, 1u << 20);
+  if (tokens > 0 && (q == nullptr || scale == nullptr)) return sh::fail(SH_ERR_INVALID, "%s: q or scale is NULL", who);
+  if (misaligned(q, 16)) return sh::fail(SH_ERR_INVALID, "%s: q is not 16-byte aligned", who);
+  if (misaligned(scale, 4) || misaligned(sums, 4))
+    return sh::fail(SH_ERR_INVALID, "%s: scale or sums is not 4-byte aligned", who);
+  return SH_OK;
+}
+
+int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* who) {
+  void* args[] = {(void*)&a};
+  return sh::launch_kernel(sh::kKernQuantizeTokens, a.tokens, 256, stream, args, who);
+}
+
+int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who) {
+  const uint64_t tiles = ((uint64_t)a.tokens + 15) / 16 * (((uint64_t)a.rows + 63) / 64);
+  const uint64_t grid = (tiles + 3) / 4;
+  if (grid > 0xFFFFFFFFull / 256)
+    return sh::fail(SH_ERR_INVALID, "%s: %u tokens x %u rows are too many for one launch", who, a.tokens, a.rows);
+  void* args[] = {(void*)&a};
+  return sh::launch_kernel(sh::kKernMatmulI8, (uint32_t)grid, 256, stream, args, who);
+}
+
+struct Workspace {
+  uint64_t q_ld, sums, scale, bytes;
+};
+
+// q, then the scales, then the sums.
+Workspace workspace_of(uint32_t tokens, uint32_t cols) {
+  Workspace s{};
+  s.q_ld = token_ld(cols);
+  s.scale = s.q_ld * tokens;
+  s.sums = s.scale + 4ull * tokens;
+  s.bytes = s.sums + 4ull * tokens;
+  return s;
+}
+
+}  // namespace
+
+extern "C" int sh_quantize_tokens(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, uint32_t cols, void* q,
+                                  uint64_t q_ld, float* scale, int32_t* sums, void* stream) {
+  const char* who = "sh_quantize_tokens";
+  sh::clear_error();
+  if (int st = check_x(x, dtype, x_ld, tokens, cols, who)) return st;
+  if (int st = check_tokens(q, q_ld, scale, sums, tokens, cols, who)) return st;
+  if (tokens == 0) return SH_OK;
+  if (tokens > 0xFFFFFFFFu / 256)
+    return sh::fail(SH_ERR_INVALID, "%s: %u tokens are too many for one launch", who, tokens);
+  const sh::QuantizeArgs a{x, q, scale, sums, x_ld, q_ld, tokens, cols, dtype};
+  return launch_quantize(a, (hipStream_t)stream, who);
+}
+
+extern "C" int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, const int32_t* sums, uint32_t tokens,
+                            const sh_i8_weight* w, void* out, uint32_t out_dtype, uint64_t out_ld, void* stream) {
+  const char* who = "sh_matmul_i8";
+  sh::clear_error();
+  if (int st = check_weight(w, who)) return st;
+  if (int st = check_tokens(q, q_ld, scale, sums, tokens, w->cols, who)) return st;
+  if (int st = check_out(out, out_dtype, out_ld, tokens, w->rows, who)) return st;
+  if (tokens == 0 || w->rows == 0) return SH_OK;
+  if (w->zero_point != nullptr && sums == nullptr)
+    return sh::fail(SH_ERR_INVALID, "%s: sums is NULL, but the weight has zero points", who);
+  const sh::MatmulI8Args a{q,   scale, sums, w->q,   w->scale, w->zero_point, w->bias, out,
+                           q_ld, w->ld, out_ld, tokens, w->rows, w->cols,       out_dtype};
+  return launch_matmul(a, (hipStream_t)stream, who);
+}
+
+extern "C" int sh_linear_i8_workspace(uint32_t tokens, uint32_t cols, uint64_t* bytes) {
+  sh::clear_error();
+  if (bytes == nullptr) return sh::fail(SH_ERR_INVALID, "sh_linear_i8_workspace: bytes is NULL");
+  *bytes = workspace_of(tokens, cols).bytes;
+  return SH_OK;
+}
+
+extern "C" int sh_linear_i8(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, const sh_i8_weight* w,
+                            void* out, uint64_t out_ld, void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* who = "sh_linear_i8";
+  sh::clear_error();
+  if (int st = check_weight(w, who)) return st;
+  if (int st = check_x(x, dtype, x_ld, tokens, w->cols, who)) return st;
+  if (int st = check_out(out, dtype, out_ld, tokens, w->rows, who)) return st;
+  if (tokens == 0 || w->rows == 0) return SH_OK;
+  const Workspace s = workspace_of(tokens, w->cols);
+  if (workspace_bytes < s.bytes || (s.bytes > 0 && workspace == nullptr))
+    return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
+                    (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
+  if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(ws + s.scale);
+  int32_t* sums = reinterpret_cast<int32_t*>(ws + s.sums);
+  if (int st = sh_quantize_tokens(x, dtype, x_ld, tokens, w->cols, ws, s.q_ld, scale, sums, stream)) return st;
+  return sh_matmul_i8(ws, s.q_ld, scale, sums, tokens, w, out, dtype, out_ld, stream);
+}

@@ -90,6 +90,11 @@ enum KernelId : int {
   kKernDigestWide,
   kKernDigestCompare,
   kKernDigestCompareWide,
+  kKernQuantizeTokens,
+  kKernMatmulI8,
+  kKernQkNormRope,
+  kKernQkNormRopeBackward,
+  kKernQkNormDweight,
   kKernelCount
 };
 // Launches kernel `id` of the current device: a 1-D grid of `grid` workgroups of `block`

@@ -8,7 +8,9 @@
 // unregistration (a call into HIP that unloads the code on every device) for the exit-time
 // destructors, to run in whatever order the runtime, a profiler's tool library and the other
 // libraries end in. Here each device loads the code objects on first use, with that device
-// current, and sh_shutdown unloads them (unload_kernels) while the runtime is whole.
+// current, and sh_shutdown unloads them (unload_kernels) while the runtime is whole. The streaming
+// path's kernels load together; each operator's load at that operator's first call, so a program
+// that only streams does not wait for them.
 
 #include <hip/hip_runtime.h>
 
@@ -22,11 +24,27 @@
 extern "C" {
 extern const unsigned char sh_co_unpack[];
 extern const unsigned char sh_co_digest[];
+extern const unsigned char sh_co_int8[];
+extern const unsigned char sh_co_qk_norm[];
 }
 
 namespace {
 
-enum ModuleId : int { kModUnpack = 0, kModDigest, kModules };
+enum ModuleId : int { kModUnpack = 0, kModDigest, kModInt8, kModQkNorm, kModules };
+
+struct ModuleSpec {
+  const unsigned char* image;
+  const char* name;
+  int set;  // modules of one set load together
+};
+
+constexpr int kSets = 3;
+const ModuleSpec kModuleSpecs[kModules] = {
+    {sh_co_unpack, "unpack", 0},
+    {sh_co_digest, "digest", 0},
+    {sh_co_int8, "int8", 1},
+    {sh_co_qk_norm, "qk_norm", 2},
+};
 
 struct KernelSpec {
   ModuleId module;
@@ -50,6 +68,11 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModDigest, "sh_digest_wide_kernel"},
     {kModDigest, "sh_digest_compare_kernel"},
     {kModDigest, "sh_digest_compare_wide_kernel"},
+    {kModInt8, "sh_quantize_tokens_kernel"},
+    {kModInt8, "sh_matmul_i8_kernel"},
+    {kModQkNorm, "sh_qk_norm_rope_kernel"},
+    {kModQkNorm, "sh_qk_norm_rope_backward_kernel"},
+    {kModQkNorm, "sh_qk_norm_dweight_kernel"},
 };
 
 struct DeviceKernels {
@@ -61,10 +84,8 @@ struct DeviceKernels {
 
 constexpr int kMaxDevices = 64;
 // Published once loaded (release); read without the lock on every launch (acquire).
-std::atomic<DeviceKernels*> g_kernels[kMaxDevices];
+std::atomic<DeviceKernels*> g_kernels[kSets][kMaxDevices];
 std::mutex g_load_mu;
-
-const void* image_of(ModuleId m) { return m == kModUnpack ? (const void*)sh_co_unpack : (const void*)sh_co_digest; }
 
 int unload(DeviceKernels* k) {
   hipError_t first = hipSuccess;
@@ -79,8 +100,9 @@ int unload(DeviceKernels* k) {
                                         hipGetErrorString(first));
 }
 
-// Loads the code objects on device `dev` (current) and resolves every kernel and the scratch.
-int load(int dev, DeviceKernels** out, const char* who) {
+// Loads a set's code objects on device `dev` (current) and resolves its kernels and, for the streaming
+// path, the scratch.
+int load(int set, int dev, DeviceKernels** out, const char* who) {
   DeviceKernels* k = new (std::nothrow) DeviceKernels();
   if (k == nullptr) return sh::fail(SH_ERR_OOM, "%s: out of host memory", who);
   auto bail = [&](hipError_t e, const char* what, const char* name) {
@@ -90,12 +112,18 @@ int load(int dev, DeviceKernels** out, const char* who) {
                     who, what, name, dev, (int)e, hipGetErrorString(e));
   };
   for (int m = 0; m < kModules; ++m) {
-    const hipError_t e = hipModuleLoadData(&k->module[m], image_of((ModuleId)m));
-    if (e != hipSuccess) return bail(e, "loading code object", m == kModUnpack ? "unpack" : "digest");
+    if (kModuleSpecs[m].set != set) continue;
+    const hipError_t e = hipModuleLoadData(&k->module[m], kModuleSpecs[m].image);
+    if (e != hipSuccess) return bail(e, "loading code object", kModuleSpecs[m].name);
   }
   for (int i = 0; i < sh::kKernelCount; ++i) {
+    if (kModuleSpecs[kKernelSpecs[i].module].set != set) continue;
     const hipError_t e = hipModuleGetFunction(&k->fn[i], k->module[kKernelSpecs[i].module], kKernelSpecs[i].name);
     if (e != hipSuccess) return bail(e, "resolving kernel", kKernelSpecs[i].name);
+  }
+  if (set != kModuleSpecs[kModUnpack].set) {
+    *out = k;
+    return SH_OK;
   }
   hipDeviceptr_t p = nullptr;
   const hipError_t e = hipModuleGetGlobal(&p, &k->scratch_bytes, k->module[kModUnpack], "scratch");
@@ -112,17 +140,17 @@ int load(int dev, DeviceKernels** out, const char* who) {
   return SH_OK;
 }
 
-int current(DeviceKernels** out, const char* who) {
+int current(int set, DeviceKernels** out, const char* who) {
   int dev = -1;
   SH_HIP(hipGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return sh::fail(SH_ERR_INVALID, "%s: device %d out of range", who, dev);
-  DeviceKernels* k = g_kernels[dev].load(std::memory_order_acquire);
+  DeviceKernels* k = g_kernels[set][dev].load(std::memory_order_acquire);
   if (k == nullptr) {
     std::lock_guard<std::mutex> lk(g_load_mu);
-    k = g_kernels[dev].load(std::memory_order_relaxed);
+    k = g_kernels[set][dev].load(std::memory_order_relaxed);
     if (k == nullptr) {
-      if (int st = load(dev, &k, who)) return st;
-      g_kernels[dev].store(k, std::memory_order_release);
+      if (int st = load(set, dev, &k, who)) return st;
+      g_kernels[set][dev].store(k, std::memory_order_release);
     }
   }
   *out = k;
@@ -135,7 +163,7 @@ namespace sh {
 
 int launch_kernel(KernelId id, uint32_t grid, uint32_t block, hipStream_t stream, void** args, const char* who) {
   DeviceKernels* k = nullptr;
-  if (int st = current(&k, who)) return st;
+  if (int st = current(kModuleSpecs[kKernelSpecs[id].module].set, &k, who)) return st;
   const hipError_t e = hipModuleLaunchKernel(k->fn[id], grid, 1, 1, block, 1, 1, 0, stream, args, nullptr);
   if (e != hipSuccess)
     return fail(SH_ERR_HIP, "%s: launching %s (%u workgroups): HIP error %d (%s)", who, kKernelSpecs[id].name, grid,
@@ -145,7 +173,7 @@ int launch_kernel(KernelId id, uint32_t grid, uint32_t block, hipStream_t stream
 
 int noalloc_scratch(void** ptr, const char* who) {
   DeviceKernels* k = nullptr;
-  if (int st = current(&k, who)) return st;
+  if (int st = current(kModuleSpecs[kModUnpack].set, &k, who)) return st;
   *ptr = k->scratch;
   return SH_OK;
 }
@@ -155,8 +183,9 @@ int unload_kernels() {
   int cur = -1;
   (void)hipGetDevice(&cur);
   int status = SH_OK;
-  for (int dev = 0; dev < kMaxDevices; ++dev) {
-    DeviceKernels* k = g_kernels[dev].load(std::memory_order_acquire);
+  for (int i = 0; i < kSets * kMaxDevices; ++i) {
+    const int set = i / kMaxDevices, dev = i % kMaxDevices;
+    DeviceKernels* k = g_kernels[set][dev].load(std::memory_order_acquire);
     if (k == nullptr) continue;
     // Work queued with these kernels must end before their code is unloaded.
     hipError_t e = hipSetDevice(dev);
@@ -167,7 +196,7 @@ int unload_kernels() {
                       dev, (int)e, hipGetErrorString(e));
       continue;  // left loaded: something may still run them
     }
-    g_kernels[dev].store(nullptr, std::memory_order_release);
+    g_kernels[set][dev].store(nullptr, std::memory_order_release);
     const int st = unload(k);
     if (status == SH_OK) status = st;
     delete k;
@@ -178,7 +207,11 @@ int unload_kernels() {
 
 int kernels_loaded() {
   int n = 0;
-  for (int dev = 0; dev < kMaxDevices; ++dev) n += g_kernels[dev].load(std::memory_order_acquire) != nullptr;
+  for (int dev = 0; dev < kMaxDevices; ++dev) {
+    bool any = false;
+    for (int set = 0; set < kSets; ++set) any |= g_kernels[set][dev].load(std::memory_order_acquire) != nullptr;
+    n += any;
+  }
   return n;
 }
 

@@ -1,0 +1,215 @@
+"""RMS norms of query and key heads with the position rotation, in one pass, with gradients.
+
+For every head of the queries and keys::
+
+    n = x * weight * rsqrt(mean(x²) + eps)
+    out[a], out[b] = n[a] c - n[b] s, n[b] c + n[a] s        for the rot / 2 pairs (a, b)
+
+with ``(a, b) = (p, p + rot / 2)``, or ``(2p, 2p + 1)`` when ``interleaved``, and ``c, s`` the row of
+the tables ``cos`` and ``sin`` that belongs to the token's position. Statistics, products and the
+weights' gradients are held in fp32; outputs and gradients are rounded once.
+
+Everything runs on the caller's current torch stream unless ``stream`` is given. There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from stagehand_amd import _native
+from stagehand_amd.int8 import DTYPE_CODES, check_device, on_stream
+from stagehand_amd.unpack import current_stream_handle
+
+__all__ = ["qk_norm_rope"]
+
+MAX_DIM = 512  # SH_QK_MAX_DIM
+
+# Mirror of `struct sh_qk_norm_rope_args`: six sh_heads, then pointers and strides, then 32-bit fields.
+_ARGS = struct.Struct("<24Q" "7Q" "2Q" "q" "11If")
+
+
+def _heads(t: torch.Tensor | None) -> tuple[int, int, int, int]:
+    if t is None:
+        return 0, 0, 0, 0
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1], s[2]
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _rows_of_values(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(3) == 1 else t.contiguous()
+
+
+def _pack(q, k, q_out, k_out, dq, dk, q_weight, k_weight, dq_weight, dk_weight, cos, sin, positions, start,
+          interleaved, eps) -> bytes:
+    x = q if q is not None else k
+    batch, _, seq, dim = x.shape
+    weight = q_weight if q_weight is not None else k_weight
+    rot = 0 if cos is None else 2 * cos.shape[1]
+    return _ARGS.pack(
+        *_heads(q), *_heads(k), *_heads(q_out), *_heads(k_out), *_heads(dq), *_heads(dk),
+        _ptr(q_weight), _ptr(k_weight), _ptr(dq_weight), _ptr(dk_weight), _ptr(cos), _ptr(sin), _ptr(positions),
+        cos.stride(0) if rot else 0, positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
+        start, cos.shape[0] if rot else 0, positions.element_size() if positions is not None else 0,
+        batch, seq, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], dim, rot,
+        DTYPE_CODES[x.dtype], DTYPE_CODES[x.dtype if weight is None else weight.dtype], int(interleaved), eps)
+
+
+def _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out):
+    _native.check(_native.lib().sh_qk_norm_rope(
+        _pack(q, k, q_out, k_out, None, None, q_weight, k_weight, None, None, cos, sin, positions, start, interleaved,
+              eps), current_stream_handle()))
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.options = start, interleaved, eps
+        return q_out, k_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        want_q, want_k, want_qw, want_kw = ctx.needs_input_grad[:4]
+        if not (want_q or want_qw):
+            q = dq_out = None
+        if not (want_k or want_kw):
+            k = dk_out = None
+        device = (q if q is not None else k).device
+        with torch.cuda.device(device):
+            dq = _like(q) if want_q else None
+            dk = _like(k) if want_k else None
+            dqw = torch.empty_like(q_weight) if want_qw else None
+            dkw = torch.empty_like(k_weight) if want_kw else None
+            dq_out = None if q is None else _rows_of_values(dq_out)
+            dk_out = None if k is None else _rows_of_values(dk_out)
+            args = _pack(q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, dqw, dkw, cos, sin, positions, *ctx.options)
+            lib = _native.lib()
+            need = ctypes.c_uint64()
+            _native.check(lib.sh_qk_norm_rope_workspace(args, ctypes.byref(need)))
+            ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+            _native.check(lib.sh_qk_norm_rope_backward(args, _ptr(ws), need.value, current_stream_handle()))
+        return dq, dk, dqw, dkw, None, None, None, None, None, None
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A tensor for the gradient of ``x``, with its dims in the order of ``x``'s memory."""
+    d = torch.empty_like(x)
+    return d if d.stride(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    *,
+    positions: torch.Tensor | None = None,
+    start: int = 0,
+    interleaved: bool = False,
+    eps: float = 1e-6,
+    out: tuple[torch.Tensor, torch.Tensor | None] | None = None,
+    stream: torch.cuda.Stream | int | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Normed and rotated ``(q, k)``; see the module's formulas.
+
+    ``q`` is ``(batch, heads, seq, dim)``, ``k`` the same with any number of heads (or None). Any
+    strides: views of a fused projection are read in place. ``q_weight`` and ``k_weight`` hold ``dim``
+    values of one type, None stands for ones. ``cos`` and ``sin`` are float32 ``(positions, rot / 2)``
+    with ``rot <= dim``; without them there is only the norm. Token ``s`` is at position ``start + s``,
+    or at ``positions[s]`` / ``positions[b, s]`` (int32 or int64 on the device; a position that the
+    tables do not have gives NaN for that token).
+
+    The outputs are contiguous, or written to ``out``: tensors of the same shapes with any strides
+    that keep a head's values together (a slice of a joint sequence, or ``q`` and ``k`` themselves).
+    Gradients flow to ``q``, ``k`` and the weights, not to the tables, and not through ``out``."""
+    if stream is not None:
+        with on_stream(stream):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
+                                interleaved=interleaved, eps=eps, out=out)
+    device = q.device
+    check_device(q, None, "q")
+    if q.dim() != 4 or q.dtype not in DTYPE_CODES:
+        raise ValueError(f"q must be (batch, heads, seq, dim) in bfloat16, float16 or float32, got {q.dtype} {tuple(q.shape)}")
+    batch, _, seq, dim = q.shape
+    if dim % 2 or not 2 <= dim <= MAX_DIM:
+        raise ValueError(f"dim {dim} is not an even number in 2 .. {MAX_DIM}")
+    if k is not None:
+        check_device(k, device, "k")
+        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (batch, seq, dim):
+            raise ValueError(f"k must be {q.dtype} with q's batch, seq and dim, got {k.dtype} {tuple(k.shape)} for q {tuple(q.shape)}")
+    elif k_weight is not None:
+        raise ValueError("k_weight is given without k")
+    for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        check_device(w, device, what)
+        if w.shape != (dim,) or w.dtype not in DTYPE_CODES or w.stride(0) != 1:
+            raise ValueError(f"{what} must be {dim} contiguous values in bfloat16, float16 or float32, got {w.dtype} {tuple(w.shape)}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin are given together or not at all")
+    if cos is not None:
+        check_device(cos, device, "cos")
+        check_device(sin, device, "sin")
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
+                2 * cos.shape[1] > dim or cos.stride() != sin.stride() or (cos.shape[1] > 1 and cos.stride(1) != 1):
+            raise ValueError(f"cos and sin must be float32 (positions, rot / 2) rows with rot <= {dim}, "
+                             f"got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+        if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+            raise ValueError("cos and sin have no gradient: detach them")
+        if cos.shape[1] == 0:
+            cos = sin = None
+    if positions is not None:
+        if cos is None or start:
+            raise ValueError("positions are given with cos and sin, and without start")
+        check_device(positions, device, "positions")
+        if positions.dtype not in (torch.int32, torch.int64) or \
+                tuple(positions.shape) not in ((seq,), (batch, seq), (1, seq)):
+            raise ValueError(f"positions must be int32 or int64 ({seq},) or ({batch}, {seq}), got {positions.dtype} {tuple(positions.shape)}")
+        if positions.dim() == 2 and positions.shape[0] == 1:
+            positions = positions[0]
+        if seq > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+    elif cos is not None and not 0 <= start <= cos.shape[0] - seq:
+        raise ValueError(f"positions {start} .. {start + seq - 1} are not all in the tables' {cos.shape[0]} rows")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
+                                interleaved=interleaved, eps=eps, out=out)
+    q = _rows_of_values(q)
+    k = None if k is None else _rows_of_values(k)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    if out is None:
+        if grad:
+            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, start, bool(interleaved), float(eps))
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+    else:
+        if grad:
+            raise RuntimeError("out= has no gradient: call qk_norm_rope under torch.no_grad(), or without out")
+        q_out, k_out = out
+        for what, o, x in (("q", q_out, q), ("k", k_out, k)):
+            if (o is None) != (x is None):
+                raise ValueError(f"out has {'no' if o is None else 'a'} tensor for {what}")
+            if o is None:
+                continue
+            check_device(o, device, f"out for {what}")
+            if o.shape != x.shape or o.dtype != x.dtype or o.stride(3) != 1:
+                raise ValueError(f"out for {what} must be {x.dtype} {tuple(x.shape)} with contiguous heads, "
+                                 f"got {o.dtype} {tuple(o.shape)} strides {o.stride()}")
+    _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
+    return q_out, k_out
