@@ -74,6 +74,12 @@ int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* w
 }
 
 int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who) {
+  if (a.tokens > 128) {
+    const uint64_t grid = (((uint64_t)a.tokens + 255) / 256) * (((uint64_t)a.rows + 255) / 256);
+    if (grid > 0xFFFFFFFFull / 512) return sh::fail(SH_ERR_INVALID, "%s: %u tokens x %u rows are too many for one launch", who, a.tokens, a.rows);
+    void* args[] = {(void*)&a};
+    return sh::launch_kernel(sh::kKernMatmulI8Tile256, (uint32_t)grid, 512, stream, args, who);
+  }
   const uint64_t tiles = ((uint64_t)a.tokens + 15) / 16 * (((uint64_t)a.rows + 63) / 64);
   const uint64_t grid = (tiles + 3) / 4;
   if (grid > 0xFFFFFFFFull / 256)

@@ -79,6 +79,204 @@ extern "C" __global__ __launch_bounds__(256) void sh_quantize_tokens_kernel(sh::
   }
 }
 
+// ── the tiled product ─────────────────────────────────────────────────────
+
+namespace {
+
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kStep = 128;  // bytes of a row that one stage holds: a cache line, two MFMAs'
+
+// The 16-byte chunk c of a stage's row lies in slot c ^ swizzle(row): the 16 rows of a fragment then lie in
+// different LDS banks.
+__device__ __forceinline__ constexpr uint32_t swizzle(uint32_t row) { return (row >> 1) & 7; }
+
+// Buffer resource of up to `tile` rows from row `first` on: reads past them give 0.
+__device__ __forceinline__ i32x4_t rows_resource(const void* base, uint64_t ld, uint32_t first, uint32_t count,
+                                                 uint32_t tile) {
+  const uint64_t p = (uint64_t)base + (uint64_t)first * ld;
+  i32x4_t r;
+  r[0] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)p);
+  r[1] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(p >> 32) & 0xFFFF);  // stride 0
+  r[2] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(min(count - first, tile) * ld));
+  r[3] = 0x00020000;
+  return r;
+}
+
+// Brings 16 bytes per lane from the resource into LDS, at lds + 16 * lane. Written as assembly: the compiler
+// would wait for the load before the next LDS read, whatever stage that reads. It has no output register;
+// whoever reads the stage waits for it (vmcnt) and for the barrier after that. M0 has no other use here. The
+// whole offset is in the register that the resource's range check covers.
+__device__ __forceinline__ void load_to_lds(i32x4_t r, uint32_t lds, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
+               "s"(r));
+}
+
+struct alignas(16) Words4 {
+  uint32_t w[4];
+};
+
+// Stores 16 consecutive values; `whole`: all of them lie in the row, at a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_run(T* out, const float (&v)[16], bool whole, uint32_t count) {
+  if (whole) {
+    constexpr uint32_t kPer = 16 / sizeof(T);
+#pragma unroll
+    for (uint32_t i = 0; i < 16 / kPer; ++i) {
+      Words4 w;
+      T x[kPer];
+#pragma unroll
+      for (uint32_t j = 0; j < kPer; ++j) x[j] = (T)v[i * kPer + j];
+      __builtin_memcpy(&w, x, 16);
+      *reinterpret_cast<Words4*>(out + i * kPer) = w;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j)
+      if (j < count) out[j] = (T)v[j];
+  }
+}
+
+// TT tokens x TN rows by WT x WN wavefronts, each with FT x FN MFMA tiles.
+template <uint32_t TT, uint32_t TN, uint32_t WT, uint32_t WN>
+__device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* lds) {
+  constexpr uint32_t kStage = (TT + TN) * kStep;
+  constexpr uint32_t kWaves = WT * WN;
+  constexpr uint32_t FT = TT / WT / 16, FN = TN / WN / 16;
+  constexpr uint32_t LT = TT / 8 / kWaves, LN = TN / 8 / kWaves;  // loads of 8 rows per wavefront
+  static_assert(FN == 4, "a wavefront's rows are one group of 64 permuted ones");
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  // the workgroup's tile: XCDs take consecutive runs of tiles, tiles run down groups of 8 in the tokens
+  const uint32_t tiles_t = (a.tokens + TT - 1) / TT, tiles_n = (a.rows + TN - 1) / TN, tiles = tiles_t * tiles_n;
+  uint32_t p = blockIdx.x;
+  {
+    const uint32_t per = tiles / 8, extra = tiles % 8, x = p % 8, i = p / 8;
+    p = x * per + min(x, extra) + i;
+  }
+  const uint32_t group = p / (8 * tiles_n), in_group = p % (8 * tiles_n), g_rows = min(tiles_t - group * 8, 8u);
+  const uint32_t t0 = (group * 8 + in_group % g_rows) * TT, n0 = in_group / g_rows * TN;
+
+  const i32x4_t tr = rows_resource(a.tq, a.t_ld, t0, a.tokens, TT);
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, TN);
+  // Lane l of a load brings slot l % 8 of row l / 8. The rows of the weight lie permuted in LDS, so that the
+  // MFMA results of one lane are 16 consecutive ones: fragment f, row i holds row (i / 4) * 16 + f * 4 + i % 4
+  // of the wavefront's 64.
+  uint32_t t_off[LT], n_off[LN];
+#pragma unroll
+  for (uint32_t j = 0; j < LT; ++j) {
+    const uint32_t row = (j * kWaves + wave) * 8 + lane / 8;
+    t_off[j] = row * (uint32_t)a.t_ld + ((lane % 8) ^ swizzle(row)) * 16;
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < LN; ++j) {
+    const uint32_t row = (j * kWaves + wave) * 8 + lane / 8;
+    const uint32_t src = row / 64 * 64 + row % 16 / 4 * 16 + row / 16 % 4 * 4 + row % 4;
+    n_off[j] = src * (uint32_t)a.w_ld + ((lane % 8) ^ swizzle(row)) * 16;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 1024;
+  auto load = [&](uint32_t stage, uint32_t k) {
+#pragma unroll
+    for (uint32_t j = 0; j < LT; ++j) load_to_lds(tr, lds0 + stage * kStage + j * kWaves * 1024, t_off[j] + k);
+#pragma unroll
+    for (uint32_t j = 0; j < LN; ++j)
+      load_to_lds(wr, lds0 + stage * kStage + TT * kStep + j * kWaves * 1024, n_off[j] + k);
+  };
+  const uint32_t l16 = lane & 15, part = lane / 16;
+  const uint32_t wt = wave / WN, wn = wave % WN;
+  i32x4_t acc[FT][FN] = {};
+  const uint8_t* t_at = lds + (wt * (TT / WT) + l16) * kStep;
+  const uint8_t* n_at = lds + (TT + wn * (TN / WN) + l16) * kStep;
+  struct Fragments {
+    i32x4_t t[FT], n[FN];
+  };
+  auto read = [&](Fragments& f, uint32_t stage, uint32_t half) {
+    const uint32_t slot = ((half * 4 + part) ^ swizzle(l16)) * 16 + stage * kStage;
+#pragma unroll
+    for (uint32_t j = 0; j < FN; ++j) f.n[j] = *reinterpret_cast<const i32x4_t*>(n_at + slot + j * 16 * kStep);
+#pragma unroll
+    for (uint32_t i = 0; i < FT; ++i) f.t[i] = *reinterpret_cast<const i32x4_t*>(t_at + slot + i * 16 * kStep);
+  };
+  auto multiply = [&](const Fragments& f) {
+#pragma unroll
+    for (uint32_t i = 0; i < FT; ++i)
+#pragma unroll
+      for (uint32_t j = 0; j < FN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.n[j], f.t[i], acc[i][j], 0, 0, 0);
+    // an LDS read, then the MFMAs that hide it
+#pragma unroll
+    for (uint32_t i = 0; i < FT + FN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, FT * FN / (FT + FN), 0);
+    }
+  };
+  // Two stages. The fragments of a half stage are read into registers while the half before is multiplied, so
+  // a stage is read to its end when the first half of its products is done: the loads of the stage after the
+  // next start there and have one stage's products to land in.
+  // Each wavefront waits for its own loads, then the barrier says that everyone's have landed and that
+  // everyone has read the stage whose place the next loads take.
+  const uint32_t end = (uint32_t)a.t_ld;  // a multiple of kStep; the tokens are zero past cols
+  auto landed = [&] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  Fragments f0, f1;
+  load(0, 0);
+  landed();
+  if (kStep < end) load(1, kStep);
+  read(f0, 0, 0);
+  uint32_t s = 0;
+  for (uint32_t k = kStep; k < end; k += kStep) {
+    read(f1, s, 1);
+    multiply(f0);
+    landed();
+    if (k + kStep < end) load(s, k + kStep);
+    s ^= 1;
+    read(f0, s, 0);
+    multiply(f1);
+  }
+  read(f1, s, 1);
+  multiply(f0);
+  multiply(f1);
+
+  // lane: token t0 + .. + l16 of each token fragment, 16 consecutive rows
+  const uint32_t n = n0 + wn * (TN / WN) + part * 16;
+  if (n >= a.rows) return;
+  const uint32_t count = min(a.rows - n, 16u);
+  float ws[16], wz[16], wb[16];
+#pragma unroll
+  for (uint32_t j = 0; j < 16; ++j) {
+    ws[j] = j < count ? a.w_scale[n + j] : 0.0f;
+    wz[j] = j < count && a.w_zp != nullptr ? a.w_zp[n + j] : 0.0f;
+    wb[j] = j < count && a.bias != nullptr ? a.bias[n + j] : 0.0f;
+  }
+  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
+  const bool whole = count == 16 && ((uintptr_t)a.out | a.out_ld * bytes | n * bytes) % 16 == 0;
+#pragma unroll
+  for (uint32_t i = 0; i < FT; ++i) {
+    const uint32_t t = t0 + wt * (TT / WT) + i * 16 + l16;
+    if (t >= a.tokens) continue;
+    const float scale = a.t_scale[t];
+    const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
+    float v[16];
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) {
+      // wz is 0 without zero points: the same value
+      v[j] = __builtin_fmaf(-wz[j], sum, (float)acc[i][j / 4][j % 4]) * (scale * ws[j]) + wb[j];
+    }
+    const uint64_t at = (uint64_t)t * a.out_ld + n;
+    if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, v, whole, count);
+    else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, v, whole, count);
+    else store_run(static_cast<float*>(a.out) + at, v, whole, count);
+  }
+}
+
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(512, 2) void sh_matmul_i8_256_kernel(sh::MatmulI8Args a) {
+  __shared__ uint8_t lds[2 * 512 * kStep];
+  matmul_tile<256, 256, 2, 4>(a, lds);
+}
+
 // Each wavefront: 16 tokens x 64 rows, operands straight from global memory. In a 16x16x64 MFMA lane
 // l gives row l % 16 of each operand, bytes (l / 16) * 16 .. + 15, and holds elements (l / 16) * 4 + r
 // of the first operand's rows for column l % 16 of the second's.

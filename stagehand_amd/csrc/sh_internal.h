@@ -92,6 +92,7 @@ enum KernelId : int {
   kKernDigestCompareWide,
   kKernQuantizeTokens,
   kKernMatmulI8,
+  kKernMatmulI8Tile256,
   kKernQkNormRope,
   kKernQkNormRopeBackward,
   kKernQkNormDweight,

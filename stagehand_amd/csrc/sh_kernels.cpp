@@ -70,6 +70,7 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModDigest, "sh_digest_compare_wide_kernel"},
     {kModInt8, "sh_quantize_tokens_kernel"},
     {kModInt8, "sh_matmul_i8_kernel"},
+    {kModInt8, "sh_matmul_i8_256_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_backward_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
