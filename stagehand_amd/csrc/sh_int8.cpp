@@ -69,8 +69,14 @@ int check_tokens(const void* q, uint64_t q_ld, const float* scale, const int32_t
 }
 
 int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* who) {
+  static_assert(sh::kKernQuantizeF16512 == sh::kKernQuantizeBf16512 + 4 &&
+                    sh::kKernQuantizeF32512 == sh::kKernQuantizeBf16512 + 8,
+                "four kernels for each type, in the order of enum sh_dtype");
+  const uint32_t width = a.cols <= 512 ? 0 : a.cols <= 2048 ? 1 : a.cols <= 4096 ? 2 : 3;
+  const uint32_t grid = width < 3 ? (a.tokens + 3) / 4 : a.tokens;
   void* args[] = {(void*)&a};
-  return sh::launch_kernel(sh::kKernQuantizeTokens, a.tokens, 256, stream, args, who);
+  return sh::launch_kernel((sh::KernelId)(sh::kKernQuantizeBf16512 + (a.dtype - SH_DTYPE_BF16) * 4 + width), grid, 256,
+                           stream, args, who);
 }
 
 int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who) {

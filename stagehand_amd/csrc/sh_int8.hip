@@ -12,12 +12,6 @@ namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float load_value(const void* p, uint64_t i, uint32_t dtype) {
-  if (dtype == SH_DTYPE_BF16) return (float)static_cast<const __bf16*>(p)[i];
-  if (dtype == SH_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return static_cast<const float*>(p)[i];
-}
-
 __device__ __forceinline__ void store_value(void* p, uint64_t i, float v, uint32_t dtype) {
   if (dtype == SH_DTYPE_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
   else if (dtype == SH_DTYPE_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
@@ -40,44 +34,183 @@ __device__ __forceinline__ void token_scale(uint32_t amax_bits, float* inv, floa
   }
 }
 
-// |x * inv| is at most 127 (1 + 2^-23), which rounds to 127. inv = 0 stands for a token without values:
-// a NaN or an infinity times 0 must give 0, not a NaN.
-__device__ __forceinline__ int32_t quantize(float x, float inv) {
-  return inv == 0.0f ? 0 : (int32_t)__builtin_rintf(x * inv);
+// ── quantisation ──────────────────────────────────────────────────────────
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+
+// Eight consecutive values of a token as they lie in memory. gfx950 loads 16 bytes from any address.
+template <typename T>
+struct Chunk {
+  static constexpr uint32_t kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const T* p, uint32_t count) {
+    if (count >= 8) {
+#pragma unroll
+      for (uint32_t i = 0; i < kWords / 4; ++i) {
+        const u32x4 v = *(reinterpret_cast<const u32x4_a2*>(p) + i);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) w[i * 4 + j] = v[j];
+      }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kWords; ++i) w[i] = 0;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (i < count) w[i] = __builtin_bit_cast(uint32_t, p[i]);
+      } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (i < count) w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << (i % 2 * 16);
+      }
+    }
+  }
+
+  // The largest of m and the magnitudes' bits (16-bit types: two maxima side by side). Bits order as
+  // magnitudes do, with infinities and NaNs last: a maximum of floats would pass over a NaN.
+  __device__ __forceinline__ uint32_t amax(uint32_t m) const {
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        m = max(m, w[i] & 0x7FFFFFFFu);
+      } else {
+        const u16x2 v = __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu);
+        m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), v));
+      }
+    }
+    return m;
+  }
+
+  __device__ __forceinline__ float value(uint32_t i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, w[i]);
+    else if constexpr (__is_same(T, __bf16))
+      return __builtin_bit_cast(float, i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
+    else return (float)__builtin_bit_cast(T, (uint16_t)(w[i / 2] >> (i % 2 * 16)));
+  }
+
+  // rint(x * inv) of the eight values as bytes. |x * inv| is at most 127 (1 + 2^-23): added to 1.5 * 2^23 it is
+  // rounded to an integer, ties to even, that the sum's low byte holds. `mask` is 0 for a token of zeros or
+  // with a NaN or an infinity, else all ones.
+  __device__ __forceinline__ uint2 quantize(float inv, uint32_t mask) const {
+#pragma clang fp contract(off)  // the product is rounded before the sum
+    uint32_t b[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const float p = value(i) * inv;
+      b[i] = __builtin_bit_cast(uint32_t, p + 12582912.0f);
+    }
+    uint2 q;
+    q.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u), __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), 0x05040100u) & mask;
+    q.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[7], b[6], 0x0C0C0400u), __builtin_amdgcn_perm(b[5], b[4], 0x0C0C0400u), 0x05040100u) & mask;
+    return q;
+  }
+};
+
+// The bits of the larger float magnitude from amax()'s word.
+template <typename T>
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  const uint32_t h = max(m & 0xFFFFu, m >> 16);
+  if constexpr (__is_same(T, __bf16)) return h << 16;
+  return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, (uint16_t)h));
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+  return v;
+}
+
+__device__ __forceinline__ int32_t wave_sum(int32_t v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+// WAVES wavefronts per token, C chunks of each work-item in registers between the maximum and the rounding:
+// the token is read once if its cols are at most WAVES * 512 * C, else its end is read twice (the second time
+// out of a cache).
+template <typename T, uint32_t WAVES, uint32_t C>
+__device__ __forceinline__ void quantize_body(const sh::QuantizeArgs& a) {
+  constexpr uint32_t kWide = WAVES * 64;  // chunks side by side
+  const uint32_t wave = threadIdx.x / 64;
+  const uint32_t t = WAVES == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const uint32_t me = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+  if (WAVES == 1 && t >= a.tokens) return;
+  const T* x = static_cast<const T*>(a.x) + (uint64_t)t * a.x_ld;
+  const uint32_t chunks = (uint32_t)(a.q_ld / 8);  // past cols they are zeros
+  auto left = [&](uint32_t c) { return c * 8 < a.cols ? a.cols - c * 8 : 0; };
+  Chunk<T> held[C];
+  uint32_t m = 0;
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) held[j].load(x + (uint64_t)(j * kWide + me) * 8, left(j * kWide + me));
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) m = held[j].amax(m);
+  for (uint32_t c = C * kWide + me; c < chunks; c += kWide) {
+    Chunk<T> v;
+    v.load(x + (uint64_t)c * 8, left(c));
+    m = v.amax(m);
+  }
+  m = wave_max(amax_bits<T>(m));
+  __shared__ uint32_t part[4];
+  __shared__ int32_t part_sum[4];
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) part[wave] = m;
+    __syncthreads();
+    m = max(max(part[0], part[1]), max(part[2], part[3]));
+  }
+  float inv, scale;
+  token_scale(m, &inv, &scale);
+  const uint32_t mask = inv == 0.0f ? 0u : ~0u;
+  uint2* q = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + (uint64_t)t * a.q_ld);
+  int32_t sum = 0;
+  auto put = [&](const Chunk<T>& v, uint32_t c) {
+    const uint2 b = v.quantize(inv, mask);
+    sum = __builtin_amdgcn_sdot4((int)b.x, 0x01010101, sum, false);
+    sum = __builtin_amdgcn_sdot4((int)b.y, 0x01010101, sum, false);
+    q[c] = b;
+  };
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j)
+    if (j * kWide + me < chunks) put(held[j], j * kWide + me);
+  for (uint32_t c = C * kWide + me; c < chunks; c += kWide) {
+    Chunk<T> v;
+    v.load(x + (uint64_t)c * 8, left(c));
+    put(v, c);
+  }
+  sum = wave_sum(sum);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & 63) == 0) part_sum[wave] = sum;
+    __syncthreads();
+    sum = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3];
+  }
+  if (me == 0) {
+    a.scale[t] = scale;
+    if (a.sums != nullptr) a.sums[t] = sum;
+  }
 }
 
 }  // namespace
 
-// One workgroup of 256 per token.
-extern "C" __global__ __launch_bounds__(256) void sh_quantize_tokens_kernel(sh::QuantizeArgs a) {
-  __shared__ uint32_t part[4];
-  __shared__ int32_t part_sum[4];
-  const uint64_t t = blockIdx.x;
-  const uint64_t at = t * a.x_ld;
-  uint32_t amax = 0;
-  for (uint32_t i = threadIdx.x; i < a.cols; i += 256)
-    amax = max(amax, __builtin_bit_cast(uint32_t, load_value(a.x, at + i, a.dtype)) & 0x7FFFFFFFu);
-  for (int m = 32; m >= 1; m >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, m));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x / 64] = amax;
-  __syncthreads();
-  amax = max(max(part[0], part[1]), max(part[2], part[3]));
-  float inv, scale;
-  token_scale(amax, &inv, &scale);
-  int8_t* q = static_cast<int8_t*>(a.q) + t * a.q_ld;
-  int32_t sum = 0;
-  for (uint32_t i = threadIdx.x; i < a.q_ld; i += 256) {
-    const int32_t v = i < a.cols ? quantize(load_value(a.x, at + i, a.dtype), inv) : 0;
-    q[i] = (int8_t)v;
-    sum += v;
+#define SH_QUANTIZE(name, T)                                                                              \
+  extern "C" __global__ __launch_bounds__(256) void sh_quantize_##name##_512_kernel(sh::QuantizeArgs a) {  \
+    quantize_body<T, 1, 1>(a);                                                                            \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void sh_quantize_##name##_2048_kernel(sh::QuantizeArgs a) { \
+    quantize_body<T, 1, 4>(a);                                                                            \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void sh_quantize_##name##_4096_kernel(sh::QuantizeArgs a) { \
+    quantize_body<T, 1, 8>(a);                                                                            \
+  }                                                                                                       \
+  extern "C" __global__ __launch_bounds__(256) void sh_quantize_##name##_16384_kernel(sh::QuantizeArgs a) { \
+    quantize_body<T, 4, 8>(a);                                                                            \
   }
-  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
-  if ((threadIdx.x & 63) == 0) part_sum[threadIdx.x / 64] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    a.scale[t] = scale;
-    if (a.sums != nullptr) a.sums[t] = part_sum[0] + part_sum[1] + part_sum[2] + part_sum[3];
-  }
-}
+SH_QUANTIZE(bf16, __bf16)
+SH_QUANTIZE(f16, _Float16)
+SH_QUANTIZE(f32, float)
 
 // ── the tiled product ─────────────────────────────────────────────────────
 

@@ -90,7 +90,19 @@ enum KernelId : int {
   kKernDigestWide,
   kKernDigestCompare,
   kKernDigestCompareWide,
-  kKernQuantizeTokens,
+  // int8: one quantisation per type and columns held in registers, in this order
+  kKernQuantizeBf16512,
+  kKernQuantizeBf162048,
+  kKernQuantizeBf164096,
+  kKernQuantizeBf1616384,
+  kKernQuantizeF16512,
+  kKernQuantizeF162048,
+  kKernQuantizeF164096,
+  kKernQuantizeF1616384,
+  kKernQuantizeF32512,
+  kKernQuantizeF322048,
+  kKernQuantizeF324096,
+  kKernQuantizeF3216384,
   kKernMatmulI8,
   kKernMatmulI8Tile256,
   kKernQkNormRope,

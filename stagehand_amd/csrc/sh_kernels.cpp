@@ -68,7 +68,18 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModDigest, "sh_digest_wide_kernel"},
     {kModDigest, "sh_digest_compare_kernel"},
     {kModDigest, "sh_digest_compare_wide_kernel"},
-    {kModInt8, "sh_quantize_tokens_kernel"},
+    {kModInt8, "sh_quantize_bf16_512_kernel"},
+    {kModInt8, "sh_quantize_bf16_2048_kernel"},
+    {kModInt8, "sh_quantize_bf16_4096_kernel"},
+    {kModInt8, "sh_quantize_bf16_16384_kernel"},
+    {kModInt8, "sh_quantize_f16_512_kernel"},
+    {kModInt8, "sh_quantize_f16_2048_kernel"},
+    {kModInt8, "sh_quantize_f16_4096_kernel"},
+    {kModInt8, "sh_quantize_f16_16384_kernel"},
+    {kModInt8, "sh_quantize_f32_512_kernel"},
+    {kModInt8, "sh_quantize_f32_2048_kernel"},
+    {kModInt8, "sh_quantize_f32_4096_kernel"},
+    {kModInt8, "sh_quantize_f32_16384_kernel"},
     {kModInt8, "sh_matmul_i8_kernel"},
     {kModInt8, "sh_matmul_i8_256_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_kernel"},
