@@ -3,6 +3,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "sh_int8_args.h"
@@ -79,19 +81,35 @@ int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* w
                            stream, args, who);
 }
 
-int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who) {
-  if (a.tokens > 128) {
-    const uint64_t grid = (((uint64_t)a.tokens + 255) / 256) * (((uint64_t)a.rows + 255) / 256);
-    if (grid > 0xFFFFFFFFull / 512) return sh::fail(SH_ERR_INVALID, "%s: %u tokens x %u rows are too many for one launch", who, a.tokens, a.rows);
-    void* args[] = {(void*)&a};
-    return sh::launch_kernel(sh::kKernMatmulI8Tile256, (uint32_t)grid, 512, stream, args, who);
+// The tile of the least estimated time: rounds of tiles over the 256 compute units, times what 128 columns of
+// one round take (MI355X, measured over 64 to 1500 tiles of 3072 and 4096 columns). Larger tiles read LDS and the
+// caches less for each product (256 x 256: 2500 TOPS; 64 x 64: 1000), smaller ones leave fewer compute units
+// idle. Around the switches, 4096 x 4096 weights unless said: 64 tokens 8.6 us with 32x32, 11 with 64x64; 128 x
+// 9216 x 3072: 13.1 with 64x64, 20.8 with 32x32, 15 with 128x128; 1024 tokens 21 with 128x128, 24 with 128x256, 45
+// with 256x256; 512 x 9216 x 3072: 21.6 with 128x256, 29 with 128x128, 38 with 256x256; 2048 tokens 34 with
+// 128x256, 60 with 256x256; 1024 x 12288 x 3072: 41 with 256x256, 45 with 128x256.
+int choose_tile(uint32_t tokens, uint32_t rows) {
+  int best = 0;
+  double best_cost = 0;
+  for (int i = 0; i < sh::kMatmulTileCount; ++i) {
+    const sh::MatmulTile& m = sh::kMatmulTiles[i];
+    const double tiles = (double)((tokens + (uint64_t)m.tokens - 1) / m.tokens) * ((rows + (uint64_t)m.rows - 1) / m.rows);
+    const double rounds = m.fractional ? std::max(1.0, tiles / 256) : std::ceil(tiles / 256);
+    const double cost = rounds * m.cost;
+    if (i == 0 || cost < best_cost) best = i, best_cost = cost;
   }
-  const uint64_t tiles = ((uint64_t)a.tokens + 15) / 16 * (((uint64_t)a.rows + 63) / 64);
-  const uint64_t grid = (tiles + 3) / 4;
-  if (grid > 0xFFFFFFFFull / 256)
+  return best;
+}
+
+int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who) {
+  const int i = choose_tile(a.tokens, a.rows);
+  const sh::MatmulTile& m = sh::kMatmulTiles[i];
+  const uint64_t grid = ((uint64_t)a.tokens + m.tokens - 1) / m.tokens * (((uint64_t)a.rows + m.rows - 1) / m.rows);
+  if (grid > 0xFFFFFFFFull / m.threads)
     return sh::fail(SH_ERR_INVALID, "%s: %u tokens x %u rows are too many for one launch", who, a.tokens, a.rows);
   void* args[] = {(void*)&a};
-  return sh::launch_kernel(sh::kKernMatmulI8, (uint32_t)grid, 256, stream, args, who);
+  static_assert(sh::kKernMatmulI8256x256 - sh::kKernMatmulI816x16 == sh::kMatmulTileCount - 1, "one kernel per tile");
+  return sh::launch_kernel((sh::KernelId)(sh::kKernMatmulI816x16 + i), (uint32_t)grid, m.threads, stream, args, who);
 }
 
 struct Workspace {

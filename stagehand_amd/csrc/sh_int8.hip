@@ -12,12 +12,6 @@ namespace {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void store_value(void* p, uint64_t i, float v, uint32_t dtype) {
-  if (dtype == SH_DTYPE_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else if (dtype == SH_DTYPE_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
-  else static_cast<float*>(p)[i] = v;
-}
-
 // A token's factor 127 / a and scale a / 127 from the bits of a = max |x|. The bits order as the
 // values do, with infinities and NaNs last, so their maximum finds a NaN too.
 __device__ __forceinline__ void token_scale(uint32_t amax_bits, float* inv, float* scale) {
@@ -218,6 +212,7 @@ namespace {
 
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
+constexpr uint32_t kPastEnd = 0x80000000u;  // an offset outside every resource
 constexpr uint32_t kStep = 128;  // bytes of a row that one stage holds: a cache line, two MFMAs'
 
 // The 16-byte chunk c of a stage's row lies in slot c ^ swizzle(row): the 16 rows of a fragment then lie in
@@ -245,33 +240,28 @@ __device__ __forceinline__ void load_to_lds(i32x4_t r, uint32_t lds, uint32_t of
                "s"(r));
 }
 
-struct alignas(16) Words4 {
-  uint32_t w[4];
-};
-
-// Stores 16 consecutive values; `whole`: all of them lie in the row, at a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void store_run(T* out, const float (&v)[16], bool whole, uint32_t count) {
+// Stores N consecutive values; `whole`: all of them lie in the row, at a multiple of 16 bytes (or of all N).
+template <typename T, uint32_t N>
+__device__ __forceinline__ void store_run(T* out, const float (&v)[N], bool whole, uint32_t count) {
+  constexpr uint32_t kPer = N * sizeof(T) < 16 ? N : 16 / sizeof(T);
+  typedef T Run __attribute__((ext_vector_type(kPer)));
   if (whole) {
-    constexpr uint32_t kPer = 16 / sizeof(T);
 #pragma unroll
-    for (uint32_t i = 0; i < 16 / kPer; ++i) {
-      Words4 w;
-      T x[kPer];
+    for (uint32_t i = 0; i < N / kPer; ++i) {
+      Run x;
 #pragma unroll
       for (uint32_t j = 0; j < kPer; ++j) x[j] = (T)v[i * kPer + j];
-      __builtin_memcpy(&w, x, 16);
-      *reinterpret_cast<Words4*>(out + i * kPer) = w;
+      *reinterpret_cast<Run*>(out + i * kPer) = x;
     }
   } else {
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j)
+    for (uint32_t j = 0; j < N; ++j)
       if (j < count) out[j] = (T)v[j];
   }
 }
 
-// TT tokens x TN rows by WT x WN wavefronts, each with FT x FN MFMA tiles.
-template <uint32_t TT, uint32_t TN, uint32_t WT, uint32_t WN>
+// TT tokens x TN rows by WT x WN wavefronts, each with FT x FN MFMA tiles; D stages.
+template <uint32_t TT, uint32_t TN, uint32_t WT, uint32_t WN, uint32_t D>
 __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* lds) {
   constexpr uint32_t kStage = (TT + TN) * kStep;
   constexpr uint32_t kWaves = WT * WN;
@@ -342,34 +332,35 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
       __builtin_amdgcn_sched_group_barrier(0x8, FT * FN / (FT + FN), 0);
     }
   };
-  // Two stages. The fragments of a half stage are read into registers while the half before is multiplied, so
-  // a stage is read to its end when the first half of its products is done: the loads of the stage after the
-  // next start there and have one stage's products to land in.
-  // Each wavefront waits for its own loads, then the barrier says that everyone's have landed and that
-  // everyone has read the stage whose place the next loads take.
+  // A ring of D stages. The fragments of a half stage are read into registers while the half before is
+  // multiplied, so a stage is read to its end when the first half of its products is done: the loads of the
+  // stage D after it start there and have the products of D - 1 stages to land in.
+  // Each wavefront waits for its own loads of the next stage, then the barrier says that everyone's have landed
+  // and that everyone has read the stage whose place the next loads take. Past the end the offsets are outside
+  // the resources: such loads read nothing and keep the count of loads in flight the same.
   const uint32_t end = (uint32_t)a.t_ld;  // a multiple of kStep; the tokens are zero past cols
-  auto landed = [&] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
   Fragments f0, f1;
-  load(0, 0);
-  landed();
-  if (kStep < end) load(1, kStep);
+#pragma unroll
+  for (uint32_t i = 0; i < D; ++i) load(i, i * kStep < end ? i * kStep : kPastEnd);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (LT + LN)) : "memory");
+  __syncthreads();
   read(f0, 0, 0);
   uint32_t s = 0;
   for (uint32_t k = kStep; k < end; k += kStep) {
     read(f1, s, 1);
     multiply(f0);
-    landed();
-    if (k + kStep < end) load(s, k + kStep);
-    s ^= 1;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * (LT + LN)) : "memory");
+    __syncthreads();
+    const uint32_t next = k + (D - 1) * kStep;
+    load(s, next < end ? next : kPastEnd);
+    s = s == D - 1 ? 0 : s + 1;
     read(f0, s, 0);
     multiply(f1);
   }
   read(f1, s, 1);
   multiply(f0);
   multiply(f1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may outlive the workgroup
 
   // lane: token t0 + .. + l16 of each token fragment, 16 consecutive rows
   const uint32_t n = n0 + wn * (TN / WN) + part * 16;
@@ -405,51 +396,120 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(512, 2) void sh_matmul_i8_256_kernel(sh::MatmulI8Args a) {
-  __shared__ uint8_t lds[2 * 512 * kStep];
-  matmul_tile<256, 256, 2, 4>(a, lds);
-}
+// ── the product for few tokens ────────────────────────────────────────────
 
-// Each wavefront: 16 tokens x 64 rows, operands straight from global memory. In a 16x16x64 MFMA lane
-// l gives row l % 16 of each operand, bytes (l / 16) * 16 .. + 15, and holds elements (l / 16) * 4 + r
-// of the first operand's rows for column l % 16 of the second's.
-extern "C" __global__ __launch_bounds__(256) void sh_matmul_i8_kernel(sh::MatmulI8Args a) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-  const uint32_t row_tiles = (a.rows + 63) / 64;
-  const uint64_t tile = (uint64_t)blockIdx.x * 4 + wave;
-  const uint32_t t0 = (uint32_t)(tile / row_tiles) * 16, n0 = (uint32_t)(tile % row_tiles) * 64;
-  if (t0 >= a.tokens) return;
+namespace {
+
+// 16 FT tokens x 16 FN rows by W wavefronts, each with every W-th 128 columns. A wavefront keeps a ring of D
+// stages of its own in LDS (tokens, then rows), so nothing waits for another wavefront until the sums are
+// joined at the end.
+template <uint32_t FT, uint32_t FN, uint32_t W, uint32_t D>
+__device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t* lds) {
+  constexpr uint32_t kStage = (FT + FN) * 16 * kStep;
+  constexpr uint32_t kLoads = 2 * (FT + FN);  // of 8 rows each
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t tiles_n = (a.rows + 16 * FN - 1) / (16 * FN);
+  const uint32_t t0 = blockIdx.x / tiles_n * (16 * FT), n0 = blockIdx.x % tiles_n * (16 * FN);
+  const i32x4_t tr = rows_resource(a.tq, a.t_ld, t0, a.tokens, 16 * FT);
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, 16 * FN);
+  // row + 8 has the swizzle of row with bit 2 changed: two offsets cover every load
+  const uint32_t row = lane / 8, slot = lane % 8;
+  const uint32_t s0 = (slot ^ swizzle(row)) * 16, s1 = (slot ^ swizzle(row + 8)) * 16;
+  const uint32_t t_ld = (uint32_t)a.t_ld, w_ld = (uint32_t)a.w_ld;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * D * kStage;
+  auto load = [&](uint32_t stage, uint32_t k) {
+#pragma unroll
+    for (uint32_t j = 0; j < 2 * FN; ++j)
+      load_to_lds(wr, lds0 + stage * kStage + (2 * FT + j) * 1024, (row + j * 8) * w_ld + (j % 2 ? s1 : s0) + k);
+#pragma unroll
+    for (uint32_t j = 0; j < 2 * FT; ++j)
+      load_to_lds(tr, lds0 + stage * kStage + j * 1024, (row + j * 8) * t_ld + (j % 2 ? s1 : s0) + k);
+  };
   const uint32_t l16 = lane & 15, part = lane / 16;
-  const uint32_t t = min(t0 + l16, a.tokens - 1);
-  const int8_t* tp = static_cast<const int8_t*>(a.tq) + (uint64_t)t * a.t_ld + part * 16;
-  const int8_t* wp[4];
-  for (uint32_t f = 0; f < 4; ++f)
-    wp[f] = static_cast<const int8_t*>(a.wq) + (uint64_t)min(n0 + f * 16 + l16, a.rows - 1) * a.w_ld + part * 16;
-  i32x4 acc[4] = {};
-  for (uint32_t k = 0; k < a.cols; k += 64) {
-    // the tokens' rows are zero-filled to a multiple of 128; the weight's end at a multiple of 16
-    const i32x4 tv = *reinterpret_cast<const i32x4*>(tp + k);
+  const uint8_t* mine = lds + wave * D * kStage + l16 * kStep;
+  i32x4_t acc[FT][FN] = {};
+  const uint32_t end = t_ld;
 #pragma unroll
-    for (uint32_t f = 0; f < 4; ++f) {
-      i32x4 wv = {};
-      if (k + part * 16 < a.cols) wv = *reinterpret_cast<const i32x4*>(wp[f] + k);
-      acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, tv, acc[f], 0, 0, 0);
-    }
+  for (uint32_t i = 0; i < D; ++i) {
+    const uint32_t k = (i * W + wave) * kStep;
+    load(i, k < end ? k : kPastEnd);
   }
-  if (t0 + l16 >= a.tokens) return;
-  const float ts = a.t_scale[t];
-  const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
+  uint32_t s = 0;
+  for (uint32_t k = wave * kStep; k < end; k += W * kStep) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
+    i32x4_t tf[2][FT], nf[2][FN];
 #pragma unroll
-  for (uint32_t f = 0; f < 4; ++f) {
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint8_t* at = mine + s * kStage + ((h * 4 + part) ^ swizzle(l16)) * 16;
+#pragma unroll
+      for (uint32_t i = 0; i < FT; ++i) tf[h][i] = *reinterpret_cast<const i32x4_t*>(at + i * 16 * kStep);
+#pragma unroll
+      for (uint32_t j = 0; j < FN; ++j) nf[h][j] = *reinterpret_cast<const i32x4_t*>(at + (FT + j) * 16 * kStep);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the place is loaded again
+    const uint32_t next = k + D * W * kStep;
+    load(s, next < end ? next : kPastEnd);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+      for (uint32_t i = 0; i < FT; ++i)
+#pragma unroll
+        for (uint32_t j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(nf[h][j], tf[h][i], acc[i][j], 0, 0, 0);
+    s = s == D - 1 ? 0 : s + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may land on the sums below
+  __syncthreads();
+  i32x4_t* sums = reinterpret_cast<i32x4_t*>(lds);
+#pragma unroll
+  for (uint32_t i = 0; i < FT; ++i)
+#pragma unroll
+    for (uint32_t j = 0; j < FN; ++j) sums[((i * FN + j) * W + wave) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
+  for (uint32_t f = wave; f < FT * FN; f += W) {
+    i32x4_t v = sums[f * W * 64 + lane];
+#pragma unroll
+    for (uint32_t w = 1; w < W; ++w) v += sums[(f * W + w) * 64 + lane];
+    const uint32_t t = t0 + f / FN * 16 + l16, n = n0 + f % FN * 16 + part * 4;
+    if (t >= a.tokens || n >= a.rows) continue;
+    const float scale = a.t_scale[t];
+    const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
+    const uint32_t count = min(a.rows - n, 4u);
+    float y[4];
 #pragma unroll
     for (uint32_t r = 0; r < 4; ++r) {
-      const uint32_t n = n0 + f * 16 + part * 4 + r;
-      if (n >= a.rows) continue;
-      float v = (float)acc[f][r];
-      if (a.w_zp != nullptr) v = __builtin_fmaf(-a.w_zp[n], sum, v);
-      v *= ts * a.w_scale[n];
-      if (a.bias != nullptr) v += a.bias[n];
-      store_value(a.out, (uint64_t)t * a.out_ld + n, v, a.out_dtype);
+      const bool in = r < count;
+      const float ws = in ? a.w_scale[n + r] : 0.0f;
+      const float wz = in && a.w_zp != nullptr ? a.w_zp[n + r] : 0.0f;
+      const float wb = in && a.bias != nullptr ? a.bias[n + r] : 0.0f;
+      y[r] = __builtin_fmaf(-wz, sum, (float)v[r]) * (scale * ws) + wb;
     }
+    const uint64_t at = (uint64_t)t * a.out_ld + n;
+    const bool whole = count == 4 && ((uintptr_t)a.out | a.out_ld * bytes) % (4 * bytes) == 0;
+    if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, whole, count);
+    else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, y, whole, count);
+    else store_run(static_cast<float*>(a.out) + at, y, whole, count);
   }
 }
+
+}  // namespace
+
+// The tiles of sh_int8_args.h.
+#define SH_MATMUL_FEW(name, FT, FN, W, D)                                                                     \
+  extern "C" __global__ __launch_bounds__(W * 64) void sh_matmul_i8_##name##_kernel(sh::MatmulI8Args a) {      \
+    __shared__ alignas(16) uint8_t lds[W * D * (FT + FN) * 16 * kStep];                                       \
+    matmul_skinny<FT, FN, W, D>(a, lds);                                                                      \
+  }
+#define SH_MATMUL_TILE(name, TT, TN, WT, WN, D)                                                               \
+  extern "C" __global__ __launch_bounds__(WT * WN * 64) void sh_matmul_i8_##name##_kernel(sh::MatmulI8Args a) { \
+    __shared__ alignas(16) uint8_t lds[D * (TT + TN) * kStep];                                                \
+    matmul_tile<TT, TN, WT, WN, D>(a, lds);                                                                   \
+  }
+SH_MATMUL_FEW(16x16, 1, 1, 8, 3)
+SH_MATMUL_FEW(16x32, 1, 2, 4, 3)
+SH_MATMUL_FEW(32x32, 2, 2, 4, 2)
+SH_MATMUL_TILE(64x64, 64, 64, 4, 1, 3)
+SH_MATMUL_TILE(128x128, 128, 128, 4, 2, 3)
+SH_MATMUL_TILE(128x256, 128, 256, 4, 4, 3)
+SH_MATMUL_TILE(256x256, 256, 256, 2, 4, 2)

@@ -36,4 +36,16 @@ struct MatmulI8Args {
   uint32_t out_dtype;
 };
 
+// The product's kernels, smallest tile first.
+struct MatmulTile {
+  uint32_t tokens, rows, threads;
+  uint32_t cost;   // of 128 columns on a full chip, in 10 ns
+  bool fractional;  // several workgroups share a compute unit: a last round that is not full costs its share
+};
+constexpr MatmulTile kMatmulTiles[] = {
+    {16, 16, 512, 11, true},    {16, 32, 256, 15, true},     {32, 32, 256, 19, true},     {64, 64, 256, 30, true},
+    {128, 128, 512, 62, false}, {128, 256, 1024, 100, false}, {256, 256, 512, 175, false},
+};
+constexpr int kMatmulTileCount = sizeof(kMatmulTiles) / sizeof(kMatmulTiles[0]);
+
 }  // namespace sh

@@ -103,8 +103,14 @@ enum KernelId : int {
   kKernQuantizeF322048,
   kKernQuantizeF324096,
   kKernQuantizeF3216384,
-  kKernMatmulI8,
-  kKernMatmulI8Tile256,
+  // one product per tile of sh_int8_args.h, in this order
+  kKernMatmulI816x16,
+  kKernMatmulI816x32,
+  kKernMatmulI832x32,
+  kKernMatmulI864x64,
+  kKernMatmulI8128x128,
+  kKernMatmulI8128x256,
+  kKernMatmulI8256x256,
   kKernQkNormRope,
   kKernQkNormRopeBackward,
   kKernQkNormDweight,

@@ -80,8 +80,13 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModInt8, "sh_quantize_f32_2048_kernel"},
     {kModInt8, "sh_quantize_f32_4096_kernel"},
     {kModInt8, "sh_quantize_f32_16384_kernel"},
-    {kModInt8, "sh_matmul_i8_kernel"},
-    {kModInt8, "sh_matmul_i8_256_kernel"},
+    {kModInt8, "sh_matmul_i8_16x16_kernel"},
+    {kModInt8, "sh_matmul_i8_16x32_kernel"},
+    {kModInt8, "sh_matmul_i8_32x32_kernel"},
+    {kModInt8, "sh_matmul_i8_64x64_kernel"},
+    {kModInt8, "sh_matmul_i8_128x128_kernel"},
+    {kModInt8, "sh_matmul_i8_128x256_kernel"},
+    {kModInt8, "sh_matmul_i8_256x256_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_backward_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
