@@ -112,6 +112,11 @@ int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who
   return sh::launch_kernel((sh::KernelId)(sh::kKernMatmulI816x16 + i), (uint32_t)grid, m.threads, stream, args, who);
 }
 
+// Whether the tokens are few enough for every workgroup to quantise them for itself.
+bool in_one_launch(uint32_t tokens, uint32_t cols) {
+  return tokens <= 16 && (uint64_t)tokens * ((cols + 511) / 512) <= sh::kFewPieces;
+}
+
 struct Workspace {
   uint64_t q_ld, sums, scale, bytes;
 };
@@ -119,6 +124,7 @@ struct Workspace {
 // q, then the scales, then the sums.
 Workspace workspace_of(uint32_t tokens, uint32_t cols) {
   Workspace s{};
+  if (in_one_launch(tokens, cols)) return s;
   s.q_ld = token_ld(cols);
   s.scale = s.q_ld * tokens;
   s.sums = s.scale + 4ull * tokens;
@@ -176,6 +182,19 @@ extern "C" int sh_linear_i8(const void* x, uint32_t dtype, uint64_t x_ld, uint32
     return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
                     (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
   if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+  if (in_one_launch(tokens, w->cols)) {
+    const bool wide = w->rows > 32 * 256 - 32;  // 32 rows a workgroup leave no compute unit idle
+    const uint32_t grid = wide ? (w->rows + 31) / 32 : (w->rows + 15) / 16;
+    if (grid > 0xFFFFFFFFu / 512) return sh::fail(SH_ERR_INVALID, "%s: %u rows are too many for one launch", who, w->rows);
+    const sh::MatmulI8Args a{x,    nullptr, nullptr, w->q,   w->scale, w->zero_point, w->bias, out,
+                             x_ld, w->ld,   out_ld,  tokens, w->rows,  w->cols,       dtype};
+    void* args[] = {(void*)&a};
+    static_assert(sh::kKernLinearI8F1616x16 == sh::kKernLinearI8Bf1616x16 + 2 &&
+                      sh::kKernLinearI8F3216x16 == sh::kKernLinearI8Bf1616x16 + 4,
+                  "two kernels for each type, in the order of enum sh_dtype");
+    return sh::launch_kernel((sh::KernelId)(sh::kKernLinearI8Bf1616x16 + (dtype - SH_DTYPE_BF16) * 2 + wide), grid,
+                             wide ? 256 : 512, (hipStream_t)stream, args, who);
+  }
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float* scale = reinterpret_cast<float*>(ws + s.scale);
   int32_t* sums = reinterpret_cast<int32_t*>(ws + s.sums);

@@ -400,6 +400,32 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
 
 namespace {
 
+// Joins the W wavefronts' sums of rows n .. n + 3 for token t (64 entries apart) and stores the outputs.
+template <uint32_t W>
+__device__ __forceinline__ void store_joined(const sh::MatmulI8Args& a, const i32x4_t* sums, uint32_t t, uint32_t n,
+                                             float scale, int32_t t_sum) {
+  if (n >= a.rows) return;
+  i32x4_t v = sums[0];
+#pragma unroll
+  for (uint32_t w = 1; w < W; ++w) v += sums[w * 64];
+  const uint32_t count = min(a.rows - n, 4u);
+  float y[4];
+#pragma unroll
+  for (uint32_t r = 0; r < 4; ++r) {
+    const bool in = r < count;
+    const float ws = in ? a.w_scale[n + r] : 0.0f;
+    const float wz = in && a.w_zp != nullptr ? a.w_zp[n + r] : 0.0f;
+    const float wb = in && a.bias != nullptr ? a.bias[n + r] : 0.0f;
+    y[r] = __builtin_fmaf(-wz, (float)t_sum, (float)v[r]) * (scale * ws) + wb;
+  }
+  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
+  const uint64_t at = (uint64_t)t * a.out_ld + n;
+  const bool whole = count == 4 && ((uintptr_t)a.out | a.out_ld * bytes) % (4 * bytes) == 0;
+  if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, whole, count);
+  else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, y, whole, count);
+  else store_run(static_cast<float*>(a.out) + at, y, whole, count);
+}
+
 // 16 FT tokens x 16 FN rows by W wavefronts, each with every W-th 128 columns. A wavefront keeps a ring of D
 // stages of its own in LDS (tokens, then rows), so nothing waits for another wavefront until the sums are
 // joined at the end.
@@ -466,34 +492,145 @@ __device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t
 #pragma unroll
     for (uint32_t j = 0; j < FN; ++j) sums[((i * FN + j) * W + wave) * 64 + lane] = acc[i][j];
   __syncthreads();
-  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
   for (uint32_t f = wave; f < FT * FN; f += W) {
-    i32x4_t v = sums[f * W * 64 + lane];
-#pragma unroll
-    for (uint32_t w = 1; w < W; ++w) v += sums[(f * W + w) * 64 + lane];
     const uint32_t t = t0 + f / FN * 16 + l16, n = n0 + f % FN * 16 + part * 4;
-    if (t >= a.tokens || n >= a.rows) continue;
-    const float scale = a.t_scale[t];
-    const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
-    const uint32_t count = min(a.rows - n, 4u);
-    float y[4];
-#pragma unroll
-    for (uint32_t r = 0; r < 4; ++r) {
-      const bool in = r < count;
-      const float ws = in ? a.w_scale[n + r] : 0.0f;
-      const float wz = in && a.w_zp != nullptr ? a.w_zp[n + r] : 0.0f;
-      const float wb = in && a.bias != nullptr ? a.bias[n + r] : 0.0f;
-      y[r] = __builtin_fmaf(-wz, sum, (float)v[r]) * (scale * ws) + wb;
-    }
-    const uint64_t at = (uint64_t)t * a.out_ld + n;
-    const bool whole = count == 4 && ((uintptr_t)a.out | a.out_ld * bytes) % (4 * bytes) == 0;
-    if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, whole, count);
-    else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, y, whole, count);
-    else store_run(static_cast<float*>(a.out) + at, y, whole, count);
+    if (t >= a.tokens) continue;
+    store_joined<W>(a, sums + f * W * 64 + lane, t, n, a.t_scale[t], a.w_zp != nullptr ? a.t_sums[t] : 0);
   }
 }
 
 }  // namespace
+
+// ── a few tokens, quantised where they are multiplied ─────────────────────
+
+namespace {
+
+// As matmul_skinny for up to 16 tokens, which every workgroup quantises for itself into LDS: one launch, and the
+// weight is on its way meanwhile. A wavefront's piece of a token is 512 values; all of them, kFewPieces / W a
+// wavefront, stay in registers between maximum and rounding. In `a`, tq is the tokens as they are, t_ld their
+// distance in elements; t_scale and t_sums are not used.
+template <typename T, uint32_t FN, uint32_t W, uint32_t D>
+__device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* ring, uint8_t* tq, uint32_t* amax,
+                                           int32_t* sum) {
+  constexpr uint32_t kStage = FN * 16 * kStep;
+  constexpr uint32_t kLoads = 2 * FN;
+  constexpr uint32_t kMine = sh::kFewPieces / W;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t n0 = blockIdx.x * (16 * FN);
+  const uint32_t end = (a.cols + kStep - 1) / kStep * kStep;
+  const uint32_t q_ld = end + 16;  // 16 bytes more: the rows of a fragment in different LDS banks
+  const uint32_t pieces = (a.cols + 511) / 512;
+
+  Chunk<T> held[kMine];
+  uint32_t token_of[kMine], at_of[kMine];
+#pragma unroll
+  for (uint32_t j = 0; j < kMine; ++j) {
+    const uint32_t item = j * W + wave;
+    // item / pieces: exact for item < 64, pieces <= 64 (the quotient's error is under 64 / 2^16)
+    const uint32_t t = item * ((65536 + pieces - 1) / pieces) >> 16, at = ((item - t * pieces) * 64 + lane) * 8;
+    token_of[j] = t;
+    at_of[j] = at;
+    if (t < a.tokens)
+      held[j].load(static_cast<const T*>(a.tq) + (uint64_t)t * a.t_ld + at, at < a.cols ? a.cols - at : 0);
+  }
+  if (threadIdx.x < 16) {
+    amax[threadIdx.x] = 0;
+    sum[threadIdx.x] = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t j = 0; j < kMine; ++j) {
+    const uint32_t t = token_of[j];
+    if (t >= a.tokens) continue;
+    const uint32_t m = wave_max(amax_bits<T>(held[j].amax(0)));
+    if (lane == 0) atomicMax(amax + t, m);
+  }
+
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, 16 * FN);
+  const uint32_t row = lane / 8, slot = lane % 8;
+  const uint32_t s0 = (slot ^ swizzle(row)) * 16, s1 = (slot ^ swizzle(row + 8)) * 16;
+  const uint32_t w_ld = (uint32_t)a.w_ld;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring + wave * D * kStage;
+  auto load = [&](uint32_t stage, uint32_t k) {
+#pragma unroll
+    for (uint32_t j = 0; j < 2 * FN; ++j)
+      load_to_lds(wr, lds0 + stage * kStage + j * 1024, (row + j * 8) * w_ld + (j % 2 ? s1 : s0) + k);
+  };
+#pragma unroll
+  for (uint32_t i = 0; i < D; ++i) {
+    const uint32_t k = (i * W + wave) * kStep;
+    load(i, k < end ? k : kPastEnd);
+  }
+
+  __syncthreads();
+#pragma unroll
+  for (uint32_t j = 0; j < kMine; ++j) {
+    const uint32_t t = token_of[j], at = at_of[j];
+    if (t >= a.tokens) continue;
+    float inv, scale;
+    token_scale(amax[t], &inv, &scale);
+    const uint2 b = held[j].quantize(inv, inv == 0.0f ? 0u : ~0u);
+    if (at < end) *reinterpret_cast<uint2*>(tq + t * q_ld + at) = b;
+    if (a.w_zp != nullptr) {
+      const int32_t v = wave_sum(__builtin_amdgcn_sdot4((int)b.y, 0x01010101, __builtin_amdgcn_sdot4((int)b.x, 0x01010101, 0, false), false));
+      if (lane == 0) atomicAdd(sum + t, v);
+    }
+  }
+  __syncthreads();
+
+  const uint32_t l16 = lane & 15, part = lane / 16;
+  const uint8_t* mine = ring + wave * D * kStage + l16 * kStep;
+  const uint8_t* token = tq + min(l16, a.tokens - 1) * q_ld + part * 16;
+  i32x4_t acc[FN] = {};
+  uint32_t s = 0;
+  for (uint32_t k = wave * kStep; k < end; k += W * kStep) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
+    i32x4_t tf[2], nf[2][FN];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+      const uint8_t* at = mine + s * kStage + ((h * 4 + part) ^ swizzle(l16)) * 16;
+      tf[h] = *reinterpret_cast<const i32x4_t*>(token + k + h * 64);
+#pragma unroll
+      for (uint32_t j = 0; j < FN; ++j) nf[h][j] = *reinterpret_cast<const i32x4_t*>(at + j * 16 * kStep);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the place is loaded again
+    const uint32_t next = k + D * W * kStep;
+    load(s, next < end ? next : kPastEnd);
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+      for (uint32_t j = 0; j < FN; ++j)
+        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(nf[h][j], tf[h], acc[j], 0, 0, 0);
+    s = s == D - 1 ? 0 : s + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may land on the sums below
+  __syncthreads();
+  i32x4_t* sums = reinterpret_cast<i32x4_t*>(ring);
+#pragma unroll
+  for (uint32_t j = 0; j < FN; ++j) sums[(j * W + wave) * 64 + lane] = acc[j];
+  __syncthreads();
+  if (wave >= FN || l16 >= a.tokens) return;
+  float inv, scale;
+  token_scale(amax[l16], &inv, &scale);
+  store_joined<W>(a, sums + wave * W * 64 + lane, l16, n0 + wave * 16 + part * 4, scale, sum[l16]);
+}
+
+}  // namespace
+
+#define SH_LINEAR_FEW(name, T, tile, FN, W, D)                                                                \
+  extern "C" __global__ __launch_bounds__(W * 64) void sh_linear_i8_##name##_##tile##_kernel(sh::MatmulI8Args a) { \
+    __shared__ alignas(16) uint8_t ring[W * D * FN * 16 * kStep];                                             \
+    __shared__ alignas(16) uint8_t tq[sh::kFewPieces * 512 + 16 * 16];                                        \
+    __shared__ uint32_t amax[16];                                                                             \
+    __shared__ int32_t sum[16];                                                                               \
+    linear_few<T, FN, W, D>(a, ring, tq, amax, sum);                                                          \
+  }
+SH_LINEAR_FEW(bf16, __bf16, 16x16, 1, 8, 3)
+SH_LINEAR_FEW(bf16, __bf16, 16x32, 2, 4, 2)
+SH_LINEAR_FEW(f16, _Float16, 16x16, 1, 8, 3)
+SH_LINEAR_FEW(f16, _Float16, 16x32, 2, 4, 2)
+SH_LINEAR_FEW(f32, float, 16x16, 1, 8, 3)
+SH_LINEAR_FEW(f32, float, 16x32, 2, 4, 2)
 
 // The tiles of sh_int8_args.h.
 #define SH_MATMUL_FEW(name, FT, FN, W, D)                                                                     \

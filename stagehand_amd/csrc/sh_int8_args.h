@@ -36,6 +36,9 @@ struct MatmulI8Args {
   uint32_t out_dtype;
 };
 
+// Pieces of 512 values that one launch quantises and multiplies (at most 16 tokens).
+constexpr uint32_t kFewPieces = 16;
+
 // The product's kernels, smallest tile first.
 struct MatmulTile {
   uint32_t tokens, rows, threads;

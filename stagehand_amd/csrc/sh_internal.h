@@ -111,6 +111,13 @@ enum KernelId : int {
   kKernMatmulI8128x128,
   kKernMatmulI8128x256,
   kKernMatmulI8256x256,
+  // quantisation and product in one, per type and tile
+  kKernLinearI8Bf1616x16,
+  kKernLinearI8Bf1616x32,
+  kKernLinearI8F1616x16,
+  kKernLinearI8F1616x32,
+  kKernLinearI8F3216x16,
+  kKernLinearI8F3216x32,
   kKernQkNormRope,
   kKernQkNormRopeBackward,
   kKernQkNormDweight,

@@ -87,6 +87,12 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModInt8, "sh_matmul_i8_128x128_kernel"},
     {kModInt8, "sh_matmul_i8_128x256_kernel"},
     {kModInt8, "sh_matmul_i8_256x256_kernel"},
+    {kModInt8, "sh_linear_i8_bf16_16x16_kernel"},
+    {kModInt8, "sh_linear_i8_bf16_16x32_kernel"},
+    {kModInt8, "sh_linear_i8_f16_16x16_kernel"},
+    {kModInt8, "sh_linear_i8_f16_16x32_kernel"},
+    {kModInt8, "sh_linear_i8_f32_16x16_kernel"},
+    {kModInt8, "sh_linear_i8_f32_16x32_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_kernel"},
     {kModQkNorm, "sh_qk_norm_rope_backward_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
