@@ -118,8 +118,43 @@ enum KernelId : int {
   kKernLinearI8F1616x32,
   kKernLinearI8F3216x16,
   kKernLinearI8F3216x32,
-  kKernQkNormRope,
-  kKernQkNormRopeBackward,
+  // query/key norms: per type and run of pairs, forward and backward, halves and interleaved
+  kKernQkNormBf168,
+  kKernQkNormBf168Interleaved,
+  kKernQkNormBackwardBf168,
+  kKernQkNormBackwardBf168Interleaved,
+  kKernQkNormBf162,
+  kKernQkNormBf162Interleaved,
+  kKernQkNormBackwardBf162,
+  kKernQkNormBackwardBf162Interleaved,
+  kKernQkNormBf161,
+  kKernQkNormBf161Interleaved,
+  kKernQkNormBackwardBf161,
+  kKernQkNormBackwardBf161Interleaved,
+  kKernQkNormF168,
+  kKernQkNormF168Interleaved,
+  kKernQkNormBackwardF168,
+  kKernQkNormBackwardF168Interleaved,
+  kKernQkNormF162,
+  kKernQkNormF162Interleaved,
+  kKernQkNormBackwardF162,
+  kKernQkNormBackwardF162Interleaved,
+  kKernQkNormF161,
+  kKernQkNormF161Interleaved,
+  kKernQkNormBackwardF161,
+  kKernQkNormBackwardF161Interleaved,
+  kKernQkNormF328,
+  kKernQkNormF328Interleaved,
+  kKernQkNormBackwardF328,
+  kKernQkNormBackwardF328Interleaved,
+  kKernQkNormF322,
+  kKernQkNormF322Interleaved,
+  kKernQkNormBackwardF322,
+  kKernQkNormBackwardF322Interleaved,
+  kKernQkNormF321,
+  kKernQkNormF321Interleaved,
+  kKernQkNormBackwardF321,
+  kKernQkNormBackwardF321Interleaved,
   kKernQkNormDweight,
   kKernelCount
 };

@@ -93,8 +93,42 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModInt8, "sh_linear_i8_f16_16x32_kernel"},
     {kModInt8, "sh_linear_i8_f32_16x16_kernel"},
     {kModInt8, "sh_linear_i8_f32_16x32_kernel"},
-    {kModQkNorm, "sh_qk_norm_rope_kernel"},
-    {kModQkNorm, "sh_qk_norm_rope_backward_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_1_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_1_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_1_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_1_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_8_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_2_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_2_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_1_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_1_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_1_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
 };
 

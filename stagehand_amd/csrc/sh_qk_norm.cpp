@@ -79,28 +79,45 @@ uint32_t lanes_of(uint32_t dim) {
   return lanes;
 }
 
-uint32_t workgroups(uint64_t rows, uint32_t lanes, uint32_t most) {
-  const uint64_t groups = sh::kQkThreads / lanes;
-  return (uint32_t)std::min<uint64_t>((rows + groups - 1) / groups, most);
+// Pairs that are loaded and stored together: 8 if a head's rotated pairs and its others come in such runs.
+int run_of(const sh_qk_norm_rope_args* a) {
+  const uint32_t rotated = a->rot / 2, all = a->dim / 2;
+  return rotated % 8 == 0 && all % 8 == 0 ? 0 : rotated % 2 == 0 && all % 2 == 0 ? 1 : 2;  // 8, 2, 1
 }
 
-constexpr uint32_t kBackwardGrid = 1024;
+constexpr uint32_t kComputeUnits = 256;
+constexpr uint32_t kWaves = sh::kQkThreads / 64;
+// Workgroups at most: what runs at a time, so that each loads the weights once and takes many tokens.
+constexpr uint32_t kForwardGrid = 8 * kComputeUnits, kBackwardGrid = 3 * kComputeUnits;
 
 sh::QkNormKernelArgs kernel_args(const sh_qk_norm_rope_args* a, bool backward) {
   sh::QkNormKernelArgs ka{};
   ka.a = *a;
   ka.lanes = lanes_of(a->dim);
-  const uint64_t tokens = (uint64_t)a->batch * a->seq;
-  const uint32_t most = backward ? kBackwardGrid : 0xFFFFFFFFu / (2 * sh::kQkThreads);
-  ka.q_grid = workgroups(tokens * a->q_heads, ka.lanes, most);
-  ka.k_grid = workgroups(tokens * a->k_heads, ka.lanes, most);
+  const uint32_t heads = std::max(a->q_heads, a->k_heads);
+  ka.abreast = 1;
+  while (ka.abreast < heads && ka.abreast < 64 / ka.lanes) ka.abreast *= 2;
+  const uint64_t per_wave = 64 / ka.lanes / ka.abreast;
+  const uint64_t groups = ((uint64_t)a->batch * a->seq + per_wave - 1) / per_wave;
+  // Few tokens: their heads are spread over more wavefronts, to eight a compute unit.
+  const uint64_t most = ((uint64_t)heads + ka.abreast - 1) / ka.abreast;
+  ka.segments = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 8 * kComputeUnits / std::max<uint64_t>(groups, 1)));
+  ka.units = heads == 0 ? 0 : groups * ka.segments;
+  ka.grid = (uint32_t)std::min<uint64_t>((ka.units + kWaves - 1) / kWaves, backward ? kBackwardGrid : kForwardGrid);
   return ka;
 }
 
 bool wants_dweight(const sh_qk_norm_rope_args* a) { return a->dq_weight != nullptr || a->dk_weight != nullptr; }
 
 uint64_t partial_bytes(const sh::QkNormKernelArgs& ka) {
-  return wants_dweight(&ka.a) ? 4ull * ka.a.dim * (ka.q_grid + ka.k_grid) : 0;
+  return wants_dweight(&ka.a) ? 2 * 4ull * ka.a.dim * ka.grid : 0;
+}
+
+// Four kernels for each type and run: forward, forward interleaved, backward, backward interleaved.
+sh::KernelId kernel_of(const sh_qk_norm_rope_args* a, bool backward) {
+  static_assert(sh::kKernQkNormBackwardF321Interleaved - sh::kKernQkNormBf168 == 3 * 3 * 4 - 1, "one kernel per variant");
+  return (sh::KernelId)(sh::kKernQkNormBf168 + ((a->dtype - SH_DTYPE_BF16) * 3 + run_of(a)) * 4 + (backward ? 2 : 0) +
+                        (a->interleaved ? 1 : 0));
 }
 
 }  // namespace
@@ -110,9 +127,9 @@ extern "C" int sh_qk_norm_rope(const sh_qk_norm_rope_args* args, void* stream) {
   sh::clear_error();
   if (int st = check(args, false, who)) return st;
   const sh::QkNormKernelArgs ka = kernel_args(args, false);
-  if (ka.q_grid + ka.k_grid == 0) return SH_OK;
+  if (ka.grid == 0) return SH_OK;
   void* list[] = {(void*)&ka};
-  return sh::launch_kernel(sh::kKernQkNormRope, ka.q_grid + ka.k_grid, sh::kQkThreads, (hipStream_t)stream, list, who);
+  return sh::launch_kernel(kernel_of(args, false), ka.grid, sh::kQkThreads, (hipStream_t)stream, list, who);
 }
 
 extern "C" int sh_qk_norm_rope_workspace(const sh_qk_norm_rope_args* args, uint64_t* bytes) {
@@ -139,11 +156,10 @@ extern "C" int sh_qk_norm_rope_backward(const sh_qk_norm_rope_args* args, void* 
   if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
   ka.partials = wants_dweight(args) ? static_cast<float*>(workspace) : nullptr;
   void* list[] = {(void*)&ka};
-  if (ka.q_grid + ka.k_grid > 0)
-    if (int st = sh::launch_kernel(sh::kKernQkNormRopeBackward, ka.q_grid + ka.k_grid, sh::kQkThreads,
-                                   (hipStream_t)stream, list, who))
+  if (ka.grid > 0)
+    if (int st = sh::launch_kernel(kernel_of(args, true), ka.grid, sh::kQkThreads, (hipStream_t)stream, list, who))
       return st;
   if (!wants_dweight(args)) return SH_OK;
   // without tokens the sums are over nothing: zeros
-  return sh::launch_kernel(sh::kKernQkNormDweight, 2, sh::kQkThreads, (hipStream_t)stream, list, who);
+  return sh::launch_kernel(sh::kKernQkNormDweight, 2 * ((args->dim + 31) / 32), sh::kQkThreads, (hipStream_t)stream, list, who);
 }

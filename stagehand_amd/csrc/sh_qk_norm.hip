@@ -3,7 +3,12 @@
 //
 // A head's values are taken as dim / 2 pairs. Pairs p < rot / 2 are rotated: (p, p + rot / 2), or
 // (2p, 2p + 1) when interleaved. The values past rot form pairs the same way with the angle 0, so
-// every pair is handled alike. `lanes` work-items share a head, each holds kQkSlots pairs in registers.
+// every pair is handled alike.
+//
+// The work is bound by HBM: each value is read once and written once (backward: two reads, one write). A
+// group of `lanes` work-items holds a head, kQkSlots pairs each, in registers: the statistics, the rotation and
+// the gradient need no second read and no shared memory. A group keeps its token's cosines and sines
+// while it takes the token's heads one after another, and the weights for its life.
 
 #include <hip/hip_runtime.h>
 
@@ -15,176 +20,359 @@ namespace {
 
 constexpr uint32_t kSlots = sh::kQkSlots;
 
-__device__ __forceinline__ float load_value(const void* p, uint64_t i, uint32_t dtype) {
-  if (dtype == SH_DTYPE_BF16) return (float)static_cast<const __bf16*>(p)[i];
-  if (dtype == SH_DTYPE_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return static_cast<const float*>(p)[i];
-}
+// V values at any address of memory (gfx950 loads and stores whole vectors there), or at a multiple of ALIGN
+// bytes of LDS.
+template <typename T, uint32_t V, uint32_t ALIGN = 2>
+struct Run {
+  typedef T Vec __attribute__((ext_vector_type(V)));
+  typedef Vec VecAny __attribute__((aligned(ALIGN)));
 
-__device__ __forceinline__ void store_value(void* p, uint64_t i, float v, uint32_t dtype) {
-  if (dtype == SH_DTYPE_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else if (dtype == SH_DTYPE_F16) static_cast<_Float16*>(p)[i] = (_Float16)v;
-  else static_cast<float*>(p)[i] = v;
-}
-
-// The places of pair p's two values in a head.
-__device__ __forceinline__ void pair_places(uint32_t p, uint32_t dim, uint32_t rot, bool interleaved, uint32_t* i0,
-                                            uint32_t* i1) {
-  if (interleaved) {
-    *i0 = 2 * p;
-    *i1 = 2 * p + 1;
-  } else if (p < rot / 2) {
-    *i0 = p;
-    *i1 = p + rot / 2;
-  } else {
-    *i0 = rot / 2 + p;
-    *i1 = *i0 + (dim - rot) / 2;
+  static __device__ __forceinline__ void load(const T* p, float (&out)[V]) {
+    if constexpr (V == 1) {
+      out[0] = (float)*p;
+    } else {
+      const Vec v = *reinterpret_cast<const VecAny*>(p);
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) out[i] = (float)v[i];
+    }
   }
-}
-
-struct Row {
-  uint64_t b, h, s;
+  static __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
+    if constexpr (V == 1) {
+      *p = (T)in[0];
+    } else {
+      Vec v;
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) v[i] = (T)in[i];
+      *reinterpret_cast<VecAny*>(p) = v;
+    }
+  }
 };
 
-__device__ __forceinline__ uint64_t at(const sh_heads& v, const Row& r) {
-  return r.b * v.batch_stride + r.h * v.head_stride + r.s * v.seq_stride;
-}
-
-// A token's row of the tables, or -1 where it has none.
-__device__ __forceinline__ int64_t table_row(const sh_qk_norm_rope_args& a, const Row& r) {
-  int64_t p;
-  if (a.positions == nullptr) p = a.start + (int64_t)r.s;
-  else if (a.position_bytes == 8) p = static_cast<const int64_t*>(a.positions)[r.b * a.position_batch_stride + r.s];
-  else p = static_cast<const int32_t*>(a.positions)[r.b * a.position_batch_stride + r.s];
-  return p >= 0 && p < (int64_t)a.table_rows ? p : -1;
-}
-
-template <bool BACKWARD>
-__device__ __forceinline__ void qk_norm_body(const sh::QkNormKernelArgs& ka) {
-  const sh_qk_norm_rope_args& a = ka.a;
-  const bool is_k = blockIdx.x >= ka.q_grid;
-  const uint32_t block = is_k ? blockIdx.x - ka.q_grid : blockIdx.x;
-  const uint32_t grid = is_k ? ka.k_grid : ka.q_grid;
-  const uint32_t heads = is_k ? a.k_heads : a.q_heads;
-  const sh_heads& in = is_k ? a.k : a.q;
-  const sh_heads& out = is_k ? a.k_out : a.q_out;
-  const sh_heads& din = is_k ? a.dk : a.dq;
-  const void* weight = is_k ? a.k_weight : a.q_weight;
-  const uint32_t lanes = ka.lanes, groups = sh::kQkThreads / lanes;
-  const uint32_t lane = threadIdx.x % lanes, group = threadIdx.x / lanes;
-  const bool interleaved = a.interleaved != 0;
-  const float rdim = 1.0f / (float)a.dim;
-  float dw0[kSlots] = {}, dw1[kSlots] = {};
-
-  const uint64_t rows = (uint64_t)a.batch * a.seq * heads;
-  for (uint64_t row = (uint64_t)block * groups + group; row < rows; row += (uint64_t)grid * groups) {
-    const Row r{row / heads / a.seq, row % heads, row / heads % a.seq};
-    const int64_t tr = a.rot > 0 ? table_row(a, r) : 0;
-    float x0[kSlots], x1[kSlots], sq = 0.0f;
-#pragma unroll
-    for (uint32_t j = 0; j < kSlots; ++j) {
-      const uint32_t p = j * lanes + lane;
-      x0[j] = x1[j] = 0.0f;
-      if (p < a.dim / 2) {
-        uint32_t i0, i1;
-        pair_places(p, a.dim, a.rot, interleaved, &i0, &i1);
-        x0[j] = load_value(in.data, at(in, r) + i0, a.dtype);
-        x1[j] = load_value(in.data, at(in, r) + i1, a.dtype);
-      }
-      sq += x0[j] * x0[j] + x1[j] * x1[j];
+// A weight of `dim` values in fp32 (ones without one).
+__device__ __forceinline__ void share_weight(float* shared, const void* w, uint32_t dtype, uint32_t dim) {
+  for (uint32_t i = threadIdx.x; i < dim; i += sh::kQkThreads) {
+    float v = 1.0f;
+    if (w != nullptr) {
+      if (dtype == SH_DTYPE_BF16) v = (float)static_cast<const __bf16*>(w)[i];
+      else if (dtype == SH_DTYPE_F16) v = (float)static_cast<const _Float16*>(w)[i];
+      else v = static_cast<const float*>(w)[i];
     }
-    for (uint32_t m = lanes / 2; m >= 1; m >>= 1) sq += __shfl_xor(sq, (int)m);
-    const float rstd = 1.0f / __builtin_sqrtf(sq * rdim + a.eps);
-    float g0[kSlots], g1[kSlots], dot = 0.0f;
+    shared[i] = v;
+  }
+}
+
+// The sum over the `lanes` (a power of two) neighbouring work-items of a group, in all of them: halves of
+// 2, 4, 8 and 16 by data-parallel primitives (each adds a half that already agrees), 32 and 64 by shuffles.
+template <int CTRL>
+__device__ __forceinline__ float add_moved(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
+  if (lanes >= 2) v = add_moved<0xB1>(v);   // quad_perm 1,0,3,2
+  if (lanes >= 4) v = add_moved<0x4E>(v);   // quad_perm 2,3,0,1
+  if (lanes >= 8) v = add_moved<0x141>(v);  // row_half_mirror
+  if (lanes >= 16) v = add_moved<0x140>(v);  // row_mirror
+  if (lanes >= 32) v += __shfl_xor(v, 16);
+  if (lanes >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
+// v^(-1/2). The instruction is good to an ulp and takes no subnormal numbers.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  return v >= 0x1p-100f ? __builtin_amdgcn_rsqf(v) : 1.0f / __builtin_sqrtf(v);
+}
+
+// What a work-item knows of its pairs: chunk j is V pairs from p[j] on.
+template <typename T, uint32_t V, bool INTERLEAVED>
+struct Pairs {
+  static constexpr uint32_t kChunks = kSlots / V;
+  uint32_t lane, lanes, half, rot_half;
+
+  __device__ __forceinline__ Pairs(const sh_qk_norm_rope_args& a, uint32_t lane, uint32_t lanes)
+      : lane(lane), lanes(lanes), half(a.dim / 2), rot_half(a.rot / 2) {}
+  __device__ __forceinline__ uint32_t first(uint32_t j) const { return (j * lanes + lane) * V; }
+  __device__ __forceinline__ bool in(uint32_t j) const { return first(j) < half; }
+  __device__ __forceinline__ bool rotated(uint32_t j) const { return first(j) < rot_half; }
+  // places of the chunk's first pair: with rot / 2 and dim / 2 pairs, the second half of the rotated values
+  // starts at rot / 2, the others at rot and at rot + (dim - rot) / 2
+  __device__ __forceinline__ uint32_t i0(uint32_t j) const {
+    return INTERLEAVED ? 2 * first(j) : first(j) + (rotated(j) ? 0 : rot_half);
+  }
+  __device__ __forceinline__ uint32_t i1(uint32_t j) const {
+    return INTERLEAVED ? 2 * first(j) + 1 : first(j) + (rotated(j) ? rot_half : half);
+  }
+
+  template <uint32_t ALIGN = 2, typename U>
+  __device__ __forceinline__ void load(const U* base, float (&v0)[kSlots], float (&v1)[kSlots]) const {
 #pragma unroll
-    for (uint32_t j = 0; j < kSlots; ++j) {
-      const uint32_t p = j * lanes + lane;
-      if (p >= a.dim / 2) continue;
-      uint32_t i0, i1;
-      pair_places(p, a.dim, a.rot, interleaved, &i0, &i1);
-      float c = 1.0f, s = 0.0f;
-      if (p < a.rot / 2) {
-        c = tr < 0 ? __builtin_nanf("") : a.cos[(uint64_t)tr * a.table_ld + p];
-        s = tr < 0 ? __builtin_nanf("") : a.sin[(uint64_t)tr * a.table_ld + p];
-      }
-      const float w0 = weight != nullptr ? load_value(weight, i0, a.weight_dtype) : 1.0f;
-      const float w1 = weight != nullptr ? load_value(weight, i1, a.weight_dtype) : 1.0f;
-      x0[j] *= rstd;
-      x1[j] *= rstd;
-      if (!BACKWARD) {
-        const float n0 = x0[j] * w0, n1 = x1[j] * w1;
-        store_value(out.data, at(out, r) + i0, n0 * c - n1 * s, a.dtype);
-        store_value(out.data, at(out, r) + i1, n1 * c + n0 * s, a.dtype);
+    for (uint32_t j = 0; j < kChunks; ++j) {
+      float a[V], b[V];
+      if (in(j)) {
+        if constexpr (INTERLEAVED) {
+          float both[2 * V];
+          if constexpr (sizeof(U) * 2 * V > 16) {
+            Run<U, V, ALIGN>::load(base + i0(j), a);
+            Run<U, V, ALIGN>::load(base + i0(j) + V, b);
+#pragma unroll
+            for (uint32_t i = 0; i < V; ++i) both[i] = a[i], both[V + i] = b[i];
+          } else {
+            Run<U, 2 * V, ALIGN>::load(base + i0(j), both);
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < V; ++i) a[i] = both[2 * i], b[i] = both[2 * i + 1];
+        } else {
+          Run<U, V, ALIGN>::load(base + i0(j), a);
+          Run<U, V, ALIGN>::load(base + i1(j), b);
+        }
       } else {
-        const float y0 = load_value(out.data, at(out, r) + i0, a.dtype);
-        const float y1 = load_value(out.data, at(out, r) + i1, a.dtype);
-        g0[j] = y0 * c + y1 * s;
-        g1[j] = y1 * c - y0 * s;
-        dw0[j] += g0[j] * x0[j];
-        dw1[j] += g1[j] * x1[j];
-        g0[j] *= w0;
-        g1[j] *= w1;
-        dot += g0[j] * x0[j] + g1[j] * x1[j];
-      }
-    }
-    if (BACKWARD && din.data != nullptr) {
-      for (uint32_t m = lanes / 2; m >= 1; m >>= 1) dot += __shfl_xor(dot, (int)m);
-      const float mean = dot * rdim;
 #pragma unroll
-      for (uint32_t j = 0; j < kSlots; ++j) {
-        const uint32_t p = j * lanes + lane;
-        if (p >= a.dim / 2) continue;
-        uint32_t i0, i1;
-        pair_places(p, a.dim, a.rot, interleaved, &i0, &i1);
-        store_value(din.data, at(din, r) + i0, rstd * (g0[j] - x0[j] * mean), a.dtype);
-        store_value(din.data, at(din, r) + i1, rstd * (g1[j] - x1[j] * mean), a.dtype);
+        for (uint32_t i = 0; i < V; ++i) a[i] = b[i] = 0.0f;
       }
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) v0[j * V + i] = a[i], v1[j * V + i] = b[i];
     }
   }
-  if (BACKWARD && ka.partials != nullptr) {
-    // the workgroup's sums, group after group
-    __shared__ float sums[SH_QK_MAX_DIM];
-    for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads) sums[i] = 0.0f;
-    __syncthreads();
-    for (uint32_t g = 0; g < groups; ++g) {
-      if (g == group) {
+
+  template <uint32_t ALIGN = 2, typename U>
+  __device__ __forceinline__ void store(U* base, const float (&v0)[kSlots], const float (&v1)[kSlots]) const {
 #pragma unroll
-        for (uint32_t j = 0; j < kSlots; ++j) {
-          const uint32_t p = j * lanes + lane;
-          if (p >= a.dim / 2) continue;
-          uint32_t i0, i1;
-          pair_places(p, a.dim, a.rot, interleaved, &i0, &i1);
-          sums[i0] += dw0[j];
-          sums[i1] += dw1[j];
+    for (uint32_t j = 0; j < kChunks; ++j) {
+      if (!in(j)) continue;
+      float a[V], b[V];
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) {
+        if constexpr (INTERLEAVED) {
+          // values 0 .. V - 1 and V .. 2 V - 1 of the 2 V that lie together
+          a[i] = i % 2 ? v1[j * V + i / 2] : v0[j * V + i / 2];
+          b[i] = (V + i) % 2 ? v1[j * V + (V + i) / 2] : v0[j * V + (V + i) / 2];
+        } else {
+          a[i] = v0[j * V + i];
+          b[i] = v1[j * V + i];
         }
       }
-      __syncthreads();
+      Run<U, V, ALIGN>::store(base + i0(j), a);
+      Run<U, V, ALIGN>::store(base + (INTERLEAVED ? i0(j) + V : i1(j)), b);
     }
-    for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads)
-      ka.partials[(uint64_t)blockIdx.x * a.dim + i] = sums[i];
   }
+
+  // A weight that share_weight() has put into LDS.
+  __device__ __forceinline__ void load_weight(const float* shared, float (&v0)[kSlots], float (&v1)[kSlots]) const {
+    load<(V >= 4 ? 16 : 4 * V)>(shared, v0, v1);
+  }
+
+  // Cosines and sines of the token at (b, s); NaN where its position has no row.
+  __device__ __forceinline__ void load_angles(const sh_qk_norm_rope_args& a, uint64_t b, uint64_t s, float (&c)[kSlots],
+                                              float (&n)[kSlots]) const {
+    int64_t row = 0;
+    bool known = true;
+    if (a.rot > 0) {
+      if (a.positions == nullptr) row = a.start + (int64_t)s;
+      else if (a.position_bytes == 8) row = static_cast<const int64_t*>(a.positions)[b * a.position_batch_stride + s];
+      else row = static_cast<const int32_t*>(a.positions)[b * a.position_batch_stride + s];
+      known = row >= 0 && row < (int64_t)a.table_rows;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kChunks; ++j) {
+      float x[V], y[V];
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) {
+        x[i] = rotated(j) ? __builtin_nanf("") : 1.0f;
+        y[i] = rotated(j) ? __builtin_nanf("") : 0.0f;
+      }
+      if (rotated(j) && known) {
+        const uint64_t at = (uint64_t)row * a.table_ld + first(j);
+        Run<float, V>::load(a.cos + at, x);
+        Run<float, V>::load(a.sin + at, y);
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < V; ++i) c[j * V + i] = x[i], n[j * V + i] = y[i];
+    }
+  }
+};
+
+// The groups of a wavefront side by side: `abreast` of them share a token and take every abreast-th of its
+// heads, segment by segment; a wavefront's unit is one segment of 64 / lanes / abreast tokens.
+template <typename T, uint32_t V, bool INTERLEAVED>
+__device__ __forceinline__ void forward(const sh::QkNormKernelArgs& ka) {
+  const sh_qk_norm_rope_args& a = ka.a;
+  const uint32_t lanes = ka.lanes, abreast = ka.abreast;
+  const uint32_t lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) / lanes;
+  const uint32_t phase = group & (abreast - 1), token_of = group / abreast, per_wave = 64 / lanes / abreast;
+  const Pairs<T, V, INTERLEAVED> pairs(a, lane, lanes);
+  const float rdim = 1.0f / (float)a.dim;
+  const uint64_t tokens = (uint64_t)a.batch * a.seq;
+  __shared__ alignas(16) float shared[2][SH_QK_MAX_DIM];
+  share_weight(shared[0], a.q_weight, a.weight_dtype, a.dim);
+  share_weight(shared[1], a.k_weight, a.weight_dtype, a.dim);
+  __syncthreads();
+  float qw0[kSlots], qw1[kSlots], kw0[kSlots], kw1[kSlots];
+  pairs.load_weight(shared[0], qw0, qw1);
+  pairs.load_weight(shared[1], kw0, kw1);
+  const uint64_t waves = (uint64_t)gridDim.x * (sh::kQkThreads / 64);
+  for (uint64_t unit = (uint64_t)blockIdx.x * (sh::kQkThreads / 64) + threadIdx.x / 64; unit < ka.units; unit += waves) {
+    const uint64_t t = unit / ka.segments * per_wave + token_of;
+    const uint32_t seg = (uint32_t)(unit % ka.segments);
+    if (t >= tokens) continue;
+    const uint64_t b = t / a.seq, s = t % a.seq;
+    float c[kSlots], n[kSlots];
+    pairs.load_angles(a, b, s, c, n);
+    auto heads = [&](const sh_heads& in, const sh_heads& out, uint32_t count, const float (&w0)[kSlots],
+                     const float (&w1)[kSlots]) {
+      const T* x = static_cast<const T*>(in.data) + b * in.batch_stride + s * in.seq_stride;
+      T* y = static_cast<T*>(out.data) + b * out.batch_stride + s * out.seq_stride;
+      for (uint32_t h = seg * abreast + phase; h < count; h += ka.segments * abreast) {
+        float x0[kSlots], x1[kSlots], sq = 0.0f;
+        pairs.load(x + h * in.head_stride, x0, x1);
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
+        const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+          const float n0 = x0[i] * r * w0[i], n1 = x1[i] * r * w1[i];
+          x0[i] = n0 * c[i] - n1 * n[i];
+          x1[i] = n1 * c[i] + n0 * n[i];
+        }
+        pairs.store(y + h * out.head_stride, x0, x1);
+      }
+    };
+    heads(a.q, a.q_out, a.q_heads, qw0, qw1);
+    heads(a.k, a.k_out, a.k_heads, kw0, kw1);
+  }
+}
+
+template <typename T, uint32_t V, bool INTERLEAVED>
+__device__ __forceinline__ void backward(const sh::QkNormKernelArgs& ka) {
+  const sh_qk_norm_rope_args& a = ka.a;
+  const uint32_t lanes = ka.lanes, abreast = ka.abreast;
+  const uint32_t lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) / lanes, wave = threadIdx.x / 64;
+  const uint32_t phase = group & (abreast - 1), token_of = group / abreast, per_wave = 64 / lanes / abreast;
+  const Pairs<T, V, INTERLEAVED> pairs(a, lane, lanes);
+  const float rdim = 1.0f / (float)a.dim;
+  const uint64_t tokens = (uint64_t)a.batch * a.seq;
+  __shared__ alignas(16) float shared[2][SH_QK_MAX_DIM];
+  share_weight(shared[0], a.q_weight, a.weight_dtype, a.dim);
+  share_weight(shared[1], a.k_weight, a.weight_dtype, a.dim);
+  __syncthreads();
+  float qw0[kSlots], qw1[kSlots], kw0[kSlots], kw1[kSlots];
+  pairs.load_weight(shared[0], qw0, qw1);
+  pairs.load_weight(shared[1], kw0, kw1);
+  float dq0[kSlots] = {}, dq1[kSlots] = {}, dk0[kSlots] = {}, dk1[kSlots] = {};
+  const uint64_t waves = (uint64_t)gridDim.x * (sh::kQkThreads / 64);
+  for (uint64_t unit = (uint64_t)blockIdx.x * (sh::kQkThreads / 64) + wave; unit < ka.units; unit += waves) {
+    const uint64_t t = unit / ka.segments * per_wave + token_of;
+    const uint32_t seg = (uint32_t)(unit % ka.segments);
+    if (t >= tokens) continue;
+    const uint64_t b = t / a.seq, s = t % a.seq;
+    float c[kSlots], n[kSlots];
+    pairs.load_angles(a, b, s, c, n);
+    auto heads = [&](const sh_heads& in, const sh_heads& grad, const sh_heads& out, uint32_t count,
+                     const float (&w0)[kSlots], const float (&w1)[kSlots], float (&dw0)[kSlots], float (&dw1)[kSlots]) {
+      const T* x = static_cast<const T*>(in.data) + b * in.batch_stride + s * in.seq_stride;
+      const T* dy = static_cast<const T*>(grad.data) + b * grad.batch_stride + s * grad.seq_stride;
+      T* dx = static_cast<T*>(out.data) + b * out.batch_stride + s * out.seq_stride;
+      for (uint32_t h = seg * abreast + phase; h < count; h += ka.segments * abreast) {
+        float x0[kSlots], x1[kSlots], y0[kSlots], y1[kSlots], sq = 0.0f, dot = 0.0f;
+        pairs.load(x + h * in.head_stride, x0, x1);
+        pairs.load(dy + h * grad.head_stride, y0, y1);
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+          const float g0 = y0[i] * c[i] + y1[i] * n[i], g1 = y1[i] * c[i] - y0[i] * n[i];
+          y0[i] = g0;
+          y1[i] = g1;
+          sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
+          dot = __builtin_fmaf(g0 * w0[i], x0[i], __builtin_fmaf(g1 * w1[i], x1[i], dot));
+        }
+        const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
+        const float mean = group_sum(dot, lanes) * r * rdim;  // of h x^
+#pragma unroll
+        for (uint32_t i = 0; i < kSlots; ++i) {
+          x0[i] *= r;
+          x1[i] *= r;
+          dw0[i] = __builtin_fmaf(y0[i], x0[i], dw0[i]);
+          dw1[i] = __builtin_fmaf(y1[i], x1[i], dw1[i]);
+          x0[i] = r * (y0[i] * w0[i] - x0[i] * mean);
+          x1[i] = r * (y1[i] * w1[i] - x1[i] * mean);
+        }
+        if (out.data != nullptr) pairs.store(dx + h * out.head_stride, x0, x1);
+      }
+    };
+    heads(a.q, a.q_out, a.dq, a.q_heads, qw0, qw1, dq0, dq1);
+    heads(a.k, a.k_out, a.dk, a.k_heads, kw0, kw1, dk0, dk1);
+  }
+  if (ka.partials == nullptr) return;
+  // The workgroup's sums: over a wavefront's groups, then over the wavefronts, always in the same order.
+  __shared__ alignas(16) float sums[sh::kQkThreads / 64][SH_QK_MAX_DIM];
+  auto put = [&](float (&v0)[kSlots], float (&v1)[kSlots], uint32_t which) {
+#pragma unroll
+    for (uint32_t i = 0; i < kSlots; ++i) {
+      for (uint32_t m = lanes; m < 64; m *= 2) {
+        v0[i] += __shfl_xor(v0[i], (int)m);
+        v1[i] += __shfl_xor(v1[i], (int)m);
+      }
+    }
+    __syncthreads();
+    if (group == 0) pairs.template store<(V >= 4 ? 16 : 4 * V)>(sums[wave], v0, v1);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads) {
+      float v = 0.0f;
+      for (uint32_t w = 0; w < sh::kQkThreads / 64; ++w) v += sums[w][i];
+      ka.partials[((uint64_t)which * gridDim.x + blockIdx.x) * a.dim + i] = v;
+    }
+  };
+  put(dq0, dq1, 0);
+  put(dk0, dk1, 1);
 }
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_rope_kernel(sh::QkNormKernelArgs ka) {
-  qk_norm_body<false>(ka);
-}
+#define SH_QK(name, T, V)                                                                                           \
+  extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_##name##_##V##_kernel(                    \
+      sh::QkNormKernelArgs ka) {                                                                                    \
+    forward<T, V, false>(ka);                                                                                       \
+  }                                                                                                                 \
+  extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_##name##_##V##_interleaved_kernel(        \
+      sh::QkNormKernelArgs ka) {                                                                                    \
+    forward<T, V, true>(ka);                                                                                        \
+  }                                                                                                                 \
+  extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_backward_##name##_##V##_kernel(           \
+      sh::QkNormKernelArgs ka) {                                                                                    \
+    backward<T, V, false>(ka);                                                                                      \
+  }                                                                                                                 \
+  extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_backward_##name##_##V##_interleaved_kernel( \
+      sh::QkNormKernelArgs ka) {                                                                                    \
+    backward<T, V, true>(ka);                                                                                       \
+  }
+SH_QK(bf16, __bf16, 8)
+SH_QK(bf16, __bf16, 2)
+SH_QK(bf16, __bf16, 1)
+SH_QK(f16, _Float16, 8)
+SH_QK(f16, _Float16, 2)
+SH_QK(f16, _Float16, 1)
+SH_QK(f32, float, 8)
+SH_QK(f32, float, 2)
+SH_QK(f32, float, 1)
 
-extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_rope_backward_kernel(sh::QkNormKernelArgs ka) {
-  qk_norm_body<true>(ka);
-}
-
-// dweight[i] = sum of the workgroups' partial sums: workgroup 0 the queries', workgroup 1 the keys'.
+// dweight[i] = sum of the workgroups' partial sums. A workgroup takes 32 values i of the queries' or the keys'
+// weight; 8 work-items add up each, every 8th partial, and are joined in order.
 extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_dweight_kernel(sh::QkNormKernelArgs ka) {
   const sh_qk_norm_rope_args& a = ka.a;
-  const uint32_t first = blockIdx.x == 0 ? 0 : ka.q_grid;
-  const uint32_t count = blockIdx.x == 0 ? ka.q_grid : ka.k_grid;
-  void* out = blockIdx.x == 0 ? a.dq_weight : a.dk_weight;
+  const uint32_t blocks = (a.dim + 31) / 32;
+  const uint32_t which = blockIdx.x / blocks, i = blockIdx.x % blocks * 32 + threadIdx.x % 32;
+  void* out = which == 0 ? a.dq_weight : a.dk_weight;
   if (out == nullptr) return;
-  for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads) {
-    float v = 0.0f;
-    for (uint32_t b = 0; b < count; ++b) v += ka.partials[(uint64_t)(first + b) * a.dim + i];
-    store_value(out, i, v, a.weight_dtype);
+  __shared__ float part[8][32];
+  float v = 0.0f;
+  if (i < a.dim) {
+    const float* p = ka.partials + (uint64_t)which * ka.grid * a.dim + i;
+#pragma unroll 8
+    for (uint32_t b = threadIdx.x / 32; b < ka.grid; b += 8) v += p[(uint64_t)b * a.dim];
   }
+  part[threadIdx.x / 32][threadIdx.x % 32] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32 || i >= a.dim) return;
+  v = 0.0f;
+  for (uint32_t w = 0; w < 8; ++w) v += part[w][threadIdx.x];
+  if (a.weight_dtype == SH_DTYPE_BF16) static_cast<__bf16*>(out)[i] = (__bf16)v;
+  else if (a.weight_dtype == SH_DTYPE_F16) static_cast<_Float16*>(out)[i] = (_Float16)v;
+  else static_cast<float*>(out)[i] = v;
 }
