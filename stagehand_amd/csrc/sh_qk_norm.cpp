@@ -94,23 +94,30 @@ sh::QkNormKernelArgs kernel_args(const sh_qk_norm_rope_args* a, bool backward) {
   sh::QkNormKernelArgs ka{};
   ka.a = *a;
   ka.lanes = lanes_of(a->dim);
-  const uint32_t heads = std::max(a->q_heads, a->k_heads);
-  ka.abreast = 1;
-  while (ka.abreast < heads && ka.abreast < 64 / ka.lanes) ka.abreast *= 2;
-  const uint64_t per_wave = 64 / ka.lanes / ka.abreast;
-  const uint64_t groups = ((uint64_t)a->batch * a->seq + per_wave - 1) / per_wave;
-  // Few tokens: their heads are spread over more wavefronts, to eight a compute unit.
-  const uint64_t most = ((uint64_t)heads + ka.abreast - 1) / ka.abreast;
-  ka.segments = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 8 * kComputeUnits / std::max<uint64_t>(groups, 1)));
-  ka.units = heads == 0 ? 0 : groups * ka.segments;
-  ka.grid = (uint32_t)std::min<uint64_t>((ka.units + kWaves - 1) / kWaves, backward ? kBackwardGrid : kForwardGrid);
+  const uint64_t tokens = (uint64_t)a->batch * a->seq, all = (uint64_t)a->q_heads + a->k_heads;
+  for (int i = 0; i < 2; ++i) {
+    sh::QkNormPart& p = ka.part[i];
+    const uint32_t heads = i == 0 ? a->q_heads : a->k_heads;
+    p.abreast = p.segments = 1;
+    if (heads == 0 || tokens == 0) continue;
+    while (p.abreast < heads && p.abreast < 64 / ka.lanes) p.abreast *= 2;
+    const uint64_t per_wave = 64 / ka.lanes / p.abreast, groups = (tokens + per_wave - 1) / per_wave;
+    // Few tokens: their heads are spread over more wavefronts, to eight a compute unit.
+    const uint64_t most = ((uint64_t)heads + p.abreast - 1) / p.abreast;
+    p.segments = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 8 * kComputeUnits / groups));
+    p.units = groups * p.segments;
+    const uint64_t grid = std::max<uint64_t>(1, (backward ? kBackwardGrid : kForwardGrid) * heads / all);
+    p.grid = (uint32_t)std::min<uint64_t>((p.units + kWaves - 1) / kWaves, grid);
+  }
   return ka;
 }
+
+uint32_t grid_of(const sh::QkNormKernelArgs& ka) { return ka.part[0].grid + ka.part[1].grid; }
 
 bool wants_dweight(const sh_qk_norm_rope_args* a) { return a->dq_weight != nullptr || a->dk_weight != nullptr; }
 
 uint64_t partial_bytes(const sh::QkNormKernelArgs& ka) {
-  return wants_dweight(&ka.a) ? 2 * 4ull * ka.a.dim * ka.grid : 0;
+  return wants_dweight(&ka.a) ? 4ull * ka.a.dim * grid_of(ka) : 0;
 }
 
 // Four kernels for each type and run: forward, forward interleaved, backward, backward interleaved.
@@ -127,9 +134,9 @@ extern "C" int sh_qk_norm_rope(const sh_qk_norm_rope_args* args, void* stream) {
   sh::clear_error();
   if (int st = check(args, false, who)) return st;
   const sh::QkNormKernelArgs ka = kernel_args(args, false);
-  if (ka.grid == 0) return SH_OK;
+  if (grid_of(ka) == 0) return SH_OK;
   void* list[] = {(void*)&ka};
-  return sh::launch_kernel(kernel_of(args, false), ka.grid, sh::kQkThreads, (hipStream_t)stream, list, who);
+  return sh::launch_kernel(kernel_of(args, false), grid_of(ka), sh::kQkThreads, (hipStream_t)stream, list, who);
 }
 
 extern "C" int sh_qk_norm_rope_workspace(const sh_qk_norm_rope_args* args, uint64_t* bytes) {
@@ -156,8 +163,8 @@ extern "C" int sh_qk_norm_rope_backward(const sh_qk_norm_rope_args* args, void* 
   if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
   ka.partials = wants_dweight(args) ? static_cast<float*>(workspace) : nullptr;
   void* list[] = {(void*)&ka};
-  if (ka.grid > 0)
-    if (int st = sh::launch_kernel(kernel_of(args, true), ka.grid, sh::kQkThreads, (hipStream_t)stream, list, who))
+  if (grid_of(ka) > 0)
+    if (int st = sh::launch_kernel(kernel_of(args, true), grid_of(ka), sh::kQkThreads, (hipStream_t)stream, list, who))
       return st;
   if (!wants_dweight(args)) return SH_OK;
   // without tokens the sums are over nothing: zeros

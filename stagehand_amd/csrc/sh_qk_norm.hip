@@ -192,135 +192,141 @@ struct Pairs {
 
 // The groups of a wavefront side by side: `abreast` of them share a token and take every abreast-th of its
 // heads, segment by segment; a wavefront's unit is one segment of 64 / lanes / abreast tokens.
+// What a workgroup has to do: the first q_grid take the queries, the others the keys. The groups of a
+// wavefront lie side by side: `abreast` of them share a token and take every abreast-th of its heads, segment by
+// segment; a wavefront's unit is one segment of 64 / lanes / abreast tokens.
+struct Share {
+  const sh_heads& in;
+  const sh_heads& out;
+  const sh_heads& din;
+  uint32_t heads, block, grid, segments, abreast, phase, token_of, per_wave;
+  uint64_t units;
+
+  __device__ __forceinline__ Share(const sh::QkNormKernelArgs& ka, bool is_k)
+      : in(is_k ? ka.a.k : ka.a.q), out(is_k ? ka.a.k_out : ka.a.q_out), din(is_k ? ka.a.dk : ka.a.dq) {
+    const sh::QkNormPart& part = ka.part[is_k];
+    heads = is_k ? ka.a.k_heads : ka.a.q_heads;
+    block = blockIdx.x - (is_k ? ka.part[0].grid : 0);
+    grid = part.grid;
+    segments = part.segments;
+    abreast = part.abreast;
+    units = part.units;
+    const uint32_t group = (threadIdx.x & 63) / ka.lanes;
+    phase = group & (abreast - 1);
+    token_of = group / abreast;
+    per_wave = 64 / ka.lanes / abreast;
+  }
+};
+
 template <typename T, uint32_t V, bool INTERLEAVED>
 __device__ __forceinline__ void forward(const sh::QkNormKernelArgs& ka) {
   const sh_qk_norm_rope_args& a = ka.a;
-  const uint32_t lanes = ka.lanes, abreast = ka.abreast;
-  const uint32_t lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) / lanes;
-  const uint32_t phase = group & (abreast - 1), token_of = group / abreast, per_wave = 64 / lanes / abreast;
-  const Pairs<T, V, INTERLEAVED> pairs(a, lane, lanes);
+  const bool is_k = blockIdx.x >= ka.part[0].grid;
+  const Share m(ka, is_k);
+  const uint32_t lanes = ka.lanes;
+  const Pairs<T, V, INTERLEAVED> pairs(a, threadIdx.x & (lanes - 1), lanes);
   const float rdim = 1.0f / (float)a.dim;
   const uint64_t tokens = (uint64_t)a.batch * a.seq;
-  __shared__ alignas(16) float shared[2][SH_QK_MAX_DIM];
-  share_weight(shared[0], a.q_weight, a.weight_dtype, a.dim);
-  share_weight(shared[1], a.k_weight, a.weight_dtype, a.dim);
+  __shared__ alignas(16) float shared[SH_QK_MAX_DIM];
+  share_weight(shared, is_k ? a.k_weight : a.q_weight, a.weight_dtype, a.dim);
   __syncthreads();
-  float qw0[kSlots], qw1[kSlots], kw0[kSlots], kw1[kSlots];
-  pairs.load_weight(shared[0], qw0, qw1);
-  pairs.load_weight(shared[1], kw0, kw1);
-  const uint64_t waves = (uint64_t)gridDim.x * (sh::kQkThreads / 64);
-  for (uint64_t unit = (uint64_t)blockIdx.x * (sh::kQkThreads / 64) + threadIdx.x / 64; unit < ka.units; unit += waves) {
-    const uint64_t t = unit / ka.segments * per_wave + token_of;
-    const uint32_t seg = (uint32_t)(unit % ka.segments);
+  float w0[kSlots], w1[kSlots];
+  pairs.load_weight(shared, w0, w1);
+  constexpr uint32_t kWaves = sh::kQkThreads / 64;
+  for (uint64_t unit = (uint64_t)m.block * kWaves + threadIdx.x / 64; unit < m.units; unit += (uint64_t)m.grid * kWaves) {
+    const uint64_t t = unit / m.segments * m.per_wave + m.token_of;
+    const uint32_t seg = (uint32_t)(unit % m.segments);
     if (t >= tokens) continue;
     const uint64_t b = t / a.seq, s = t % a.seq;
     float c[kSlots], n[kSlots];
     pairs.load_angles(a, b, s, c, n);
-    auto heads = [&](const sh_heads& in, const sh_heads& out, uint32_t count, const float (&w0)[kSlots],
-                     const float (&w1)[kSlots]) {
-      const T* x = static_cast<const T*>(in.data) + b * in.batch_stride + s * in.seq_stride;
-      T* y = static_cast<T*>(out.data) + b * out.batch_stride + s * out.seq_stride;
-      for (uint32_t h = seg * abreast + phase; h < count; h += ka.segments * abreast) {
-        float x0[kSlots], x1[kSlots], sq = 0.0f;
-        pairs.load(x + h * in.head_stride, x0, x1);
+    const T* x = static_cast<const T*>(m.in.data) + b * m.in.batch_stride + s * m.in.seq_stride;
+    T* y = static_cast<T*>(m.out.data) + b * m.out.batch_stride + s * m.out.seq_stride;
+    for (uint32_t h = seg * m.abreast + m.phase; h < m.heads; h += m.segments * m.abreast) {
+      float x0[kSlots], x1[kSlots], sq = 0.0f;
+      pairs.load(x + h * m.in.head_stride, x0, x1);
 #pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
-        const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
+      for (uint32_t i = 0; i < kSlots; ++i) sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
+      const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
 #pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) {
-          const float n0 = x0[i] * r * w0[i], n1 = x1[i] * r * w1[i];
-          x0[i] = n0 * c[i] - n1 * n[i];
-          x1[i] = n1 * c[i] + n0 * n[i];
-        }
-        pairs.store(y + h * out.head_stride, x0, x1);
+      for (uint32_t i = 0; i < kSlots; ++i) {
+        const float n0 = x0[i] * r * w0[i], n1 = x1[i] * r * w1[i];
+        x0[i] = n0 * c[i] - n1 * n[i];
+        x1[i] = n1 * c[i] + n0 * n[i];
       }
-    };
-    heads(a.q, a.q_out, a.q_heads, qw0, qw1);
-    heads(a.k, a.k_out, a.k_heads, kw0, kw1);
+      pairs.store(y + h * m.out.head_stride, x0, x1);
+    }
   }
 }
 
 template <typename T, uint32_t V, bool INTERLEAVED>
 __device__ __forceinline__ void backward(const sh::QkNormKernelArgs& ka) {
   const sh_qk_norm_rope_args& a = ka.a;
-  const uint32_t lanes = ka.lanes, abreast = ka.abreast;
-  const uint32_t lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 63) / lanes, wave = threadIdx.x / 64;
-  const uint32_t phase = group & (abreast - 1), token_of = group / abreast, per_wave = 64 / lanes / abreast;
-  const Pairs<T, V, INTERLEAVED> pairs(a, lane, lanes);
+  const bool is_k = blockIdx.x >= ka.part[0].grid;
+  const Share m(ka, is_k);
+  const uint32_t lanes = ka.lanes, wave = threadIdx.x / 64;
+  const Pairs<T, V, INTERLEAVED> pairs(a, threadIdx.x & (lanes - 1), lanes);
   const float rdim = 1.0f / (float)a.dim;
   const uint64_t tokens = (uint64_t)a.batch * a.seq;
-  __shared__ alignas(16) float shared[2][SH_QK_MAX_DIM];
-  share_weight(shared[0], a.q_weight, a.weight_dtype, a.dim);
-  share_weight(shared[1], a.k_weight, a.weight_dtype, a.dim);
+  constexpr uint32_t kWaves = sh::kQkThreads / 64;
+  __shared__ alignas(16) float shared[kWaves][SH_QK_MAX_DIM];
+  share_weight(shared[0], is_k ? a.k_weight : a.q_weight, a.weight_dtype, a.dim);
   __syncthreads();
-  float qw0[kSlots], qw1[kSlots], kw0[kSlots], kw1[kSlots];
-  pairs.load_weight(shared[0], qw0, qw1);
-  pairs.load_weight(shared[1], kw0, kw1);
-  float dq0[kSlots] = {}, dq1[kSlots] = {}, dk0[kSlots] = {}, dk1[kSlots] = {};
-  const uint64_t waves = (uint64_t)gridDim.x * (sh::kQkThreads / 64);
-  for (uint64_t unit = (uint64_t)blockIdx.x * (sh::kQkThreads / 64) + wave; unit < ka.units; unit += waves) {
-    const uint64_t t = unit / ka.segments * per_wave + token_of;
-    const uint32_t seg = (uint32_t)(unit % ka.segments);
+  float w0[kSlots], w1[kSlots], dw0[kSlots] = {}, dw1[kSlots] = {};
+  pairs.load_weight(shared[0], w0, w1);
+  for (uint64_t unit = (uint64_t)m.block * kWaves + wave; unit < m.units; unit += (uint64_t)m.grid * kWaves) {
+    const uint64_t t = unit / m.segments * m.per_wave + m.token_of;
+    const uint32_t seg = (uint32_t)(unit % m.segments);
     if (t >= tokens) continue;
     const uint64_t b = t / a.seq, s = t % a.seq;
     float c[kSlots], n[kSlots];
     pairs.load_angles(a, b, s, c, n);
-    auto heads = [&](const sh_heads& in, const sh_heads& grad, const sh_heads& out, uint32_t count,
-                     const float (&w0)[kSlots], const float (&w1)[kSlots], float (&dw0)[kSlots], float (&dw1)[kSlots]) {
-      const T* x = static_cast<const T*>(in.data) + b * in.batch_stride + s * in.seq_stride;
-      const T* dy = static_cast<const T*>(grad.data) + b * grad.batch_stride + s * grad.seq_stride;
-      T* dx = static_cast<T*>(out.data) + b * out.batch_stride + s * out.seq_stride;
-      for (uint32_t h = seg * abreast + phase; h < count; h += ka.segments * abreast) {
-        float x0[kSlots], x1[kSlots], y0[kSlots], y1[kSlots], sq = 0.0f, dot = 0.0f;
-        pairs.load(x + h * in.head_stride, x0, x1);
-        pairs.load(dy + h * grad.head_stride, y0, y1);
+    const T* x = static_cast<const T*>(m.in.data) + b * m.in.batch_stride + s * m.in.seq_stride;
+    const T* dy = static_cast<const T*>(m.out.data) + b * m.out.batch_stride + s * m.out.seq_stride;
+    T* dx = static_cast<T*>(m.din.data) + b * m.din.batch_stride + s * m.din.seq_stride;
+    for (uint32_t h = seg * m.abreast + m.phase; h < m.heads; h += m.segments * m.abreast) {
+      float x0[kSlots], x1[kSlots], y0[kSlots], y1[kSlots], sq = 0.0f, dot = 0.0f;
+      pairs.load(x + h * m.in.head_stride, x0, x1);
+      pairs.load(dy + h * m.out.head_stride, y0, y1);
 #pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) {
-          const float g0 = y0[i] * c[i] + y1[i] * n[i], g1 = y1[i] * c[i] - y0[i] * n[i];
-          y0[i] = g0;
-          y1[i] = g1;
-          sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
-          dot = __builtin_fmaf(g0 * w0[i], x0[i], __builtin_fmaf(g1 * w1[i], x1[i], dot));
-        }
-        const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
-        const float mean = group_sum(dot, lanes) * r * rdim;  // of h x^
-#pragma unroll
-        for (uint32_t i = 0; i < kSlots; ++i) {
-          x0[i] *= r;
-          x1[i] *= r;
-          dw0[i] = __builtin_fmaf(y0[i], x0[i], dw0[i]);
-          dw1[i] = __builtin_fmaf(y1[i], x1[i], dw1[i]);
-          x0[i] = r * (y0[i] * w0[i] - x0[i] * mean);
-          x1[i] = r * (y1[i] * w1[i] - x1[i] * mean);
-        }
-        if (out.data != nullptr) pairs.store(dx + h * out.head_stride, x0, x1);
+      for (uint32_t i = 0; i < kSlots; ++i) {
+        const float g0 = y0[i] * c[i] + y1[i] * n[i], g1 = y1[i] * c[i] - y0[i] * n[i];
+        y0[i] = g0;
+        y1[i] = g1;
+        sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
+        dot = __builtin_fmaf(g0 * w0[i], x0[i], __builtin_fmaf(g1 * w1[i], x1[i], dot));
       }
-    };
-    heads(a.q, a.q_out, a.dq, a.q_heads, qw0, qw1, dq0, dq1);
-    heads(a.k, a.k_out, a.dk, a.k_heads, kw0, kw1, dk0, dk1);
+      const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
+      const float mean = group_sum(dot, lanes) * r * rdim;  // of h x^
+#pragma unroll
+      for (uint32_t i = 0; i < kSlots; ++i) {
+        x0[i] *= r;
+        x1[i] *= r;
+        dw0[i] = __builtin_fmaf(y0[i], x0[i], dw0[i]);
+        dw1[i] = __builtin_fmaf(y1[i], x1[i], dw1[i]);
+        x0[i] = r * (y0[i] * w0[i] - x0[i] * mean);
+        x1[i] = r * (y1[i] * w1[i] - x1[i] * mean);
+      }
+      if (m.din.data != nullptr) pairs.store(dx + h * m.din.head_stride, x0, x1);
+    }
   }
   if (ka.partials == nullptr) return;
   // The workgroup's sums: over a wavefront's groups, then over the wavefronts, always in the same order.
-  __shared__ alignas(16) float sums[sh::kQkThreads / 64][SH_QK_MAX_DIM];
-  auto put = [&](float (&v0)[kSlots], float (&v1)[kSlots], uint32_t which) {
 #pragma unroll
-    for (uint32_t i = 0; i < kSlots; ++i) {
-      for (uint32_t m = lanes; m < 64; m *= 2) {
-        v0[i] += __shfl_xor(v0[i], (int)m);
-        v1[i] += __shfl_xor(v1[i], (int)m);
-      }
+  for (uint32_t i = 0; i < kSlots; ++i) {
+    for (uint32_t d = lanes; d < 64; d *= 2) {
+      dw0[i] += __shfl_xor(dw0[i], (int)d);
+      dw1[i] += __shfl_xor(dw1[i], (int)d);
     }
-    __syncthreads();
-    if (group == 0) pairs.template store<(V >= 4 ? 16 : 4 * V)>(sums[wave], v0, v1);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads) {
-      float v = 0.0f;
-      for (uint32_t w = 0; w < sh::kQkThreads / 64; ++w) v += sums[w][i];
-      ka.partials[((uint64_t)which * gridDim.x + blockIdx.x) * a.dim + i] = v;
-    }
-  };
-  put(dq0, dq1, 0);
-  put(dk0, dk1, 1);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) < lanes) pairs.template store<(V >= 4 ? 16 : 4 * V)>(shared[wave], dw0, dw1);
+  __syncthreads();
+  for (uint32_t i = threadIdx.x; i < a.dim; i += sh::kQkThreads) {
+    float v = 0.0f;
+    for (uint32_t w = 0; w < kWaves; ++w) v += shared[w][i];
+    ka.partials[(uint64_t)blockIdx.x * a.dim + i] = v;
+  }
 }
 
 }  // namespace
@@ -363,9 +369,9 @@ extern "C" __global__ __launch_bounds__(sh::kQkThreads) void sh_qk_norm_dweight_
   __shared__ float part[8][32];
   float v = 0.0f;
   if (i < a.dim) {
-    const float* p = ka.partials + (uint64_t)which * ka.grid * a.dim + i;
+    const float* p = ka.partials + (which == 0 ? 0 : (uint64_t)ka.part[0].grid * a.dim) + i;
 #pragma unroll 8
-    for (uint32_t b = threadIdx.x / 32; b < ka.grid; b += 8) v += p[(uint64_t)b * a.dim];
+    for (uint32_t b = threadIdx.x / 32; b < ka.part[which].grid; b += 8) v += p[(uint64_t)b * a.dim];
   }
   part[threadIdx.x / 32][threadIdx.x % 32] = v;
   __syncthreads();
