@@ -260,49 +260,60 @@ __device__ __forceinline__ void store_run(T* out, const float (&v)[N], bool whol
   }
 }
 
-// TT tokens x TN rows by WT x WN wavefronts, each with FT x FN MFMA tiles; D stages.
-template <uint32_t TT, uint32_t TN, uint32_t WT, uint32_t WN, uint32_t D>
+// f(0), f(1) .. f(N - 1) with constants for the compiler: registers are not indexed at run time whatever it unrolls.
+template <uint32_t I>
+struct Constant {
+  static constexpr uint32_t value = I;
+};
+template <uint32_t N, uint32_t I = 0, typename F>
+__device__ __forceinline__ void each(const F& f) {
+  if constexpr (I < N) {
+    f(Constant<I>{});
+    each<N, I + 1>(f);
+  }
+}
+
+// TT tokens x TN rows by WT x WN wavefronts, each with FT x FN MFMA tiles; D stages. XCDs take consecutive runs of
+// tiles, which run down groups of GROUP tiles in the tokens.
+template <uint32_t TT, uint32_t TN, uint32_t WT, uint32_t WN, uint32_t D, uint32_t GROUP>
 __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* lds) {
   constexpr uint32_t kStage = (TT + TN) * kStep;
   constexpr uint32_t kWaves = WT * WN;
   constexpr uint32_t FT = TT / WT / 16, FN = TN / WN / 16;
-  constexpr uint32_t LT = TT / 8 / kWaves, LN = TN / 8 / kWaves;  // loads of 8 rows per wavefront
+  constexpr uint32_t LT = TT / 8 / kWaves, LN = TN / 8 / kWaves, kLoads = LT + LN;  // of 8 rows per wavefront
   static_assert(FN == 4, "a wavefront's rows are one group of 64 permuted ones");
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  // the workgroup's tile: XCDs take consecutive runs of tiles, tiles run down groups of 8 in the tokens
   const uint32_t tiles_t = (a.tokens + TT - 1) / TT, tiles_n = (a.rows + TN - 1) / TN, tiles = tiles_t * tiles_n;
-  uint32_t p = blockIdx.x;
-  {
-    const uint32_t per = tiles / 8, extra = tiles % 8, x = p % 8, i = p / 8;
-    p = x * per + min(x, extra) + i;
-  }
-  const uint32_t group = p / (8 * tiles_n), in_group = p % (8 * tiles_n), g_rows = min(tiles_t - group * 8, 8u);
-  const uint32_t t0 = (group * 8 + in_group % g_rows) * TT, n0 = in_group / g_rows * TN;
-
+  const uint32_t xcd = blockIdx.x % 8;
+  const uint32_t p = xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8;
+  const uint32_t group = p / (GROUP * tiles_n), in_group = p % (GROUP * tiles_n);
+  const uint32_t g_rows = min(tiles_t - group * GROUP, GROUP);
+  const uint32_t t0 = (group * GROUP + in_group % g_rows) * TT, n0 = in_group / g_rows * TN;
   const i32x4_t tr = rows_resource(a.tq, a.t_ld, t0, a.tokens, TT);
   const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, TN);
+
   // Lane l of a load brings slot l % 8 of row l / 8. The rows of the weight lie permuted in LDS, so that the
   // MFMA results of one lane are 16 consecutive ones: fragment f, row i holds row (i / 4) * 16 + f * 4 + i % 4
   // of the wavefront's 64.
   uint32_t t_off[LT], n_off[LN];
-#pragma unroll
-  for (uint32_t j = 0; j < LT; ++j) {
-    const uint32_t row = (j * kWaves + wave) * 8 + lane / 8;
-    t_off[j] = row * (uint32_t)a.t_ld + ((lane % 8) ^ swizzle(row)) * 16;
-  }
-#pragma unroll
-  for (uint32_t j = 0; j < LN; ++j) {
-    const uint32_t row = (j * kWaves + wave) * 8 + lane / 8;
+  each<LT>([&](auto j) __attribute__((always_inline)) {
+    const uint32_t row = (decltype(j)::value * kWaves + wave) * 8 + lane / 8;
+    t_off[decltype(j)::value] = row * (uint32_t)a.t_ld + ((lane % 8) ^ swizzle(row)) * 16;
+  });
+  each<LN>([&](auto j) __attribute__((always_inline)) {
+    const uint32_t row = (decltype(j)::value * kWaves + wave) * 8 + lane / 8;
     const uint32_t src = row / 64 * 64 + row % 16 / 4 * 16 + row / 16 % 4 * 4 + row % 4;
-    n_off[j] = src * (uint32_t)a.w_ld + ((lane % 8) ^ swizzle(row)) * 16;
-  }
+    n_off[decltype(j)::value] = src * (uint32_t)a.w_ld + ((lane % 8) ^ swizzle(row)) * 16;
+  });
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 1024;
-  auto load = [&](uint32_t stage, uint32_t k) {
-#pragma unroll
-    for (uint32_t j = 0; j < LT; ++j) load_to_lds(tr, lds0 + stage * kStage + j * kWaves * 1024, t_off[j] + k);
-#pragma unroll
-    for (uint32_t j = 0; j < LN; ++j)
-      load_to_lds(wr, lds0 + stage * kStage + TT * kStep + j * kWaves * 1024, n_off[j] + k);
+  const uint32_t end = (uint32_t)a.t_ld;  // a multiple of kStep; the tokens are zero past cols
+  // Load i of a stage: first the tokens', then the rows'. Past the end the offset is outside the resource: such
+  // a load reads nothing and keeps the count of loads in flight the same.
+  auto load = [&](auto i, uint32_t stage, uint32_t k) __attribute__((always_inline)) {
+    constexpr uint32_t I = decltype(i)::value;
+    k = k < end ? k : kPastEnd;
+    if constexpr (I < LT) load_to_lds(tr, lds0 + stage * kStage + I * kWaves * 1024, t_off[I] + k);
+    else load_to_lds(wr, lds0 + stage * kStage + TT * kStep + (I - LT) * kWaves * 1024, n_off[I - LT] + k);
   };
   const uint32_t l16 = lane & 15, part = lane / 16;
   const uint32_t wt = wave / WN, wn = wave % WN;
@@ -312,54 +323,59 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
   struct Fragments {
     i32x4_t t[FT], n[FN];
   };
-  auto read = [&](Fragments& f, uint32_t stage, uint32_t half) {
-    const uint32_t slot = ((half * 4 + part) ^ swizzle(l16)) * 16 + stage * kStage;
-#pragma unroll
-    for (uint32_t j = 0; j < FN; ++j) f.n[j] = *reinterpret_cast<const i32x4_t*>(n_at + slot + j * 16 * kStep);
-#pragma unroll
-    for (uint32_t i = 0; i < FT; ++i) f.t[i] = *reinterpret_cast<const i32x4_t*>(t_at + slot + i * 16 * kStep);
+  uint32_t s = 0;  // the stage that is multiplied
+  // Read i of a half stage: first the rows' fragments, then the tokens'.
+  auto read = [&](Fragments& f, auto i, uint32_t half) __attribute__((always_inline)) {
+    constexpr uint32_t I = decltype(i)::value;
+    const uint32_t slot = ((half * 4 + part) ^ swizzle(l16)) * 16 + s * kStage;
+    if constexpr (I < FN) f.n[I] = *reinterpret_cast<const i32x4_t*>(n_at + slot + I * 16 * kStep);
+    else f.t[I - FN] = *reinterpret_cast<const i32x4_t*>(t_at + slot + (I - FN) * 16 * kStep);
   };
-  auto multiply = [&](const Fragments& f) {
-#pragma unroll
-    for (uint32_t i = 0; i < FT; ++i)
-#pragma unroll
-      for (uint32_t j = 0; j < FN; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.n[j], f.t[i], acc[i][j], 0, 0, 0);
-    // an LDS read, then the MFMAs that hide it
-#pragma unroll
-    for (uint32_t i = 0; i < FT + FN; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, FT * FN / (FT + FN), 0);
-    }
+  // The products of one half stage, in FT parts. Each part starts the LDS reads (READS) and the loads (LOADS)
+  // that its products hide: all at once they would hold up the products of both wavefronts of a SIMD.
+  auto multiply = [&](auto reads, auto loads, const Fragments& f, Fragments& next, uint32_t half, uint32_t stage,
+                      uint32_t k) __attribute__((always_inline)) {
+    each<FT>([&](auto part_of) __attribute__((always_inline)) {
+      constexpr uint32_t I = decltype(part_of)::value;
+      if constexpr (decltype(reads)::value) {
+        constexpr uint32_t kFrom = I * (FT + FN) / FT, kTo = (I + 1) * (FT + FN) / FT;
+        each<kTo, kFrom>([&](auto r) __attribute__((always_inline)) { read(next, r, half); });
+      }
+      if constexpr (decltype(loads)::value) {
+        constexpr uint32_t kFrom = I * kLoads / FT, kTo = (I + 1) * kLoads / FT;
+        each<kTo, kFrom>([&](auto l) __attribute__((always_inline)) { load(l, stage, k); });
+      }
+      each<FN>([&](auto j) __attribute__((always_inline)) {
+        constexpr uint32_t J = decltype(j)::value;
+        acc[I][J] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.n[J], f.t[I], acc[I][J], 0, 0, 0);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
+  constexpr Constant<0> kNo;
+  constexpr Constant<1> kYes;
   // A ring of D stages. The fragments of a half stage are read into registers while the half before is
-  // multiplied, so a stage is read to its end when the first half of its products is done: the loads of the
-  // stage D after it start there and have the products of D - 1 stages to land in.
+  // multiplied, so a stage is read to its end when the first half of its products is done: the loads that take
+  // its place start there and have the products of D - 1 stages to land in.
   // Each wavefront waits for its own loads of the next stage, then the barrier says that everyone's have landed
-  // and that everyone has read the stage whose place the next loads take. Past the end the offsets are outside
-  // the resources: such loads read nothing and keep the count of loads in flight the same.
-  const uint32_t end = (uint32_t)a.t_ld;  // a multiple of kStep; the tokens are zero past cols
+  // and that everyone has read the stage whose place the next loads take.
   Fragments f0, f1;
-#pragma unroll
-  for (uint32_t i = 0; i < D; ++i) load(i, i * kStep < end ? i * kStep : kPastEnd);
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * (LT + LN)) : "memory");
+  each<D>([&](auto d) __attribute__((always_inline)) {
+    each<kLoads>([&](auto i) __attribute__((always_inline)) { load(i, decltype(d)::value, decltype(d)::value * kStep); });
+  });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kLoads) : "memory");
   __syncthreads();
-  read(f0, 0, 0);
-  uint32_t s = 0;
-  for (uint32_t k = kStep; k < end; k += kStep) {
-    read(f1, s, 1);
-    multiply(f0);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * (LT + LN)) : "memory");
+  each<FT + FN>([&](auto i) __attribute__((always_inline)) { read(f0, i, 0); });
+  for (uint32_t k = 0; k + kStep < end; k += kStep) {
+    multiply(kYes, kNo, f0, f1, 1, 0, 0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * kLoads) : "memory");
     __syncthreads();
-    const uint32_t next = k + (D - 1) * kStep;
-    load(s, next < end ? next : kPastEnd);
+    const uint32_t free = s;
     s = s == D - 1 ? 0 : s + 1;
-    read(f0, s, 0);
-    multiply(f1);
+    multiply(kYes, kYes, f1, f0, 0, free, k + D * kStep);
   }
-  read(f1, s, 1);
-  multiply(f0);
-  multiply(f1);
+  multiply(kYes, kNo, f0, f1, 1, 0, 0);
+  multiply(kNo, kNo, f1, f0, 0, 0, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load may outlive the workgroup
 
   // lane: token t0 + .. + l16 of each token fragment, 16 consecutive rows
@@ -375,23 +391,23 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
   }
   const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
   const bool whole = count == 16 && ((uintptr_t)a.out | a.out_ld * bytes | n * bytes) % 16 == 0;
-#pragma unroll
-  for (uint32_t i = 0; i < FT; ++i) {
-    const uint32_t t = t0 + wt * (TT / WT) + i * 16 + l16;
-    if (t >= a.tokens) continue;
+  each<FT>([&](auto i) __attribute__((always_inline)) {
+    constexpr uint32_t I = decltype(i)::value;
+    const uint32_t t = t0 + wt * (TT / WT) + I * 16 + l16;
+    if (t >= a.tokens) return;
     const float scale = a.t_scale[t];
     const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
     float v[16];
-#pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) {
+    each<16>([&](auto j) __attribute__((always_inline)) {
+      constexpr uint32_t J = decltype(j)::value;
       // wz is 0 without zero points: the same value
-      v[j] = __builtin_fmaf(-wz[j], sum, (float)acc[i][j / 4][j % 4]) * (scale * ws[j]) + wb[j];
-    }
+      v[J] = __builtin_fmaf(-wz[J], sum, (float)acc[I][J / 4][J % 4]) * (scale * ws[J]) + wb[J];
+    });
     const uint64_t at = (uint64_t)t * a.out_ld + n;
     if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, v, whole, count);
     else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, v, whole, count);
     else store_run(static_cast<float*>(a.out) + at, v, whole, count);
-  }
+  });
 }
 
 }  // namespace
@@ -638,15 +654,15 @@ SH_LINEAR_FEW(f32, float, 16x32, 2, 4, 2)
     __shared__ alignas(16) uint8_t lds[W * D * (FT + FN) * 16 * kStep];                                       \
     matmul_skinny<FT, FN, W, D>(a, lds);                                                                      \
   }
-#define SH_MATMUL_TILE(name, TT, TN, WT, WN, D)                                                               \
+#define SH_MATMUL_TILE(name, TT, TN, WT, WN, D, GROUP)                                                        \
   extern "C" __global__ __launch_bounds__(WT * WN * 64) void sh_matmul_i8_##name##_kernel(sh::MatmulI8Args a) { \
     __shared__ alignas(16) uint8_t lds[D * (TT + TN) * kStep];                                                \
-    matmul_tile<TT, TN, WT, WN, D>(a, lds);                                                                   \
+    matmul_tile<TT, TN, WT, WN, D, GROUP>(a, lds);                                                            \
   }
 SH_MATMUL_FEW(16x16, 1, 1, 8, 3)
 SH_MATMUL_FEW(16x32, 1, 2, 4, 3)
 SH_MATMUL_FEW(32x32, 2, 2, 4, 2)
-SH_MATMUL_TILE(64x64, 64, 64, 4, 1, 3)
-SH_MATMUL_TILE(128x128, 128, 128, 4, 2, 3)
-SH_MATMUL_TILE(128x256, 128, 256, 4, 4, 3)
-SH_MATMUL_TILE(256x256, 256, 256, 2, 4, 2)
+SH_MATMUL_TILE(64x64, 64, 64, 4, 1, 4, 8)
+SH_MATMUL_TILE(128x128, 128, 128, 4, 2, 3, 4)
+SH_MATMUL_TILE(128x256, 128, 256, 4, 4, 3, 4)
+SH_MATMUL_TILE(256x256, 256, 256, 2, 4, 2, 4)

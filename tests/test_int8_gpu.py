@@ -123,6 +123,9 @@ SIZES = [  # tokens, out, inp
     (32, 512, 512), (33, 257, 640), (64, 64, 4096), (65, 4096, 513), (77, 1000, 1155), (100, 1, 300), (127, 129, 127),
     (128, 128, 128), (129, 255, 384), (255, 257, 256), (256, 256, 256), (257, 513, 1025), (300, 1024, 96),
     (512, 1536, 512), (513, 320, 4097), (1024, 1024, 1024), (1025, 777, 130), (2048, 3072, 192), (4096, 64, 64),
+    # ragged edges of the larger tiles, and columns of one, two and an odd number of 128-byte steps
+    (1000, 2050, 300), (1023, 5000, 200), (2047, 4100, 130), (2049, 4097, 128), (4600, 3080, 257), (4609, 3071, 100),
+    (3000, 6000, 640),
 ]
 
 
