@@ -123,6 +123,10 @@ enum KernelId : int {
   kKernQkNormBf168Interleaved,
   kKernQkNormBackwardBf168,
   kKernQkNormBackwardBf168Interleaved,
+  kKernQkNormBf164,
+  kKernQkNormBf164Interleaved,
+  kKernQkNormBackwardBf164,
+  kKernQkNormBackwardBf164Interleaved,
   kKernQkNormBf162,
   kKernQkNormBf162Interleaved,
   kKernQkNormBackwardBf162,
@@ -135,6 +139,10 @@ enum KernelId : int {
   kKernQkNormF168Interleaved,
   kKernQkNormBackwardF168,
   kKernQkNormBackwardF168Interleaved,
+  kKernQkNormF164,
+  kKernQkNormF164Interleaved,
+  kKernQkNormBackwardF164,
+  kKernQkNormBackwardF164Interleaved,
   kKernQkNormF162,
   kKernQkNormF162Interleaved,
   kKernQkNormBackwardF162,
@@ -147,6 +155,10 @@ enum KernelId : int {
   kKernQkNormF328Interleaved,
   kKernQkNormBackwardF328,
   kKernQkNormBackwardF328Interleaved,
+  kKernQkNormF324,
+  kKernQkNormF324Interleaved,
+  kKernQkNormBackwardF324,
+  kKernQkNormBackwardF324Interleaved,
   kKernQkNormF322,
   kKernQkNormF322Interleaved,
   kKernQkNormBackwardF322,

@@ -97,6 +97,10 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModQkNorm, "sh_qk_norm_bf16_8_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_bf16_8_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_bf16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_bf16_4_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_bf16_4_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_bf16_2_kernel"},
     {kModQkNorm, "sh_qk_norm_bf16_2_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_bf16_2_kernel"},
@@ -109,6 +113,10 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModQkNorm, "sh_qk_norm_f16_8_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f16_8_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f16_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_f16_4_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f16_4_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_f16_2_kernel"},
     {kModQkNorm, "sh_qk_norm_f16_2_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f16_2_kernel"},
@@ -121,6 +129,10 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModQkNorm, "sh_qk_norm_f32_8_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f32_8_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f32_8_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_f32_4_interleaved_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_4_kernel"},
+    {kModQkNorm, "sh_qk_norm_backward_f32_4_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_f32_2_kernel"},
     {kModQkNorm, "sh_qk_norm_f32_2_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f32_2_kernel"},

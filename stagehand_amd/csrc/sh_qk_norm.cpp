@@ -79,10 +79,12 @@ uint32_t lanes_of(uint32_t dim) {
   return lanes;
 }
 
-// Pairs that are loaded and stored together: 8 if a head's rotated pairs and its others come in such runs.
-int run_of(const sh_qk_norm_rope_args* a) {
-  const uint32_t rotated = a->rot / 2, all = a->dim / 2;
-  return rotated % 8 == 0 && all % 8 == 0 ? 0 : rotated % 2 == 0 && all % 2 == 0 ? 1 : 2;  // 8, 2, 1
+// log2 of the pairs that are loaded and stored together, 8 at most: a head's rotated pairs and all its pairs
+// come in whole runs.
+uint32_t log_run(const sh_qk_norm_rope_args* a) {
+  uint32_t n = 3;
+  while ((a->rot / 2 | a->dim / 2) & ((1u << n) - 1)) --n;
+  return n;
 }
 
 constexpr uint32_t kComputeUnits = 256;
@@ -122,8 +124,8 @@ uint64_t partial_bytes(const sh::QkNormKernelArgs& ka) {
 
 // Four kernels for each type and run: forward, forward interleaved, backward, backward interleaved.
 sh::KernelId kernel_of(const sh_qk_norm_rope_args* a, bool backward) {
-  static_assert(sh::kKernQkNormBackwardF321Interleaved - sh::kKernQkNormBf168 == 3 * 3 * 4 - 1, "one kernel per variant");
-  return (sh::KernelId)(sh::kKernQkNormBf168 + ((a->dtype - SH_DTYPE_BF16) * 3 + run_of(a)) * 4 + (backward ? 2 : 0) +
+  static_assert(sh::kKernQkNormBackwardF321Interleaved - sh::kKernQkNormBf168 == 3 * 4 * 4 - 1, "one kernel per variant");
+  return (sh::KernelId)(sh::kKernQkNormBf168 + ((a->dtype - SH_DTYPE_BF16) * 4 + 3 - log_run(a)) * 4 + (backward ? 2 : 0) +
                         (a->interleaved ? 1 : 0));
 }
 

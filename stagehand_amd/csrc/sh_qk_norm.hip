@@ -349,12 +349,15 @@ __device__ __forceinline__ void backward(const sh::QkNormKernelArgs& ka) {
     backward<T, V, true>(ka);                                                                                       \
   }
 SH_QK(bf16, __bf16, 8)
+SH_QK(bf16, __bf16, 4)
 SH_QK(bf16, __bf16, 2)
 SH_QK(bf16, __bf16, 1)
 SH_QK(f16, _Float16, 8)
+SH_QK(f16, _Float16, 4)
 SH_QK(f16, _Float16, 2)
 SH_QK(f16, _Float16, 1)
 SH_QK(f32, float, 8)
+SH_QK(f32, float, 4)
 SH_QK(f32, float, 2)
 SH_QK(f32, float, 1)
 
