@@ -30,11 +30,11 @@ MAX_DIM = 512  # SH_QK_MAX_DIM
 _ARGS = struct.Struct("<24Q" "7Q" "2Q" "q" "11If")
 
 
+_NO_HEADS = (0, 0, 0, 0)
+
+
 def _heads(t: torch.Tensor | None) -> tuple[int, int, int, int]:
-    if t is None:
-        return 0, 0, 0, 0
-    s = t.stride()
-    return t.data_ptr(), s[0], s[1], s[2]
+    return _NO_HEADS if t is None else (t.data_ptr(), *t.stride()[:3])
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -50,14 +50,14 @@ def _pack(q, k, q_out, k_out, dq, dk, q_weight, k_weight, dq_weight, dk_weight, 
     x = q if q is not None else k
     batch, _, seq, dim = x.shape
     weight = q_weight if q_weight is not None else k_weight
-    rot = 0 if cos is None else 2 * cos.shape[1]
+    table_rows, half_rot = (0, 0) if cos is None else cos.shape
     return _ARGS.pack(
         *_heads(q), *_heads(k), *_heads(q_out), *_heads(k_out), *_heads(dq), *_heads(dk),
         _ptr(q_weight), _ptr(k_weight), _ptr(dq_weight), _ptr(dk_weight), _ptr(cos), _ptr(sin), _ptr(positions),
-        cos.stride(0) if rot else 0, positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
-        start, cos.shape[0] if rot else 0, positions.element_size() if positions is not None else 0,
-        batch, seq, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], dim, rot,
-        DTYPE_CODES[x.dtype], DTYPE_CODES[x.dtype if weight is None else weight.dtype], int(interleaved), eps)
+        cos.stride(0) if half_rot else 0, positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
+        start, table_rows, positions.element_size() if positions is not None else 0,
+        batch, seq, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], dim, 2 * half_rot,
+        DTYPE_CODES[x.dtype], DTYPE_CODES[(x if weight is None else weight).dtype], interleaved, eps)
 
 
 def _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out):
@@ -77,28 +77,30 @@ class _QkNormRope(torch.autograd.Function):
         return q_out, k_out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
+        if torch.is_grad_enabled():  # create_graph
+            raise RuntimeError("qk_norm_rope has no second derivatives")
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         want_q, want_k, want_qw, want_kw = ctx.needs_input_grad[:4]
-        if not (want_q or want_qw):
+        if want_q or want_qw:
+            dq_out = _rows_of_values(dq_out)
+        else:
             q = dq_out = None
-        if not (want_k or want_kw):
+        if want_k or want_kw:
+            dk_out = _rows_of_values(dk_out)
+        else:
             k = dk_out = None
-        device = (q if q is not None else k).device
-        with torch.cuda.device(device):
-            dq = _like(q) if want_q else None
-            dk = _like(k) if want_k else None
-            dqw = torch.empty_like(q_weight) if want_qw else None
-            dkw = torch.empty_like(k_weight) if want_kw else None
-            dq_out = None if q is None else _rows_of_values(dq_out)
-            dk_out = None if k is None else _rows_of_values(dk_out)
-            args = _pack(q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, dqw, dkw, cos, sin, positions, *ctx.options)
-            lib = _native.lib()
-            need = ctypes.c_uint64()
+        dq = _like(q) if want_q else None
+        dk = _like(k) if want_k else None
+        dqw = torch.empty_like(q_weight) if want_qw else None
+        dkw = torch.empty_like(k_weight) if want_kw else None
+        args = _pack(q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, dqw, dkw, cos, sin, positions, *ctx.options)
+        lib = _native.lib()
+        ws, need = None, ctypes.c_uint64()
+        if want_qw or want_kw:
             _native.check(lib.sh_qk_norm_rope_workspace(args, ctypes.byref(need)))
-            ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-            _native.check(lib.sh_qk_norm_rope_backward(args, _ptr(ws), need.value, current_stream_handle()))
+            ws = torch.empty(need.value, dtype=torch.uint8, device=(q if q is not None else k).device)
+        _native.check(lib.sh_qk_norm_rope_backward(args, _ptr(ws), need.value, current_stream_handle()))
         return dq, dk, dqw, dkw, None, None, None, None, None, None
 
 
@@ -139,17 +141,17 @@ def qk_norm_rope(
         with on_stream(stream):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
                                 interleaved=interleaved, eps=eps, out=out)
-    device = q.device
+    device, dtype = q.device, q.dtype
     check_device(q, None, "q")
-    if q.dim() != 4 or q.dtype not in DTYPE_CODES:
-        raise ValueError(f"q must be (batch, heads, seq, dim) in bfloat16, float16 or float32, got {q.dtype} {tuple(q.shape)}")
+    if q.dim() != 4 or dtype not in DTYPE_CODES:
+        raise ValueError(f"q must be (batch, heads, seq, dim) in bfloat16, float16 or float32, got {dtype} {tuple(q.shape)}")
     batch, _, seq, dim = q.shape
     if dim % 2 or not 2 <= dim <= MAX_DIM:
         raise ValueError(f"dim {dim} is not an even number in 2 .. {MAX_DIM}")
     if k is not None:
         check_device(k, device, "k")
-        if k.dim() != 4 or k.dtype != q.dtype or (k.shape[0], k.shape[2], k.shape[3]) != (batch, seq, dim):
-            raise ValueError(f"k must be {q.dtype} with q's batch, seq and dim, got {k.dtype} {tuple(k.shape)} for q {tuple(q.shape)}")
+        if k.dim() != 4 or k.dtype != dtype or (k.shape[0], *k.shape[2:]) != (batch, seq, dim):
+            raise ValueError(f"k must be {dtype} with q's batch, seq and dim, got {k.dtype} {tuple(k.shape)} for q {tuple(q.shape)}")
     elif k_weight is not None:
         raise ValueError("k_weight is given without k")
     for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
@@ -160,6 +162,7 @@ def qk_norm_rope(
             raise ValueError(f"{what} must be {dim} contiguous values in bfloat16, float16 or float32, got {w.dtype} {tuple(w.shape)}")
     if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
         raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
+    grad_mode = torch.is_grad_enabled()
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin are given together or not at all")
     if cos is not None:
@@ -169,7 +172,7 @@ def qk_norm_rope(
                 2 * cos.shape[1] > dim or cos.stride() != sin.stride() or (cos.shape[1] > 1 and cos.stride(1) != 1):
             raise ValueError(f"cos and sin must be float32 (positions, rot / 2) rows with rot <= {dim}, "
                              f"got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
-        if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        if grad_mode and (cos.requires_grad or sin.requires_grad):
             raise ValueError("cos and sin have no gradient: detach them")
         if cos.shape[1] == 0:
             cos = sin = None
@@ -192,12 +195,12 @@ def qk_norm_rope(
                                 interleaved=interleaved, eps=eps, out=out)
     q = _rows_of_values(q)
     k = None if k is None else _rows_of_values(k)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    grad = grad_mode and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
     if out is None:
         if grad:
-            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, start, bool(interleaved), float(eps))
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=device)
+            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, start, bool(interleaved), eps)
+        q_out = torch.empty(q.shape, dtype=dtype, device=device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=dtype, device=device)
     else:
         if grad:
             raise RuntimeError("out= has no gradient: call qk_norm_rope under torch.no_grad(), or without out")

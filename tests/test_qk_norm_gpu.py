@@ -299,6 +299,13 @@ def test_out_and_in_place():
     assert torch.equal(qi, want[0]) and torch.equal(ki, want[1])
 
 
+def test_second_derivatives_are_refused():
+    q, k, wq, wk = (t.requires_grad_() for t in make(1, 2, 2, 4, 32, torch.float32))
+    qo, ko = qk_norm_rope(q, k, wq, wk)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(qo.square().sum(), (q,), create_graph=True)
+
+
 def test_nothing_to_do():
     w = torch.ones(64, device="cuda", requires_grad=True)
     cos, sin = tables(4, 64)
