@@ -187,11 +187,11 @@ def test_nonfinite_tokens_stay_their_own(tokens):
 
 def test_padding_columns_do_not_count():
     """Whatever lies between in_features and the row's end, and past the last row, is not read into the result."""
-    for inp, ld in ((100, 112), (100, 160), (129, 144), (64, 80), (33, 48)):
+    for inp, ld in ((100, 112), (100, 160), (129, 144), (64, 80), (33, 48), (130, 256), (100, 128)):
         x, q, s, z, b, _ = make(9, 70, inp, zp=True, seed=inp)
         slab = torch.full((70, ld), 127, dtype=torch.int8, device="cuda")
         slab[:, :inp] = q.cuda()
-        w = Int8Weight(slab, s.cuda(), z.cuda(), b.cuda(), inp)
+        w = Int8Weight(slab, s.cuda(), z.cuda(), b.cuda(), inp, realign=ld % 128 == 0)
         assert w.qweight.data_ptr() == slab.data_ptr()
         check(linear_i8(x.cuda(), w), x, q, s, z, b)
         check(linear_i8(x.cuda().repeat(30, 1), w)[-9:], x, q, s, z, b)
@@ -201,8 +201,14 @@ def test_unaligned_weights_are_copied_once():
     x, q, s, z, b, _ = make(20, 50, 100, seed=1)
     flat = torch.zeros(50 * 100 + 1, dtype=torch.int8, device="cuda")
     flat[1:] = q.cuda().reshape(-1)
-    w = Int8Weight(flat[1:].view(50, 100), s.cuda(), bias=b.cuda())
-    assert w.qweight.stride(0) == 112 and w.qweight.data_ptr() % 16 == 0
+    for realign, ld in ((True, 128), (False, 112)):
+        w = Int8Weight(flat[1:].view(50, 100), s.cuda(), bias=b.cuda(), realign=realign)
+        assert w.qweight.stride(0) == ld and w.qweight.data_ptr() % 16 == 0
+        check(linear_i8(x.cuda(), w), x, q, s, z, b)
+    wide = torch.zeros(50, 144, dtype=torch.int8, device="cuda")
+    wide[:, :100] = q.cuda()
+    w = Int8Weight(wide, s.cuda(), bias=b.cuda(), in_features=100)
+    assert w.qweight.stride(0) == 128
     check(linear_i8(x.cuda(), w), x, q, s, z, b)
     wt = Int8Weight(q.cuda().t().contiguous().t(), s.cuda(), bias=b.cuda())
     check(linear_i8(x.cuda(), wt), x, q, s, z, b)
