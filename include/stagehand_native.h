@@ -758,7 +758,7 @@ int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, const int32_t
  * those of the two calls above. The workspace (16-byte aligned device memory,
  * in use until the call's kernels have run) holds at least
  * sh_linear_i8_workspace bytes, which is 0 for a few tokens. */
-int sh_linear_i8_workspace(uint32_t tokens, uint32_t cols, uint64_t* bytes);
+int sh_linear_i8_workspace(uint32_t tokens, const sh_i8_weight* w, uint64_t* bytes);
 int sh_linear_i8(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t tokens, const sh_i8_weight* w, void* out,
                  uint64_t out_ld, void* workspace, uint64_t workspace_bytes, void* stream);
 

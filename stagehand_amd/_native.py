@@ -226,7 +226,7 @@ _SIGNATURES: dict[str, list] = {
     "sh_turbo_set_writeback_chunks": [_vp, _u32],
     "sh_quantize_tokens": [_vp, _u32, ctypes.c_uint64, _u32, _u32, _vp, ctypes.c_uint64, _vp, _vp, _vp],
     "sh_matmul_i8": [_vp, ctypes.c_uint64, _vp, _vp, _u32, _vp, _vp, _u32, ctypes.c_uint64, _vp],
-    "sh_linear_i8_workspace": [_u32, _u32, ctypes.POINTER(ctypes.c_uint64)],
+    "sh_linear_i8_workspace": [_u32, _vp, ctypes.POINTER(ctypes.c_uint64)],
     "sh_linear_i8": [_vp, _u32, ctypes.c_uint64, _u32, _vp, _vp, ctypes.c_uint64, _vp, ctypes.c_uint64, _vp],
     "sh_qk_norm_rope": [_vp, _vp],
     "sh_qk_norm_rope_workspace": [_vp, ctypes.POINTER(ctypes.c_uint64)],

@@ -112,9 +112,13 @@ int launch_matmul(const sh::MatmulI8Args& a, hipStream_t stream, const char* who
   return sh::launch_kernel((sh::KernelId)(sh::kKernMatmulI816x16 + i), (uint32_t)grid, m.threads, stream, args, who);
 }
 
-// Whether the tokens are few enough for every workgroup to quantise them for itself.
-bool in_one_launch(uint32_t tokens, uint32_t cols) {
-  return tokens <= 16 && (uint64_t)tokens * ((cols + 511) / 512) <= sh::kFewPieces;
+// Whether the tokens are few enough for every workgroup to quantise them for itself: one launch less, about 4
+// us of a call, for work that is done once by each of the weight's rows / 16 or rows / 32 workgroups. Measured
+// (one launch against two): 1 x 4096 x 4096 7.5 and 11 us, 1 x 18432 x 3072 12.4 and 16, 4 x 18432 x 3072 14.2
+// and 15.9, 8 x 4096 x 3072 7.4 and 11.3; past the limits 8 x 18432 x 3072 24 and 16.
+bool in_one_launch(uint32_t tokens, const sh_i8_weight* w) {
+  const uint64_t pieces = (uint64_t)tokens * ((w->cols + 511) / 512);
+  return tokens <= 16 && pieces <= (w->rows > sh::kNarrowRows ? sh::kFewPiecesWide : sh::kFewPiecesNarrow);
 }
 
 struct Workspace {
@@ -122,10 +126,10 @@ struct Workspace {
 };
 
 // q, then the scales, then the sums.
-Workspace workspace_of(uint32_t tokens, uint32_t cols) {
+Workspace workspace_of(uint32_t tokens, const sh_i8_weight* w) {
   Workspace s{};
-  if (in_one_launch(tokens, cols)) return s;
-  s.q_ld = token_ld(cols);
+  if (in_one_launch(tokens, w)) return s;
+  s.q_ld = token_ld(w->cols);
   s.scale = s.q_ld * tokens;
   s.sums = s.scale + 4ull * tokens;
   s.bytes = s.sums + 4ull * tokens;
@@ -162,10 +166,11 @@ extern "C" int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, co
   return launch_matmul(a, (hipStream_t)stream, who);
 }
 
-extern "C" int sh_linear_i8_workspace(uint32_t tokens, uint32_t cols, uint64_t* bytes) {
+extern "C" int sh_linear_i8_workspace(uint32_t tokens, const sh_i8_weight* w, uint64_t* bytes) {
   sh::clear_error();
   if (bytes == nullptr) return sh::fail(SH_ERR_INVALID, "sh_linear_i8_workspace: bytes is NULL");
-  *bytes = workspace_of(tokens, cols).bytes;
+  if (int st = check_weight(w, "sh_linear_i8_workspace")) return st;
+  *bytes = workspace_of(tokens, w).bytes;
   return SH_OK;
 }
 
@@ -177,13 +182,13 @@ extern "C" int sh_linear_i8(const void* x, uint32_t dtype, uint64_t x_ld, uint32
   if (int st = check_x(x, dtype, x_ld, tokens, w->cols, who)) return st;
   if (int st = check_out(out, dtype, out_ld, tokens, w->rows, who)) return st;
   if (tokens == 0 || w->rows == 0) return SH_OK;
-  const Workspace s = workspace_of(tokens, w->cols);
+  const Workspace s = workspace_of(tokens, w);
   if (workspace_bytes < s.bytes || (s.bytes > 0 && workspace == nullptr))
     return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
                     (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
   if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
-  if (in_one_launch(tokens, w->cols)) {
-    const bool wide = w->rows > 32 * 256 - 32;  // 32 rows a workgroup leave no compute unit idle
+  if (in_one_launch(tokens, w)) {
+    const bool wide = w->rows > sh::kNarrowRows;
     const uint32_t grid = wide ? (w->rows + 31) / 32 : (w->rows + 15) / 16;
     if (grid > 0xFFFFFFFFu / 512) return sh::fail(SH_ERR_INVALID, "%s: %u rows are too many for one launch", who, w->rows);
     const sh::MatmulI8Args a{x,    nullptr, nullptr, w->q,   w->scale, w->zero_point, w->bias, out,

@@ -112,16 +112,32 @@ __device__ __forceinline__ uint32_t amax_bits(uint32_t m) {
   return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, (uint16_t)h));
 }
 
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
-  return v;
+// The maximum and the sum over a wavefront, by data-parallel primitives: within rows of 16 lanes every step adds
+// a half that already agrees, then rows 0 and 2 are carried into 1 and 3 and the lower half into the upper.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t otherwise, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)otherwise, (int)v, CTRL, ROWS, 0xF, false);
 }
 
-__device__ __forceinline__ int32_t wave_sum(int32_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  return v;
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = max(v, moved<0xB1, 0xF>(v, v));   // quad_perm 1,0,3,2
+  v = max(v, moved<0x4E, 0xF>(v, v));   // quad_perm 2,3,0,1
+  v = max(v, moved<0x141, 0xF>(v, v));  // row_half_mirror
+  v = max(v, moved<0x140, 0xF>(v, v));  // row_mirror
+  v = max(v, moved<0x142, 0xA>(v, v));  // row_bcast:15
+  v = max(v, moved<0x143, 0xC>(v, v));  // row_bcast:31
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+__device__ __forceinline__ int32_t wave_sum(int32_t s) {
+  uint32_t v = (uint32_t)s;
+  v += moved<0xB1, 0xF>(0, v);
+  v += moved<0x4E, 0xF>(0, v);
+  v += moved<0x141, 0xF>(0, v);
+  v += moved<0x140, 0xF>(0, v);
+  v += moved<0x142, 0xA>(0, v);
+  v += moved<0x143, 0xC>(0, v);
+  return (int32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // WAVES wavefronts per token, C chunks of each work-item in registers between the maximum and the rounding:
@@ -522,15 +538,15 @@ __device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t
 namespace {
 
 // As matmul_skinny for up to 16 tokens, which every workgroup quantises for itself into LDS: one launch, and the
-// weight is on its way meanwhile. A wavefront's piece of a token is 512 values; all of them, kFewPieces / W a
+// weight is on its way meanwhile. A wavefront's piece of a token is 512 values; all of them, PIECES / W a
 // wavefront, stay in registers between maximum and rounding. In `a`, tq is the tokens as they are, t_ld their
 // distance in elements; t_scale and t_sums are not used.
-template <typename T, uint32_t FN, uint32_t W, uint32_t D>
+template <typename T, uint32_t FN, uint32_t W, uint32_t D, uint32_t PIECES>
 __device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* ring, uint8_t* tq, uint32_t* amax,
                                            int32_t* sum) {
   constexpr uint32_t kStage = FN * 16 * kStep;
   constexpr uint32_t kLoads = 2 * FN;
-  constexpr uint32_t kMine = sh::kFewPieces / W;
+  constexpr uint32_t kMine = PIECES / W;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t n0 = blockIdx.x * (16 * FN);
   const uint32_t end = (a.cols + kStep - 1) / kStep * kStep;
@@ -633,20 +649,20 @@ __device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* r
 
 }  // namespace
 
-#define SH_LINEAR_FEW(name, T, tile, FN, W, D)                                                                \
+#define SH_LINEAR_FEW(name, T, tile, FN, W, D, PIECES)                                                        \
   extern "C" __global__ __launch_bounds__(W * 64) void sh_linear_i8_##name##_##tile##_kernel(sh::MatmulI8Args a) { \
     __shared__ alignas(16) uint8_t ring[W * D * FN * 16 * kStep];                                             \
-    __shared__ alignas(16) uint8_t tq[sh::kFewPieces * 512 + 16 * 16];                                        \
+    __shared__ alignas(16) uint8_t tq[PIECES * 512 + 16 * 16];                                                \
     __shared__ uint32_t amax[16];                                                                             \
     __shared__ int32_t sum[16];                                                                               \
-    linear_few<T, FN, W, D>(a, ring, tq, amax, sum);                                                          \
+    linear_few<T, FN, W, D, PIECES>(a, ring, tq, amax, sum);                                                  \
   }
-SH_LINEAR_FEW(bf16, __bf16, 16x16, 1, 8, 3)
-SH_LINEAR_FEW(bf16, __bf16, 16x32, 2, 4, 2)
-SH_LINEAR_FEW(f16, _Float16, 16x16, 1, 8, 3)
-SH_LINEAR_FEW(f16, _Float16, 16x32, 2, 4, 2)
-SH_LINEAR_FEW(f32, float, 16x16, 1, 8, 3)
-SH_LINEAR_FEW(f32, float, 16x32, 2, 4, 2)
+SH_LINEAR_FEW(bf16, __bf16, 16x16, 1, 8, 3, sh::kFewPiecesNarrow)
+SH_LINEAR_FEW(bf16, __bf16, 16x32, 2, 4, 2, sh::kFewPiecesWide)
+SH_LINEAR_FEW(f16, _Float16, 16x16, 1, 8, 3, sh::kFewPiecesNarrow)
+SH_LINEAR_FEW(f16, _Float16, 16x32, 2, 4, 2, sh::kFewPiecesWide)
+SH_LINEAR_FEW(f32, float, 16x16, 1, 8, 3, sh::kFewPiecesNarrow)
+SH_LINEAR_FEW(f32, float, 16x32, 2, 4, 2, sh::kFewPiecesWide)
 
 // The tiles of sh_int8_args.h.
 #define SH_MATMUL_FEW(name, FT, FN, W, D)                                                                     \

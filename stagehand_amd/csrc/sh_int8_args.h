@@ -36,8 +36,11 @@ struct MatmulI8Args {
   uint32_t out_dtype;
 };
 
-// Pieces of 512 values that one launch quantises and multiplies (at most 16 tokens).
-constexpr uint32_t kFewPieces = 16;
+// Pieces of 512 values that one launch quantises and multiplies (at most 16 tokens), for weights of up to
+// kNarrowRows rows, which 16 rows a workgroup spread over the whole chip, and for wider ones, with 32 rows a
+// workgroup and more than one workgroup on a compute unit.
+constexpr uint32_t kNarrowRows = 32 * 255;
+constexpr uint32_t kFewPiecesNarrow = 64, kFewPiecesWide = 32;
 
 // The product's kernels, smallest tile first.
 struct MatmulTile {

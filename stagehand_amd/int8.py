@@ -265,7 +265,7 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = No
     y, out_ld = _output(out, (*x.shape[:-1], weight.out_features), x.dtype, device)
     lib = _native.lib()
     need = ctypes.c_uint64()
-    _native.check(lib.sh_linear_i8_workspace(tokens, weight.in_features, ctypes.byref(need)))
+    _native.check(lib.sh_linear_i8_workspace(tokens, weight._ref, ctypes.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
     _native.check(lib.sh_linear_i8(rows.data_ptr(), code, ld, tokens, weight._ref, y.data_ptr(), out_ld,
                                    None if ws is None else ws.data_ptr(), need.value, current_stream_handle()))

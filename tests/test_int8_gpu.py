@@ -126,6 +126,9 @@ SIZES = [  # tokens, out, inp
     # ragged edges of the larger tiles, and columns of one, two and an odd number of 128-byte steps
     (1000, 2050, 300), (1023, 5000, 200), (2047, 4100, 130), (2049, 4097, 128), (4600, 3080, 257), (4609, 3071, 100),
     (3000, 6000, 640),
+    # the most pieces of 512 values that one launch takes, and one more, for narrow and wide weights
+    (8, 100, 4096), (9, 100, 4096), (16, 33, 2048), (15, 50, 2049), (1, 200, 32768), (1, 70, 32769), (16, 8161, 1024),
+    (11, 8200, 1025), (1, 9000, 16384), (2, 8161, 8193), (16, 8160, 2000), (5, 20000, 513),
 ]
 
 

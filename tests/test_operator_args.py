@@ -107,8 +107,11 @@ def test_matmul_and_linear_refusals():
     assert _native.lib().sh_matmul_i8(*{**ok, "tokens": 0}.values()) == _native.SH_OK
 
     need = ctypes.c_uint64()
-    refused("sh_linear_i8_workspace", 3, 64, None, match="NULL")
-    assert _native.lib().sh_linear_i8_workspace(1000, 100, ctypes.byref(need)) == _native.SH_OK
+    refused("sh_linear_i8_workspace", 3, weight(), None, match="NULL")
+    refused("sh_linear_i8_workspace", 3, None, ctypes.byref(need), match="NULL")
+    refused("sh_linear_i8_workspace", 3, weight(ld=72), ctypes.byref(need), match="ld")
+    assert _native.lib().sh_linear_i8_workspace(1, weight(), ctypes.byref(need)) == _native.SH_OK and need.value == 0
+    assert _native.lib().sh_linear_i8_workspace(1000, weight(), ctypes.byref(need)) == _native.SH_OK
     assert need.value >= 1000 * (128 + 8)
     ok = dict(x=P, dtype=1, x_ld=64, tokens=1000, w=weight(), out=P, out_ld=8, ws=P, ws_bytes=need.value, stream=0)
 
