@@ -254,19 +254,24 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = No
         with on_stream(stream):
             return linear_i8(x, weight, out)
     code = _check_input(x, "linear_i8")
-    device = weight.device
-    check_device(x, device, "x")
+    index = weight.device.index
+    if x.get_device() != index:
+        raise ValueError(f"x must be on {weight.device}, got {x.device}")
     rows, tokens, ld = _token_rows(x, "x")
     if rows.shape[1] != weight.in_features:
         raise ValueError(f"x has {rows.shape[1]} values per token, the weight takes {weight.in_features}")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return linear_i8(x, weight, out)
-    y, out_ld = _output(out, (*x.shape[:-1], weight.out_features), x.dtype, device)
+    if out is None:
+        out_ld = weight.out_features
+        y = x.new_empty((*x.shape[:-1], out_ld))
+    else:
+        y, out_ld = _output(out, (*x.shape[:-1], weight.out_features), x.dtype, weight.device)
     lib = _native.lib()
     need = ctypes.c_uint64()
     _native.check(lib.sh_linear_i8_workspace(tokens, weight._ref, ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
+    ws = x.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _native.check(lib.sh_linear_i8(rows.data_ptr(), code, ld, tokens, weight._ref, y.data_ptr(), out_ld,
                                    None if ws is None else ws.data_ptr(), need.value, current_stream_handle()))
     return y

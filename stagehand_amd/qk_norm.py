@@ -19,7 +19,7 @@ import struct
 import torch
 
 from stagehand_amd import _native
-from stagehand_amd.int8 import DTYPE_CODES, check_device, on_stream
+from stagehand_amd.int8 import DTYPE_CODES, on_stream
 from stagehand_amd.unpack import current_stream_handle
 
 __all__ = ["qk_norm_rope"]
@@ -34,7 +34,10 @@ _NO_HEADS = (0, 0, 0, 0)
 
 
 def _heads(t: torch.Tensor | None) -> tuple[int, int, int, int]:
-    return _NO_HEADS if t is None else (t.data_ptr(), *t.stride()[:3])
+    if t is None:
+        return _NO_HEADS
+    b, h, s, _ = t.stride()
+    return t.data_ptr(), b, h, s
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -45,32 +48,36 @@ def _rows_of_values(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 else t.contiguous()
 
 
-def _pack(q, k, q_out, k_out, dq, dk, q_weight, k_weight, dq_weight, dk_weight, cos, sin, positions, start,
-          interleaved, eps) -> bytes:
-    x = q if q is not None else k
+def _fields(x, q_heads, k_heads, weight, cos, positions, start, interleaved, eps) -> tuple:
+    """The struct's fields from table_ld on, for heads like those of ``x``."""
     batch, _, seq, dim = x.shape
-    weight = q_weight if q_weight is not None else k_weight
-    table_rows, half_rot = (0, 0) if cos is None else cos.shape
-    return _ARGS.pack(
-        *_heads(q), *_heads(k), *_heads(q_out), *_heads(k_out), *_heads(dq), *_heads(dk),
-        _ptr(q_weight), _ptr(k_weight), _ptr(dq_weight), _ptr(dk_weight), _ptr(cos), _ptr(sin), _ptr(positions),
-        cos.stride(0) if half_rot else 0, positions.stride(0) if positions is not None and positions.dim() == 2 else 0,
-        start, table_rows, positions.element_size() if positions is not None else 0,
-        batch, seq, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], dim, 2 * half_rot,
-        DTYPE_CODES[x.dtype], DTYPE_CODES[(x if weight is None else weight).dtype], interleaved, eps)
+    code = DTYPE_CODES[x.dtype]
+    if cos is None:
+        table_rows = half_rot = table_ld = 0
+    else:
+        table_rows, half_rot = cos.shape
+        table_ld = cos.stride(0)
+    if positions is None:
+        position_stride = position_bytes = 0
+    else:
+        position_stride, position_bytes = positions.stride(0) if positions.dim() == 2 else 0, positions.element_size()
+    return (table_ld, position_stride, start, table_rows, position_bytes, batch, seq, q_heads, k_heads, dim, 2 * half_rot,
+            code, code if weight is None else DTYPE_CODES[weight.dtype], interleaved, eps)
 
 
 def _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out):
-    _native.check(_native.lib().sh_qk_norm_rope(
-        _pack(q, k, q_out, k_out, None, None, q_weight, k_weight, None, None, cos, sin, positions, start, interleaved,
-              eps), current_stream_handle()))
+    fields = _fields(q, q.shape[1], 0 if k is None else k.shape[1], k_weight if q_weight is None else q_weight, cos, positions,
+                     start, interleaved, eps)
+    args = _ARGS.pack(*_heads(q), *_heads(k), *_heads(q_out), *_heads(k_out), *_NO_HEADS, *_NO_HEADS, _ptr(q_weight),
+                      _ptr(k_weight), 0, 0, _ptr(cos), _ptr(sin), _ptr(positions), *fields)
+    _native.check(_native.lib().sh_qk_norm_rope(args, current_stream_handle()))
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out = q.new_empty(q.shape)
+        k_out = None if k is None else k.new_empty(k.shape)
         _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
         ctx.options = start, interleaved, eps
@@ -94,7 +101,10 @@ class _QkNormRope(torch.autograd.Function):
         dk = _like(k) if want_k else None
         dqw = torch.empty_like(q_weight) if want_qw else None
         dkw = torch.empty_like(k_weight) if want_kw else None
-        args = _pack(q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, dqw, dkw, cos, sin, positions, *ctx.options)
+        fields = _fields(k if q is None else q, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1],
+                         k_weight if q_weight is None else q_weight, cos, positions, *ctx.options)
+        args = _ARGS.pack(*_heads(q), *_heads(k), *_heads(dq_out), *_heads(dk_out), *_heads(dq), *_heads(dk),
+                          _ptr(q_weight), _ptr(k_weight), _ptr(dqw), _ptr(dkw), _ptr(cos), _ptr(sin), _ptr(positions), *fields)
         lib = _native.lib()
         ws, need = None, ctypes.c_uint64()
         if want_qw or want_kw:
@@ -102,6 +112,12 @@ class _QkNormRope(torch.autograd.Function):
             ws = torch.empty(need.value, dtype=torch.uint8, device=(q if q is not None else k).device)
         _native.check(lib.sh_qk_norm_rope_backward(args, _ptr(ws), need.value, current_stream_handle()))
         return dq, dk, dqw, dkw, None, None, None, None, None, None
+
+
+def _check_weight(w: torch.Tensor, what: str, device: int, dim: int) -> None:
+    if w.get_device() != device or w.shape != (dim,) or w.dtype not in DTYPE_CODES or w.stride(0) != 1:
+        raise ValueError(f"{what} must be {dim} contiguous values in bfloat16, float16 or float32 on q's device, "
+                         f"got {w.device} {w.dtype} {tuple(w.shape)}")
 
 
 def _like(x: torch.Tensor) -> torch.Tensor:
@@ -141,66 +157,66 @@ def qk_norm_rope(
         with on_stream(stream):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
                                 interleaved=interleaved, eps=eps, out=out)
-    device, dtype = q.device, q.dtype
-    check_device(q, None, "q")
-    if q.dim() != 4 or dtype not in DTYPE_CODES:
-        raise ValueError(f"q must be (batch, heads, seq, dim) in bfloat16, float16 or float32, got {dtype} {tuple(q.shape)}")
-    batch, _, seq, dim = q.shape
+    device, shape, dtype = q.get_device(), q.shape, q.dtype
+    if device < 0 or len(shape) != 4 or dtype not in DTYPE_CODES:
+        raise ValueError("q must be a device tensor (batch, heads, seq, dim) in bfloat16, float16 or float32, "
+                         f"got {q.device} {dtype} {tuple(shape)}")
+    batch, _, seq, dim = shape
     if dim % 2 or not 2 <= dim <= MAX_DIM:
         raise ValueError(f"dim {dim} is not an even number in 2 .. {MAX_DIM}")
     if k is not None:
-        check_device(k, device, "k")
-        if k.dim() != 4 or k.dtype != dtype or (k.shape[0], *k.shape[2:]) != (batch, seq, dim):
-            raise ValueError(f"k must be {dtype} with q's batch, seq and dim, got {k.dtype} {tuple(k.shape)} for q {tuple(q.shape)}")
+        ks = k.shape
+        if k.get_device() != device or k.dtype != dtype or len(ks) != 4 or ks[0] != batch or ks[2] != seq or ks[3] != dim:
+            raise ValueError(f"k must be {dtype} on q's device with q's batch, seq and dim, got {k.device} {k.dtype} {tuple(ks)} "
+                             f"for q {q.device} {tuple(shape)}")
     elif k_weight is not None:
         raise ValueError("k_weight is given without k")
-    for what, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is None:
-            continue
-        check_device(w, device, what)
-        if w.shape != (dim,) or w.dtype not in DTYPE_CODES or w.stride(0) != 1:
-            raise ValueError(f"{what} must be {dim} contiguous values in bfloat16, float16 or float32, got {w.dtype} {tuple(w.shape)}")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
+    if q_weight is not None:
+        _check_weight(q_weight, "q_weight", device, dim)
+    if k_weight is not None:
+        _check_weight(k_weight, "k_weight", device, dim)
+        if q_weight is not None and q_weight.dtype != k_weight.dtype:
+            raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
     grad_mode = torch.is_grad_enabled()
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin are given together or not at all")
-    if cos is not None:
-        check_device(cos, device, "cos")
-        check_device(sin, device, "sin")
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
-                2 * cos.shape[1] > dim or cos.stride() != sin.stride() or (cos.shape[1] > 1 and cos.stride(1) != 1):
-            raise ValueError(f"cos and sin must be float32 (positions, rot / 2) rows with rot <= {dim}, "
-                             f"got {cos.dtype} {tuple(cos.shape)} and {sin.dtype} {tuple(sin.shape)}")
+    if cos is not None and sin is not None:
+        table = cos.shape
+        if cos.get_device() != device or sin.get_device() != device or len(table) != 2 or sin.shape != table or \
+                cos.dtype != torch.float32 or sin.dtype != torch.float32 or 2 * table[1] > dim or \
+                cos.stride() != sin.stride() or (table[1] > 1 and cos.stride(1) != 1):
+            raise ValueError(f"cos and sin must be float32 (positions, rot / 2) rows on q's device with rot <= {dim}, got "
+                             f"{cos.device} {cos.dtype} {tuple(table)} and {sin.device} {sin.dtype} {tuple(sin.shape)}")
         if grad_mode and (cos.requires_grad or sin.requires_grad):
             raise ValueError("cos and sin have no gradient: detach them")
-        if cos.shape[1] == 0:
+        if positions is None and not 0 <= start <= table[0] - seq:
+            raise ValueError(f"positions {start} .. {start + seq - 1} are not all in the tables' {table[0]} rows")
+        if table[1] == 0:
             cos = sin = None
+    elif cos is not sin:
+        raise ValueError("cos and sin are given together or not at all")
     if positions is not None:
         if cos is None or start:
             raise ValueError("positions are given with cos and sin, and without start")
-        check_device(positions, device, "positions")
-        if positions.dtype not in (torch.int32, torch.int64) or \
-                tuple(positions.shape) not in ((seq,), (batch, seq), (1, seq)):
-            raise ValueError(f"positions must be int32 or int64 ({seq},) or ({batch}, {seq}), got {positions.dtype} {tuple(positions.shape)}")
-        if positions.dim() == 2 and positions.shape[0] == 1:
+        ps = tuple(positions.shape)
+        if positions.get_device() != device or positions.dtype not in (torch.int64, torch.int32) or \
+                ps not in ((batch, seq), (seq,), (1, seq)):
+            raise ValueError(f"positions must be int32 or int64 ({seq},) or ({batch}, {seq}) on q's device, got "
+                             f"{positions.device} {positions.dtype} {ps}")
+        if len(ps) == 2 and ps[0] == 1:
             positions = positions[0]
         if seq > 1 and positions.stride(-1) != 1:
             positions = positions.contiguous()
-    elif cos is not None and not 0 <= start <= cos.shape[0] - seq:
-        raise ValueError(f"positions {start} .. {start + seq - 1} are not all in the tables' {cos.shape[0]} rows")
-    if device.index != torch.cuda.current_device():
+    if device != torch.cuda.current_device():
         with torch.cuda.device(device):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
                                 interleaved=interleaved, eps=eps, out=out)
     q = _rows_of_values(q)
     k = None if k is None else _rows_of_values(k)
-    grad = grad_mode and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    grad = grad_mode and any([t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)])
     if out is None:
         if grad:
             return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, start, bool(interleaved), eps)
-        q_out = torch.empty(q.shape, dtype=dtype, device=device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=dtype, device=device)
+        q_out = q.new_empty(shape)
+        k_out = None if k is None else k.new_empty(k.shape)
     else:
         if grad:
             raise RuntimeError("out= has no gradient: call qk_norm_rope under torch.no_grad(), or without out")
@@ -210,9 +226,8 @@ def qk_norm_rope(
                 raise ValueError(f"out has {'no' if o is None else 'a'} tensor for {what}")
             if o is None:
                 continue
-            check_device(o, device, f"out for {what}")
-            if o.shape != x.shape or o.dtype != x.dtype or o.stride(3) != 1:
-                raise ValueError(f"out for {what} must be {x.dtype} {tuple(x.shape)} with contiguous heads, "
-                                 f"got {o.dtype} {tuple(o.shape)} strides {o.stride()}")
+            if o.get_device() != device or o.shape != x.shape or o.dtype != dtype or o.stride(3) != 1:
+                raise ValueError(f"out for {what} must be {dtype} {tuple(x.shape)} with contiguous heads on q's device, "
+                                 f"got {o.device} {o.dtype} {tuple(o.shape)} strides {o.stride()}")
     _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
     return q_out, k_out
