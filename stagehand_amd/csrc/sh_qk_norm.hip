@@ -27,14 +27,9 @@ struct Run {
   typedef T Vec __attribute__((ext_vector_type(V)));
   typedef Vec VecAny __attribute__((aligned(ALIGN)));
 
-  static __device__ __forceinline__ void load(const T* p, float (&out)[V]) {
-    if constexpr (V == 1) {
-      out[0] = (float)*p;
-    } else {
-      const Vec v = *reinterpret_cast<const VecAny*>(p);
-#pragma unroll
-      for (uint32_t i = 0; i < V; ++i) out[i] = (float)v[i];
-    }
+  static __device__ __forceinline__ Vec load(const T* p) {
+    if constexpr (V == 1) return Vec{*p};
+    else return *reinterpret_cast<const VecAny*>(p);
   }
   static __device__ __forceinline__ void store(T* p, const float (&in)[V]) {
     if constexpr (V == 1) {
@@ -102,35 +97,41 @@ struct Pairs {
     return INTERLEAVED ? 2 * first(j) + 1 : first(j) + (rotated(j) ? rot_half : half);
   }
 
+  // A head's values as they lie in memory: a load in flight until they are looked at.
+  template <typename U>
+  struct Raw {
+    typename Run<U, V>::Vec a[kChunks], b[kChunks];
+
+    __device__ __forceinline__ void values(float (&v0)[kSlots], float (&v1)[kSlots]) const {
+#pragma unroll
+      for (uint32_t j = 0; j < kChunks; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) {
+          if constexpr (INTERLEAVED) {
+            // pair i is values 2 i and 2 i + 1 of the 2 V that a and b hold
+            v0[j * V + i] = 2 * i < V ? (float)a[j][2 * i % V] : (float)b[j][2 * i % V];
+            v1[j * V + i] = 2 * i + 1 < V ? (float)a[j][(2 * i + 1) % V] : (float)b[j][(2 * i + 1) % V];
+          } else {
+            v0[j * V + i] = (float)a[j][i];
+            v1[j * V + i] = (float)b[j][i];
+          }
+        }
+      }
+    }
+  };
+
   template <uint32_t ALIGN = 2, typename U>
-  __device__ __forceinline__ void load(const U* base, float (&v0)[kSlots], float (&v1)[kSlots]) const {
+  __device__ __forceinline__ Raw<U> load(const U* base) const {
+    Raw<U> r;
 #pragma unroll
     for (uint32_t j = 0; j < kChunks; ++j) {
-      float a[V], b[V];
+      r.a[j] = r.b[j] = (U)0.0f;
       if (in(j)) {
-        if constexpr (INTERLEAVED) {
-          float both[2 * V];
-          if constexpr (sizeof(U) * 2 * V > 16) {
-            Run<U, V, ALIGN>::load(base + i0(j), a);
-            Run<U, V, ALIGN>::load(base + i0(j) + V, b);
-#pragma unroll
-            for (uint32_t i = 0; i < V; ++i) both[i] = a[i], both[V + i] = b[i];
-          } else {
-            Run<U, 2 * V, ALIGN>::load(base + i0(j), both);
-          }
-#pragma unroll
-          for (uint32_t i = 0; i < V; ++i) a[i] = both[2 * i], b[i] = both[2 * i + 1];
-        } else {
-          Run<U, V, ALIGN>::load(base + i0(j), a);
-          Run<U, V, ALIGN>::load(base + i1(j), b);
-        }
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < V; ++i) a[i] = b[i] = 0.0f;
+        r.a[j] = Run<U, V, ALIGN>::load(base + i0(j));
+        r.b[j] = Run<U, V, ALIGN>::load(base + (INTERLEAVED ? i0(j) + V : i1(j)));
       }
-#pragma unroll
-      for (uint32_t i = 0; i < V; ++i) v0[j * V + i] = a[i], v1[j * V + i] = b[i];
     }
+    return r;
   }
 
   template <uint32_t ALIGN = 2, typename U>
@@ -157,7 +158,7 @@ struct Pairs {
 
   // A weight that share_weight() has put into LDS.
   __device__ __forceinline__ void load_weight(const float* shared, float (&v0)[kSlots], float (&v1)[kSlots]) const {
-    load<(V >= 4 ? 16 : 4 * V)>(shared, v0, v1);
+    load<(V >= 4 ? 16 : 4 * V)>(shared).values(v0, v1);
   }
 
   // Cosines and sines of the token at (b, s); NaN where its position has no row.
@@ -181,8 +182,9 @@ struct Pairs {
       }
       if (rotated(j) && known) {
         const uint64_t at = (uint64_t)row * a.table_ld + first(j);
-        Run<float, V>::load(a.cos + at, x);
-        Run<float, V>::load(a.sin + at, y);
+        const typename Run<float, V>::Vec cv = Run<float, V>::load(a.cos + at), sv = Run<float, V>::load(a.sin + at);
+#pragma unroll
+        for (uint32_t i = 0; i < V; ++i) x[i] = cv[i], y[i] = sv[i];
       }
 #pragma unroll
       for (uint32_t i = 0; i < V; ++i) c[j * V + i] = x[i], n[j * V + i] = y[i];
@@ -238,13 +240,13 @@ __device__ __forceinline__ void forward(const sh::QkNormKernelArgs& ka) {
     const uint32_t seg = (uint32_t)(unit % m.segments);
     if (t >= tokens) continue;
     const uint64_t b = t / a.seq, s = t % a.seq;
-    float c[kSlots], n[kSlots];
-    pairs.load_angles(a, b, s, c, n);
     const T* x = static_cast<const T*>(m.in.data) + b * m.in.batch_stride + s * m.in.seq_stride;
     T* y = static_cast<T*>(m.out.data) + b * m.out.batch_stride + s * m.out.seq_stride;
+    float c[kSlots], n[kSlots];
+    pairs.load_angles(a, b, s, c, n);
     for (uint32_t h = seg * m.abreast + m.phase; h < m.heads; h += m.segments * m.abreast) {
       float x0[kSlots], x1[kSlots], sq = 0.0f;
-      pairs.load(x + h * m.in.head_stride, x0, x1);
+      pairs.load(x + h * m.in.head_stride).values(x0, x1);
 #pragma unroll
       for (uint32_t i = 0; i < kSlots; ++i) sq = __builtin_fmaf(x0[i], x0[i], __builtin_fmaf(x1[i], x1[i], sq));
       const float r = inv_sqrt(group_sum(sq, lanes) * rdim + a.eps);
@@ -279,15 +281,17 @@ __device__ __forceinline__ void backward(const sh::QkNormKernelArgs& ka) {
     const uint32_t seg = (uint32_t)(unit % m.segments);
     if (t >= tokens) continue;
     const uint64_t b = t / a.seq, s = t % a.seq;
-    float c[kSlots], n[kSlots];
-    pairs.load_angles(a, b, s, c, n);
     const T* x = static_cast<const T*>(m.in.data) + b * m.in.batch_stride + s * m.in.seq_stride;
     const T* dy = static_cast<const T*>(m.out.data) + b * m.out.batch_stride + s * m.out.seq_stride;
     T* dx = static_cast<T*>(m.din.data) + b * m.din.batch_stride + s * m.din.seq_stride;
+    float c[kSlots], n[kSlots];
+    pairs.load_angles(a, b, s, c, n);
     for (uint32_t h = seg * m.abreast + m.phase; h < m.heads; h += m.segments * m.abreast) {
       float x0[kSlots], x1[kSlots], y0[kSlots], y1[kSlots], sq = 0.0f, dot = 0.0f;
-      pairs.load(x + h * m.in.head_stride, x0, x1);
-      pairs.load(dy + h * m.out.head_stride, y0, y1);
+      const auto xr = pairs.load(x + h * m.in.head_stride);
+      const auto yr = pairs.load(dy + h * m.out.head_stride);
+      xr.values(x0, x1);
+      yr.values(y0, y1);
 #pragma unroll
       for (uint32_t i = 0; i < kSlots; ++i) {
         const float g0 = y0[i] * c[i] + y1[i] * n[i], g1 = y1[i] * c[i] - y0[i] * n[i];
