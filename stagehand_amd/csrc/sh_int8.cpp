@@ -83,11 +83,12 @@ int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* w
 
 // The tile of the least estimated time: rounds of tiles over the 256 compute units, times what 128 columns of
 // one round take (MI355X, measured over 64 to 1500 tiles of 3072 and 4096 columns). Larger tiles read LDS and the
-// caches less for each product (256 x 256: 2500 TOPS; 64 x 64: 1000), smaller ones leave fewer compute units
-// idle. Around the switches, 4096 x 4096 weights unless said: 64 tokens 8.6 us with 32x32, 11 with 64x64; 128 x
-// 9216 x 3072: 13.1 with 64x64, 20.8 with 32x32, 15 with 128x128; 1024 tokens 21 with 128x128, 24 with 128x256, 45
-// with 256x256; 512 x 9216 x 3072: 21.6 with 128x256, 29 with 128x128, 38 with 256x256; 2048 tokens 34 with
-// 128x256, 60 with 256x256; 1024 x 12288 x 3072: 41 with 256x256, 45 with 128x256.
+// caches less for each product (8192^3: 256 x 256 415 us, 128 x 256 475, 128 x 128 580, 64 x 64 880), smaller
+// ones leave fewer compute units idle. Around the switches, times in us:
+//   64 x 4096 x 4096     32x32 8.6   64x64 11          1024 x 4096 x 4096   128x128 20   128x256 25   256x256 42
+//   128 x 9216 x 3072    64x64 13.4  32x32 21          2048 x 4096 x 4096   128x256 33   128x128 37   256x256 44
+//   256 x 9216 x 3072    128x128 16  64x64 18          1024 x 12288 x 3072  256x256 41   128x256 45
+//   512 x 9216 x 3072    128x256 22  128x128 28        4608 x 3072 x 3072   256x256 40   128x256 44
 int choose_tile(uint32_t tokens, uint32_t rows) {
   int best = 0;
   double best_cost = 0;

@@ -45,7 +45,7 @@ constexpr uint32_t kFewPiecesNarrow = 64, kFewPiecesWide = 32;
 // The product's kernels, smallest tile first.
 struct MatmulTile {
   uint32_t tokens, rows, threads;
-  uint32_t cost;   // of 128 columns on a full chip, in 10 ns
+  uint32_t cost;    // of 128 columns on a full chip, in 10 ns
   bool fractional;  // several workgroups share a compute unit: a last round that is not full costs its share
 };
 constexpr MatmulTile kMatmulTiles[] = {

@@ -5,10 +5,23 @@
 // (2p, 2p + 1) when interleaved. The values past rot form pairs the same way with the angle 0, so
 // every pair is handled alike.
 //
+// With n = x r w, r = (mean(x^2) + eps)^(-1/2), and R the rotation by the token's angles: y = R n. For a gradient
+// dy, with g = R^-1 dy and x^ = x r: dw = sum over all heads and tokens of g x^, and dx = r (g w - x^ mean(g w x^)).
+// Both means come from one pass over a head's values: mean(g w x^) = r mean(g w x).
+//
 // The work is bound by HBM: each value is read once and written once (backward: two reads, one write). A
 // group of `lanes` work-items holds a head, kQkSlots pairs each, in registers: the statistics, the rotation and
-// the gradient need no second read and no shared memory. A group keeps its token's cosines and sines
-// while it takes the token's heads one after another, and the weights for its life.
+// the gradient need no second read and no shared memory, and the backward pass takes the statistics again
+// instead of reading them. A group keeps its token's cosines and sines while it takes the token's heads one
+// after another, and the weights for its life. The weights' gradients are summed in registers, over a
+// workgroup, and over the workgroups by a second small kernel, always in the same order.
+//
+// Measured: 4608 tokens x 48 heads of 128 bf16 20 us (5.7 TB/s; 24.5 us, 4.7 TB/s, where the caches do not help),
+// 2 x 8192 x 64 heads forward 100 us (5.4 TB/s) and backward 140 to 166 us (4.9 to 5.8 TB/s); a large copy 5.1 TB/s
+// by torch, 6.6 by this library's kernel. Heads of 64 4.4 TB/s: pieces of 128 bytes at the outputs' stride.
+// Scalar loads of single values took 5 times as long (115 us). Not kept: the next head's values loaded
+// ahead (113 against 108 us), consecutive tokens for one XCD (33 against 24.5 us at 4608 tokens), non-temporal
+// loads (10% slower backward) and stores (what the backward gained the next forward lost).
 
 #include <hip/hip_runtime.h>
 
