@@ -60,7 +60,7 @@ class Int8Weight:
 
     ``qweight`` is int8 ``(out_features, padded_in)``; ``in_features`` of its columns count (default:
     all). ``scale`` and the optional ``zero_point`` and ``bias`` hold ``out_features`` values; they are
-    kept in fp32. ``qweight`` is used where it lies if its rows start on 128-byte boundaries and its
+    constants here (no gradient), kept in fp32. ``qweight`` is used where it lies if its rows start on 128-byte boundaries and its
     memory holds all of the last row; changes of it are then seen by later calls. Otherwise it is copied
     once into such rows. With ``realign=False`` rows that start on 16-byte boundaries are used where
     they lie too: no copy, and 7% slower products of many tokens (4608 x 21504 x 3072: 288 us against

@@ -53,7 +53,7 @@ def _fields(x, q_heads, k_heads, weight, cos, positions, start, interleaved, eps
     batch, _, seq, dim = x.shape
     code = DTYPE_CODES[x.dtype]
     if cos is None:
-        table_rows = half_rot = table_ld = 0
+        table_rows = half_rot = table_ld = start = 0
     else:
         table_rows, half_rot = cos.shape
         table_ld = cos.stride(0)
@@ -177,6 +177,8 @@ def qk_norm_rope(
         _check_weight(k_weight, "k_weight", device, dim)
         if q_weight is not None and q_weight.dtype != k_weight.dtype:
             raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
+    if not 0.0 <= eps <= 1e38:
+        raise ValueError(f"eps {eps} is negative or not finite")
     grad_mode = torch.is_grad_enabled()
     if cos is not None and sin is not None:
         table = cos.shape

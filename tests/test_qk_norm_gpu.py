@@ -394,7 +394,7 @@ def test_refusals():
         lambda: qk_norm_rope(q, k, wq, wk, cos, sin, positions=p[:5]), lambda: qk_norm_rope(q, k, wq, wk, cos, sin, positions=p.float()),
         lambda: qk_norm_rope(q, k, wq, wk, cos, sin, positions=p.cpu()), lambda: qk_norm_rope(q, k, wq, wk, positions=p),
         lambda: qk_norm_rope(q, k, wq, wk, cos, sin, positions=p, start=1), lambda: qk_norm_rope(q, k, wq, wk, cos, sin, eps=-1.0),
-        lambda: qk_norm_rope(q, k, wq, wk, cos, sin, eps=float("nan")),
+        lambda: qk_norm_rope(q, k, wq, wk, cos, sin, eps=float("nan")), lambda: qk_norm_rope(q, k, wq, wk, cos, sin, eps=1e40),
         lambda: qk_norm_rope(q, k, wq, wk, cos.clone().requires_grad_(), sin),
         lambda: qk_norm_rope(q, k, wq, wk, cos, sin, out=(torch.empty_like(q), None)),
         lambda: qk_norm_rope(q, k, wq, wk, cos, sin, out=(torch.empty_like(q).float(), torch.empty_like(k))),
