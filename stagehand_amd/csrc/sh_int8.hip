@@ -267,18 +267,20 @@ __device__ __forceinline__ void load_to_lds(i32x4_t r, uint32_t lds, uint32_t of
                "s"(r));
 }
 
-// Stores N consecutive values; `whole`: all of them lie in the row, at a multiple of 16 bytes (or of all N).
+// Stores N consecutive values, or the first `count` of them. Whole runs are stored as vectors whatever their
+// address (gfx950 stores vectors anywhere).
 template <typename T, uint32_t N>
-__device__ __forceinline__ void store_run(T* out, const float (&v)[N], bool whole, uint32_t count) {
+__device__ __forceinline__ void store_run(T* out, const float (&v)[N], uint32_t count) {
   constexpr uint32_t kPer = N * sizeof(T) < 16 ? N : 16 / sizeof(T);
   typedef T Run __attribute__((ext_vector_type(kPer)));
-  if (whole) {
+  typedef Run RunAny __attribute__((aligned(2)));
+  if (count >= N) {
 #pragma unroll
     for (uint32_t i = 0; i < N / kPer; ++i) {
       Run x;
 #pragma unroll
       for (uint32_t j = 0; j < kPer; ++j) x[j] = (T)v[i * kPer + j];
-      *reinterpret_cast<Run*>(out + i * kPer) = x;
+      *reinterpret_cast<RunAny*>(out + i * kPer) = x;
     }
   } else {
 #pragma unroll
@@ -430,8 +432,6 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
     wz[j] = j < count && a.w_zp != nullptr ? a.w_zp[n + j] : 0.0f;
     wb[j] = j < count && a.bias != nullptr ? a.bias[n + j] : 0.0f;
   }
-  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
-  const bool whole = count == 16 && ((uintptr_t)a.out | a.out_ld * bytes | n * bytes) % 16 == 0;
   each<FT>([&](auto i) __attribute__((always_inline)) {
     constexpr uint32_t I = decltype(i)::value;
     const uint32_t t = t0 + wt * (TT / WT) + I * 16 + l16;
@@ -445,9 +445,9 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
       v[J] = __builtin_fmaf(-wz[J], sum, (float)acc[I][J / 4][J % 4]) * (scale * ws[J]) + wb[J];
     });
     const uint64_t at = (uint64_t)t * a.out_ld + n;
-    if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, v, whole, count);
-    else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, v, whole, count);
-    else store_run(static_cast<float*>(a.out) + at, v, whole, count);
+    if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, v, count);
+    else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, v, count);
+    else store_run(static_cast<float*>(a.out) + at, v, count);
   });
 }
 
@@ -475,12 +475,10 @@ __device__ __forceinline__ void store_joined(const sh::MatmulI8Args& a, const i3
     const float wb = in && a.bias != nullptr ? a.bias[n + r] : 0.0f;
     y[r] = __builtin_fmaf(-wz, (float)t_sum, (float)v[r]) * (scale * ws) + wb;
   }
-  const uint32_t bytes = a.out_dtype == SH_DTYPE_F32 ? 4 : 2;
   const uint64_t at = (uint64_t)t * a.out_ld + n;
-  const bool whole = count == 4 && ((uintptr_t)a.out | a.out_ld * bytes) % (4 * bytes) == 0;
-  if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, whole, count);
-  else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, y, whole, count);
-  else store_run(static_cast<float*>(a.out) + at, y, whole, count);
+  if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, count);
+  else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, y, count);
+  else store_run(static_cast<float*>(a.out) + at, y, count);
 }
 
 // 16 FT tokens x 16 FN rows by W wavefronts, each with every W-th 128 columns. A wavefront keeps a ring of D
