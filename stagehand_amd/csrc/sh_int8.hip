@@ -50,17 +50,26 @@ struct Chunk {
   static constexpr uint32_t kWords = sizeof(T) * 2;
   uint32_t w[kWords];
 
-  __device__ __forceinline__ void load(const T* p, uint32_t count) {
-    if (count >= 8) {
+  // The first `count` of them; the rest are 0. `beyond`: memory goes on for eight values past the end.
+  __device__ __forceinline__ void load(const T* p, uint32_t count, bool beyond) {
+    if (count >= 8 || (beyond && count > 0)) {
 #pragma unroll
       for (uint32_t i = 0; i < kWords / 4; ++i) {
         const u32x4 v = *(reinterpret_cast<const u32x4_a2*>(p) + i);
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) w[i * 4 + j] = v[j];
       }
+      if (count < 8) {
+#pragma unroll
+        for (uint32_t i = 0; i < kWords; ++i) {
+          if constexpr (sizeof(T) == 4) w[i] = i < count ? w[i] : 0;
+          else w[i] &= 2 * i + 1 < count ? 0xFFFFFFFFu : 2 * i < count ? 0xFFFFu : 0;
+        }
+      }
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < kWords; ++i) w[i] = 0;
+      if (count == 0) return;
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i)
@@ -150,6 +159,11 @@ __device__ __forceinline__ int32_t wave_sum(int32_t s) {
   return (int32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// Whether a token's end may be read eight values too far: another token of at least as many lies behind it.
+__device__ __forceinline__ bool goes_on(uint32_t t, uint32_t tokens, uint64_t ld, uint32_t cols) {
+  return t + 1 < tokens && ld >= cols && cols >= 8;
+}
+
 // WAVES wavefronts per token, C chunks of each work-item in registers between the maximum and the rounding:
 // the token is read once if its cols are at most WAVES * 512 * C, else its end is read twice (the second time
 // out of a cache). Bound by HBM: 16384 x 16384 bf16 145 us (5.6 TB/s), 8192 x 8192 31 us (6.5 TB/s, part of it
@@ -164,15 +178,16 @@ __device__ __forceinline__ void quantize_body(const sh::QuantizeArgs& a) {
   const T* x = static_cast<const T*>(a.x) + (uint64_t)t * a.x_ld;
   const uint32_t chunks = (uint32_t)(a.q_ld / 8);  // past cols they are zeros
   auto left = [&](uint32_t c) { return c * 8 < a.cols ? a.cols - c * 8 : 0; };
+  const bool beyond = goes_on(t, a.tokens, a.x_ld, a.cols);
   Chunk<T> held[C];
   uint32_t m = 0;
 #pragma unroll
-  for (uint32_t j = 0; j < C; ++j) held[j].load(x + (uint64_t)(j * kWide + me) * 8, left(j * kWide + me));
+  for (uint32_t j = 0; j < C; ++j) held[j].load(x + (uint64_t)(j * kWide + me) * 8, left(j * kWide + me), beyond);
 #pragma unroll
   for (uint32_t j = 0; j < C; ++j) m = held[j].amax(m);
   for (uint32_t c = C * kWide + me; c < chunks; c += kWide) {
     Chunk<T> v;
-    v.load(x + (uint64_t)c * 8, left(c));
+    v.load(x + (uint64_t)c * 8, left(c), beyond);
     m = v.amax(m);
   }
   m = wave_max(amax_bits<T>(m));
@@ -199,7 +214,7 @@ __device__ __forceinline__ void quantize_body(const sh::QuantizeArgs& a) {
     if (j * kWide + me < chunks) put(held[j], j * kWide + me);
   for (uint32_t c = C * kWide + me; c < chunks; c += kWide) {
     Chunk<T> v;
-    v.load(x + (uint64_t)c * 8, left(c));
+    v.load(x + (uint64_t)c * 8, left(c), beyond);
     put(v, c);
   }
   sum = wave_sum(sum);
@@ -589,7 +604,8 @@ __device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* r
     token_of[j] = t;
     at_of[j] = at;
     if (t < a.tokens)
-      held[j].load(static_cast<const T*>(a.tq) + (uint64_t)t * a.t_ld + at, at < a.cols ? a.cols - at : 0);
+      held[j].load(static_cast<const T*>(a.tq) + (uint64_t)t * a.t_ld + at, at < a.cols ? a.cols - at : 0,
+                   goes_on(t, a.tokens, a.t_ld, a.cols));
   }
   if (threadIdx.x < 16) {
     amax[threadIdx.x] = 0;

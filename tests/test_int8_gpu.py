@@ -115,6 +115,23 @@ def test_quantize_tokens_of_strided_and_offset_views():
         assert t.shape == x.shape[:-1] and t.dequantize().shape == x.shape
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [8, 9, 15, 203, 517, 2047])
+def test_a_token_does_not_see_the_next_one(cols, dtype):
+    """Ragged ends with infinities and NaNs right behind them, rows that overlap, and a last row that ends its memory."""
+    x = torch.randn(12, cols).to(dtype)
+    x[1::2, :8] = torch.tensor([float("inf"), float("nan"), float("-inf"), float("nan")] * 2)
+    for v in (x.cuda(), x.cuda()[::2], x.cuda()[::2][:1].expand(5, cols), x.cuda().reshape(-1)[:cols * 8].as_strided((7, cols), (3, 1))):
+        t = quantize_tokens(v)
+        q, scale, sums = np_quantize(v.float().cpu().numpy())
+        np.testing.assert_array_equal(t.q.cpu().numpy()[:, :cols], q)
+        np.testing.assert_array_equal(t.scale.cpu().numpy(), scale)
+        np.testing.assert_array_equal(t.sums.cpu().numpy(), sums)
+        w = Int8Weight(torch.ones(3, cols, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))
+        few = linear_i8(v, w).isnan().any(1).cpu().numpy()
+        np.testing.assert_array_equal(few, np.isnan(scale))
+
+
 # ── the product ──────────────────────────────────────────────────────────────
 
 SIZES = [  # tokens, out, inp
