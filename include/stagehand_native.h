@@ -751,7 +751,9 @@ int sh_quantize_tokens(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t to
  * rounded once to out_dtype; rows of out are out_ld elements apart. The int8
  * products are summed exactly, in 32 bits. q, scale and sums as
  * sh_quantize_tokens writes them for w.cols columns (sums is read only where w
- * has zero points). out must not overlap the inputs. */
+ * has zero points); of each token's row the first w.cols bytes, rounded up to
+ * SH_I8_TOKEN_ALIGN, are read, zeros past w.cols, so the rows may be some of a
+ * larger matrix's. out must not overlap the inputs. */
 int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, const int32_t* sums, uint32_t tokens,
                  const sh_i8_weight* w, void* out, uint32_t out_dtype, uint64_t out_ld, void* stream);
 /* Both: out = quantised(x) * W^T + bias, in the type of x. The results are

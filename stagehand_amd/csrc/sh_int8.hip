@@ -257,18 +257,23 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 constexpr uint32_t kPastEnd = 0x80000000u;  // an offset outside every resource
 constexpr uint32_t kStep = 128;  // bytes of a row that one stage holds: a cache line, two MFMAs'
 
+// Bytes of a quantised token that are multiplied: whole steps, zeros past cols. How far apart the tokens lie has no
+// part in it.
+__device__ __forceinline__ constexpr uint32_t token_bytes(uint32_t cols) { return (cols + kStep - 1) / kStep * kStep; }
+
 // The 16-byte chunk c of a stage's row lies in slot c ^ swizzle(row): the 16 rows of a fragment then lie in
 // different LDS banks.
 __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t row) { return (row >> 1) & 7; }
 
-// Buffer resource of up to `tile` rows from row `first` on: reads past them give 0.
-__device__ __forceinline__ i32x4_t rows_resource(const void* base, uint64_t ld, uint32_t first, uint32_t count,
-                                                 uint32_t tile) {
+// Buffer resource of up to `tile` rows from row `first` on, each `width` of the `ld` bytes to the next: reads past
+// the last row's width give 0.
+__device__ __forceinline__ i32x4_t rows_resource(const void* base, uint64_t ld, uint64_t width, uint32_t first,
+                                                 uint32_t count, uint32_t tile) {
   const uint64_t p = (uint64_t)base + (uint64_t)first * ld;
   i32x4_t r;
   r[0] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)p);
   r[1] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(p >> 32) & 0xFFFF);  // stride 0
-  r[2] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)(min(count - first, tile) * ld));
+  r[2] = __builtin_amdgcn_readfirstlane((int32_t)(uint32_t)((min(count - first, tile) - 1) * ld + width));
   r[3] = 0x00020000;
   return r;
 }
@@ -347,8 +352,9 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
   const uint32_t group = p / (GROUP * tiles_n), in_group = p % (GROUP * tiles_n);
   const uint32_t g_rows = min(tiles_t - group * GROUP, GROUP);
   const uint32_t t0 = (group * GROUP + in_group % g_rows) * TT, n0 = in_group / g_rows * TN;
-  const i32x4_t tr = rows_resource(a.tq, a.t_ld, t0, a.tokens, TT);
-  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, TN);
+  const uint32_t end = token_bytes(a.cols);
+  const i32x4_t tr = rows_resource(a.tq, a.t_ld, end, t0, a.tokens, TT);
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, a.w_ld, n0, a.rows, TN);
 
   // Lane l of a load brings slot l % 8 of row l / 8. The rows of the weight lie permuted in LDS, so that the
   // MFMA results of one lane are 16 consecutive ones: fragment f, row i holds row (i / 4) * 16 + f * 4 + i % 4
@@ -364,7 +370,6 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
     n_off[decltype(j)::value] = src * (uint32_t)a.w_ld + ((lane % 8) ^ swizzle(row)) * 16;
   });
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 1024;
-  const uint32_t end = (uint32_t)a.t_ld;  // a multiple of kStep; the tokens are zero past cols
   // Load i of a stage: first the tokens', then the rows'. Past the end the offset is outside the resource: such
   // a load reads nothing and keeps the count of loads in flight the same.
   auto load = [&](auto i, uint32_t stage, uint32_t k) __attribute__((always_inline)) {
@@ -509,8 +514,9 @@ __device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t tiles_n = (a.rows + 16 * FN - 1) / (16 * FN);
   const uint32_t t0 = blockIdx.x / tiles_n * (16 * FT), n0 = blockIdx.x % tiles_n * (16 * FN);
-  const i32x4_t tr = rows_resource(a.tq, a.t_ld, t0, a.tokens, 16 * FT);
-  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, 16 * FN);
+  const uint32_t end = token_bytes(a.cols);
+  const i32x4_t tr = rows_resource(a.tq, a.t_ld, end, t0, a.tokens, 16 * FT);
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, a.w_ld, n0, a.rows, 16 * FN);
   // row + 8 has the swizzle of row with bit 2 changed: two offsets cover every load
   const uint32_t row = lane / 8, slot = lane % 8;
   const uint32_t s0 = (slot ^ swizzle(row)) * 16, s1 = (slot ^ swizzle(row + 8)) * 16;
@@ -527,7 +533,6 @@ __device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t
   const uint32_t l16 = lane & 15, part = lane / 16;
   const uint8_t* mine = lds + wave * D * kStage + l16 * kStep;
   i32x4_t acc[FT][FN] = {};
-  const uint32_t end = t_ld;
 #pragma unroll
   for (uint32_t i = 0; i < D; ++i) {
     const uint32_t k = (i * W + wave) * kStep;
@@ -590,7 +595,7 @@ __device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* r
   constexpr uint32_t kMine = PIECES / W;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t n0 = blockIdx.x * (16 * FN);
-  const uint32_t end = (a.cols + kStep - 1) / kStep * kStep;
+  const uint32_t end = token_bytes(a.cols);
   const uint32_t q_ld = end + 16;  // 16 bytes more: the rows of a fragment in different LDS banks
   const uint32_t pieces = (a.cols + 511) / 512;
 
@@ -620,7 +625,7 @@ __device__ __forceinline__ void linear_few(const sh::MatmulI8Args& a, uint8_t* r
     if (lane == 0) atomicMax(amax + t, m);
   }
 
-  const i32x4_t wr = rows_resource(a.wq, a.w_ld, n0, a.rows, 16 * FN);
+  const i32x4_t wr = rows_resource(a.wq, a.w_ld, a.w_ld, n0, a.rows, 16 * FN);
   const uint32_t row = lane / 8, slot = lane % 8;
   const uint32_t s0 = (slot ^ swizzle(row)) * 16, s1 = (slot ^ swizzle(row + 8)) * 16;
   const uint32_t w_ld = (uint32_t)a.w_ld;

@@ -31,6 +31,7 @@ __all__ = ["Int8Weight", "Int8Tokens", "quantize_tokens", "matmul_i8", "linear_i
 
 MAX_COLS = 131071  # SH_I8_MAX_COLS
 TOKEN_ALIGN = 128  # SH_I8_TOKEN_ALIGN
+MAX_LD = 1 << 20  # bytes between rows
 DTYPE_CODES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}  # enum sh_dtype
 
 
@@ -131,7 +132,7 @@ def _aligned_rows(q: torch.Tensor, align: int) -> torch.Tensor:
     """``q`` itself where its rows start on multiples of ``align`` bytes, else a copy in such rows."""
     rows, cols = q.shape
     ld = q.stride(0) if rows > 1 else _round_up(cols, align)
-    if (cols == 1 or q.stride(1) == 1) and ld % align == 0 and cols <= ld <= 1 << 20 and q.data_ptr() % align == 0 and \
+    if (cols == 1 or q.stride(1) == 1) and ld % align == 0 and cols <= ld <= MAX_LD and q.data_ptr() % align == 0 and \
             q.untyped_storage().nbytes() - q.storage_offset() >= rows * ld:
         return q
     padded = torch.zeros((rows, _round_up(cols, align)), dtype=torch.int8, device=q.device)
@@ -218,7 +219,10 @@ def quantize_tokens(x: torch.Tensor, stream: torch.cuda.Stream | int | None = No
 
 def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None = None,
               out_dtype: torch.dtype | None = None, stream: torch.cuda.Stream | int | None = None) -> torch.Tensor:
-    """``tokens · weightᵀ + bias`` in ``out_dtype`` (default bfloat16, or that of ``out``)."""
+    """``tokens · weightᵀ + bias`` in ``out_dtype`` (default bfloat16, or that of ``out``).
+
+    ``tokens.q`` may be rows of a larger tensor (every second token, the last one of each sequence, some of
+    its columns): rows on multiples of 128 bytes, up to 1 MiB apart, are read in place, others are copied."""
     if stream is not None:
         with on_stream(stream):
             return matmul_i8(tokens, weight, out, out_dtype)
@@ -226,8 +230,9 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
     if cols != weight.in_features:
         raise ValueError(f"the tokens have {cols} values, the weight takes {weight.in_features}")
     n = q.shape[0] if q.dim() == 2 else -1
-    if q.dtype != torch.int8 or n < 0 or q.shape[1] < cols or (q.numel() and q.stride(1) != 1):
-        raise ValueError(f"tokens.q must be int8 rows of at least {cols} values, got {q.dtype} {tuple(q.shape)}")
+    width = _round_up(cols, TOKEN_ALIGN)
+    if q.dtype != torch.int8 or n < 0 or q.shape[1] < width or (q.numel() and q.stride(1) != 1):
+        raise ValueError(f"tokens.q must be int8 rows of {cols} values and zeros up to {width}, got {q.dtype} {tuple(q.shape)}")
     if scale.dtype != torch.float32 or sums.dtype != torch.int32 or scale.shape != (n,) or sums.shape != (n,) or \
             not scale.is_contiguous() or not sums.is_contiguous():
         raise ValueError("tokens.scale and tokens.sums must be contiguous float32 and int32 with one value per token")
@@ -238,8 +243,10 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
     dtype = out_dtype if out_dtype is not None else torch.bfloat16 if out is None else out.dtype
     if dtype not in DTYPE_CODES:
         raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {dtype}")
-    ld = q.stride(0) if n > 1 else q.shape[1]
+    ld = q.stride(0) if n > 1 else width
     with torch.cuda.device(weight.device):
+        if ld % TOKEN_ALIGN or not width <= ld <= MAX_LD or q.data_ptr() % 16:
+            q, ld = q[:, :width].clone(memory_format=torch.contiguous_format), width
         y, out_ld = _output(out, (*shape, weight.out_features), dtype, weight.device)
         _native.call("sh_matmul_i8", q.data_ptr(), ld, scale.data_ptr(), sums.data_ptr(), n, weight._ref, y.data_ptr(),
                      DTYPE_CODES[dtype], out_ld, current_stream_handle())
