@@ -15,7 +15,8 @@ have to record one is refused.
 
 Everything runs on the caller's current torch stream unless ``stream`` is given; outputs and
 workspaces are allocated on that stream. As with any torch operator, inputs that were made on
-another stream must be ready, and kept, for it. There is no CPU path.
+another stream must be ready, and kept, for it. ``out`` is written in place: it must not share memory
+with the inputs, and a backward pass that needs its old values raises. There is no CPU path.
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ import ctypes
 from typing import Any, NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from stagehand_amd import _native
 from stagehand_amd.unpack import current_stream_handle
@@ -250,6 +252,8 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
         y, out_ld = _output(out, (*shape, weight.out_features), dtype, weight.device)
         _native.call("sh_matmul_i8", q.data_ptr(), ld, scale.data_ptr(), sums.data_ptr(), n, weight._ref, y.data_ptr(),
                      DTYPE_CODES[dtype], out_ld, current_stream_handle())
+    if out is not None:
+        increment_version(out)
     return y
 
 
@@ -281,4 +285,6 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = No
     ws = x.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _native.check(lib.sh_linear_i8(rows.data_ptr(), code, ld, tokens, weight._ref, y.data_ptr(), out_ld,
                                    None if ws is None else ws.data_ptr(), need.value, current_stream_handle()))
+    if out is not None:
+        increment_version(out)
     return y

@@ -17,6 +17,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from stagehand_amd import _native
 from stagehand_amd.int8 import DTYPE_CODES, on_stream
@@ -151,7 +152,8 @@ def qk_norm_rope(
     tables do not have gives NaN for that token).
 
     The outputs are contiguous, or written to ``out``: tensors of the same shapes with any strides
-    that keep a head's values together (a slice of a joint sequence, or ``q`` and ``k`` themselves).
+    that keep a head's values together (a slice of a joint sequence, or ``q`` and ``k`` themselves, but no
+    other memory of the inputs'). A backward pass that needs the old values of ``out`` raises.
     Gradients flow to ``q``, ``k`` and the weights, not to the tables, and not through ``out``."""
     if stream is not None:
         with on_stream(stream):
@@ -232,4 +234,6 @@ def qk_norm_rope(
                 raise ValueError(f"out for {what} must be {dtype} {tuple(x.shape)} with contiguous heads on q's device, "
                                  f"got {o.device} {o.dtype} {tuple(o.shape)} strides {o.stride()}")
     _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
+    if out is not None:
+        increment_version([o for o in (q_out, k_out) if o is not None])
     return q_out, k_out
