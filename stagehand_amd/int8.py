@@ -58,6 +58,11 @@ def check_device(t: torch.Tensor, device: torch.device | None, what: str) -> Non
         raise ValueError(f"{what} is on {t.device}, not on {device}")
 
 
+def check_no_grad(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what} requires grad, but what is written to it has no gradient: call under torch.no_grad()")
+
+
 class Int8Weight:
     """A SquareQ weight in device memory, as :func:`linear_i8` takes it.
 
@@ -183,6 +188,7 @@ def _output(out: torch.Tensor | None, shape: tuple[int, ...], dtype: torch.dtype
         out = torch.empty(shape, dtype=dtype, device=device)
         return out, shape[-1]
     check_device(out, device, "out")
+    check_no_grad(out, "out")
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise ValueError(f"out must be {dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     try:

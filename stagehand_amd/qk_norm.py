@@ -20,7 +20,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from stagehand_amd import _native
-from stagehand_amd.int8 import DTYPE_CODES, on_stream
+from stagehand_amd.int8 import DTYPE_CODES, check_no_grad, on_stream
 from stagehand_amd.unpack import current_stream_handle
 
 __all__ = ["qk_norm_rope"]
@@ -233,6 +233,7 @@ def qk_norm_rope(
             if o.get_device() != device or o.shape != x.shape or o.dtype != dtype or o.stride(3) != 1:
                 raise ValueError(f"out for {what} must be {dtype} {tuple(x.shape)} with contiguous heads on q's device, "
                                  f"got {o.device} {o.dtype} {tuple(o.shape)} strides {o.stride()}")
+            check_no_grad(o, f"out for {what}")
     _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
     if out is not None:
         increment_version([o for o in (q_out, k_out) if o is not None])

@@ -63,3 +63,23 @@ def test_only_outputs_change_their_version():
         x = torch.randn(3, 96, device="cuda")
         linear_i8(x, weight(), out=torch.empty(3, 64, device="cuda"))
 
+
+# ── out= that requires a gradient ────────────────────────────────────────────
+
+
+def test_out_that_requires_grad_is_refused():
+    w, x = weight(), torch.randn(4, 96, device="cuda")
+    out = torch.zeros(4, 64, device="cuda", requires_grad=True)
+    q, k = heads(1, 2, 5, 32), heads(1, 2, 5, 32)
+    qo, ko = torch.zeros_like(q).requires_grad_(), torch.zeros_like(k)
+    calls = [lambda: linear_i8(x, w, out=out), lambda: matmul_i8(quantize_tokens(x), w, out=out),
+             lambda: linear_i8(x, w, out=(out * 1)), lambda: qk_norm_rope(q, k, out=(qo, ko)),
+             lambda: qk_norm_rope(q, k, out=(ko, qo))]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+    assert not out.any() and not qo.any() and not ko.any()
+    with torch.no_grad():  # as any in-place operation
+        assert torch.equal(linear_i8(x, w, out=out), linear_i8(x, w))
+        assert torch.equal(qk_norm_rope(q, k, out=(qo, ko))[0], qk_norm_rope(q, k)[0])
+
