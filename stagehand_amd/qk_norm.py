@@ -127,6 +127,20 @@ def _like(x: torch.Tensor) -> torch.Tensor:
     return d if d.stride(3) == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+def _heads_overlap(t: torch.Tensor) -> bool:
+    """Whether heads of ``t`` may share memory: some distance between heads is less than what lies within it.
+    (Slices, permutations and windows of a dense tensor never do.)"""
+    if t.numel() == 0:
+        return False
+    reach = t.shape[3]
+    for stride, size in sorted(zip(t.stride()[:3], t.shape)):
+        if size > 1:
+            if stride < reach:
+                return True
+            reach += (size - 1) * stride
+    return False
+
+
 def qk_norm_rope(
     q: torch.Tensor,
     k: torch.Tensor | None,
@@ -233,6 +247,8 @@ def qk_norm_rope(
             if o.get_device() != device or o.shape != x.shape or o.dtype != dtype or o.stride(3) != 1:
                 raise ValueError(f"out for {what} must be {dtype} {tuple(x.shape)} with contiguous heads on q's device, "
                                  f"got {o.device} {o.dtype} {tuple(o.shape)} strides {o.stride()}")
+            if _heads_overlap(o):
+                raise ValueError(f"heads of out for {what} share memory: {tuple(o.shape)} with strides {o.stride()}")
             check_no_grad(o, f"out for {what}")
     _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
     if out is not None:
