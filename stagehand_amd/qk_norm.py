@@ -20,7 +20,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from stagehand_amd import _native
-from stagehand_amd.int8 import DTYPE_CODES, check_no_grad, on_stream
+from stagehand_amd.int8 import DTYPE_CODES, check_no_grad, check_no_tangent, on_stream
 from stagehand_amd.unpack import current_stream_handle
 
 __all__ = ["qk_norm_rope"]
@@ -195,6 +195,7 @@ def qk_norm_rope(
             raise ValueError(f"q_weight and k_weight must have one type, got {q_weight.dtype} and {k_weight.dtype}")
     if not 0.0 <= eps <= 1e38:
         raise ValueError(f"eps {eps} is negative or not finite")
+    check_no_tangent("qk_norm_rope", q, k, q_weight, k_weight, cos, sin)
     grad_mode = torch.is_grad_enabled()
     if cos is not None and sin is not None:
         table = cos.shape
@@ -250,6 +251,7 @@ def qk_norm_rope(
             if _heads_overlap(o):
                 raise ValueError(f"heads of out for {what} share memory: {tuple(o.shape)} with strides {o.stride()}")
             check_no_grad(o, f"out for {what}")
+            check_no_tangent(f"out for {what}", o)
     _run(q, k, q_weight, k_weight, cos, sin, positions, start, interleaved, eps, q_out, k_out)
     if out is not None:
         increment_version([o for o in (q_out, k_out) if o is not None])

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from stagehand_amd.int8 import Int8Weight, linear_i8, matmul_i8, quantize_tokens
 from stagehand_amd.qk_norm import qk_norm_rope
@@ -82,4 +83,45 @@ def test_out_that_requires_grad_is_refused():
     with torch.no_grad():  # as any in-place operation
         assert torch.equal(linear_i8(x, w, out=out), linear_i8(x, w))
         assert torch.equal(qk_norm_rope(q, k, out=(qo, ko))[0], qk_norm_rope(q, k)[0])
+
+
+# ── forward-mode derivatives ─────────────────────────────────────────────────
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_tangents_are_refused(grad_mode):
+    w, x = weight(), torch.randn(4, 96, device="cuda")
+    q, k = heads(1, 2, 5, 32).float(), heads(1, 2, 5, 32).float()
+    n, cos = torch.ones(32, device="cuda"), torch.ones(5, 16, device="cuda")
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = [lambda: linear_i8(dual(x), w), lambda: quantize_tokens(dual(x)),
+                 lambda: matmul_i8(quantize_tokens(x)._replace(scale=dual(torch.ones(4, device="cuda"))), w),
+                 lambda: linear_i8(x, w, out=dual(torch.zeros(4, 64, device="cuda"))),
+                 lambda: qk_norm_rope(dual(q), k, n, n, cos, cos), lambda: qk_norm_rope(q, dual(k), n, n, cos, cos),
+                 lambda: qk_norm_rope(q, k, dual(n), n, cos, cos), lambda: qk_norm_rope(q, k, n, dual(n), cos, cos),
+                 lambda: qk_norm_rope(q, k, n, n, dual(cos), cos), lambda: qk_norm_rope(q, k, n, n, cos, dual(cos)),
+                 lambda: qk_norm_rope(q, None, out=(dual(torch.zeros_like(q)), None))]
+        if grad_mode:
+            calls.append(lambda: qk_norm_rope(dual(q), k, n.clone().requires_grad_(), n, cos, cos))
+        for i, call in enumerate(calls):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was not refused")
+        # nothing that has a tangent: as always
+        assert torch.equal(linear_i8(x, w), matmul_i8(quantize_tokens(x), w, out_dtype=torch.float32))
+        qk_norm_rope(q, k, n, n, cos, cos)
+
+
+def test_transforms_of_torch_func_are_refused():
+    w, x, q = weight(), torch.randn(4, 96, device="cuda"), heads(1, 2, 5, 32).float()
+    for f, at in ((lambda t: linear_i8(t, w), x), (lambda t: qk_norm_rope(t, None)[0], q)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (at,), (torch.ones_like(at),))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(torch.stack((at, at)))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(at)
 
