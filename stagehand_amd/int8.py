@@ -256,6 +256,8 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
     if scale.dtype != torch.float32 or sums.dtype != torch.int32 or scale.shape != (n,) or sums.shape != (n,) or \
             not scale.is_contiguous() or not sums.is_contiguous():
         raise ValueError("tokens.scale and tokens.sums must be contiguous float32 and int32 with one value per token")
+    if scale.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("matmul_i8 is for inference and has no gradient: call it under torch.no_grad()")
     check_no_tangent("matmul_i8", scale)
     if torch.Size(shape).numel() != n:
         raise ValueError(f"tokens.shape {tuple(shape)} does not hold {n} tokens")

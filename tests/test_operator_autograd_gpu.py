@@ -125,3 +125,11 @@ def test_transforms_of_torch_func_are_refused():
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: f(t).sum())(at)
 
+
+def test_token_scales_that_require_grad_are_refused():
+    t = quantize_tokens(torch.randn(4, 96, device="cuda"))
+    t = t._replace(scale=t.scale.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        matmul_i8(t, weight())
+    with torch.no_grad():
+        matmul_i8(t, weight())
