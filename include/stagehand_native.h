@@ -753,7 +753,9 @@ int sh_quantize_tokens(const void* x, uint32_t dtype, uint64_t x_ld, uint32_t to
  * sh_quantize_tokens writes them for w.cols columns (sums is read only where w
  * has zero points); of each token's row the first w.cols bytes, rounded up to
  * SH_I8_TOKEN_ALIGN, are read, zeros past w.cols, so the rows may be some of a
- * larger matrix's. out must not overlap the inputs. */
+ * larger matrix's. Scales of tokens may be as small and as large as
+ * sh_quantize_tokens writes them, those of rows 2^-62 to 2^62 beside them: what
+ * fits out is not lost on the way. out must not overlap the inputs. */
 int sh_matmul_i8(const void* q, uint64_t q_ld, const float* scale, const int32_t* sums, uint32_t tokens,
                  const sh_i8_weight* w, void* out, uint32_t out_dtype, uint64_t out_ld, void* stream);
 /* Both: out = quantised(x) * W^T + bias, in the type of x. The results are

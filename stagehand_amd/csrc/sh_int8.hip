@@ -38,6 +38,21 @@ __device__ __forceinline__ void token_scale(uint32_t amax_bits, float* inv, floa
   }
 }
 
+// A token's scale as a factor for the rows' scales, within 2^-64 and 2^65, and what is left, a power of two, for the
+// token's sums (1 for all ordinary scales): the outputs are (sum on_sum) (w on_row) + bias. scale * w by itself
+// would overflow, or lose its bits below 2^-126, where the output is an ordinary number: scales go from 2^-127 to
+// 2^121. These products do so only for rows' scales under 2^-62 or over 2^62.
+struct TokenFactors {
+  float on_sum, on_row;
+};
+__device__ __forceinline__ bool ordinary(float scale) { return scale >= 0x1p-64f && scale < 0x1p65f; }
+__device__ __forceinline__ TokenFactors token_factors(float scale) {
+  if (ordinary(scale)) return {1.0f, scale};
+  const uint32_t e = __builtin_bit_cast(uint32_t, scale) >> 23 & 0xFF, near = min(max(e, 127u - 64), 127u + 64);
+  const uint32_t rest = 127 + max(e, 1u) - near;  // subnormal scales have the exponent 1, too
+  return {__builtin_bit_cast(float, rest << 23), scale * __builtin_bit_cast(float, (254 - rest) << 23)};
+}
+
 // ── quantisation ──────────────────────────────────────────────────────────
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -459,11 +474,16 @@ __device__ __forceinline__ void matmul_tile(const sh::MatmulI8Args& a, uint8_t* 
     const float scale = a.t_scale[t];
     const float sum = a.w_zp != nullptr ? (float)a.t_sums[t] : 0.0f;
     float v[16];
-    each<16>([&](auto j) __attribute__((always_inline)) {
-      constexpr uint32_t J = decltype(j)::value;
-      // wz is 0 without zero points: the same value
-      v[J] = __builtin_fmaf(-wz[J], sum, (float)acc[I][J / 4][J % 4]) * (scale * ws[J]) + wb[J];
-    });
+    auto finish = [&](TokenFactors f) __attribute__((always_inline)) {
+      each<16>([&](auto j) __attribute__((always_inline)) {
+        constexpr uint32_t J = decltype(j)::value;
+        // wz is 0 without zero points: the same value
+        const float acc_z = __builtin_fmaf(-wz[J], sum, (float)acc[I][J / 4][J % 4]);
+        v[J] = __builtin_fmaf(acc_z * f.on_sum, ws[J] * f.on_row, wb[J]);
+      });
+    };
+    if (ordinary(scale)) finish({1.0f, scale});  // two paths: one product less for each output
+    else finish(token_factors(scale));
     const uint64_t at = (uint64_t)t * a.out_ld + n;
     if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, v, count);
     else if (a.out_dtype == SH_DTYPE_F16) store_run(static_cast<_Float16*>(a.out) + at, v, count);
@@ -486,6 +506,7 @@ __device__ __forceinline__ void store_joined(const sh::MatmulI8Args& a, const i3
 #pragma unroll
   for (uint32_t w = 1; w < W; ++w) v += sums[w * 64];
   const uint32_t count = min(a.rows - n, 4u);
+  const TokenFactors f = token_factors(scale);
   float y[4];
 #pragma unroll
   for (uint32_t r = 0; r < 4; ++r) {
@@ -493,7 +514,7 @@ __device__ __forceinline__ void store_joined(const sh::MatmulI8Args& a, const i3
     const float ws = in ? a.w_scale[n + r] : 0.0f;
     const float wz = in && a.w_zp != nullptr ? a.w_zp[n + r] : 0.0f;
     const float wb = in && a.bias != nullptr ? a.bias[n + r] : 0.0f;
-    y[r] = __builtin_fmaf(-wz, (float)t_sum, (float)v[r]) * (scale * ws) + wb;
+    y[r] = __builtin_fmaf(__builtin_fmaf(-wz, (float)t_sum, (float)v[r]) * f.on_sum, ws * f.on_row, wb);
   }
   const uint64_t at = (uint64_t)t * a.out_ld + n;
   if (a.out_dtype == SH_DTYPE_BF16) store_run(static_cast<__bf16*>(a.out) + at, y, count);

@@ -1,0 +1,48 @@
+"""Int8 linear layers at the ends of their ranges: token scales from 2^-127 to the type's largest. Tolerances as in test_int8_gpu."""
+from __future__ import annotations
+
+import pytest
+import torch
+from test_int8_gpu import check, make
+
+from stagehand_amd.int8 import Int8Weight, linear_i8, matmul_i8, quantize_tokens
+
+pytestmark = pytest.mark.gpu
+
+# tokens, out, inp: one launch, two with few tokens, and the tiles
+SIZES = [(3, 100, 200), (5, 9000, 300), (24, 9000, 100), (40, 100, 130), (100, 900, 200), (250, 9200, 130), (600, 4100, 140),
+         (1100, 8200, 260)]
+
+
+def scaled(tokens, out, inp, dtype, zp, exponents, row_exponents):
+    """Tokens and rows whose magnitudes are spread evenly over the exponents given."""
+    x, q, _, z, _, _ = make(tokens, out, inp, zp=zp, bias=False, dtype=torch.float32, seed=tokens)
+    g = torch.Generator().manual_seed(1)
+    e = torch.linspace(*exponents, tokens).round()[torch.randperm(tokens, generator=g)]
+    x = x / x.abs().amax(1, keepdim=True)  # largest magnitude 1
+    x = (x.double() * torch.exp2(e.double())[:, None]).float().to(dtype)
+    r = torch.linspace(*row_exponents, out).round()[torch.randperm(out, generator=g)]
+    s = ((1 + torch.rand(out, generator=g).double()) * torch.exp2(r.double())).float()
+    return x, q, s, z, None, Int8Weight(q.cuda(), s.cuda(), None if z is None else z.cuda(), None, inp)
+
+
+@pytest.mark.parametrize("zp", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,out,inp", SIZES)
+@pytest.mark.parametrize("exponents,row_exponents", [((-119, -100), (-20, 0)), ((100, 127), (-60, -40)), ((-119, 127), (-30, -30)),
+                                                     ((-119, -119), (40, 60))])
+def test_token_scales_of_any_size(tokens, out, inp, dtype, zp, exponents, row_exponents):
+    x, q, s, z, b, w = scaled(tokens, out, inp, dtype, zp, exponents, row_exponents)
+    got = linear_i8(x.cuda(), w)
+    check(got, x, q, s, z, b)
+    assert torch.equal(got, matmul_i8(quantize_tokens(x.cuda()), w, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 300])
+def test_a_sum_of_zero_is_zero_whatever_its_scales(tokens):
+    """Scales whose product overflows, where the integers cancel: the bias, not NaN."""
+    x = torch.full((tokens, 64), 3e38)
+    x[:, ::2] = -3e38
+    b = torch.randn(70)
+    w = Int8Weight(torch.full((70, 64), 5, dtype=torch.int8, device="cuda"), torch.full((70,), 1e10, device="cuda"), bias=b.cuda())
+    assert torch.equal(linear_i8(x.cuda(), w).cpu(), b.expand(tokens, 70))
