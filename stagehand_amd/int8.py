@@ -35,6 +35,7 @@ __all__ = ["Int8Weight", "Int8Tokens", "quantize_tokens", "matmul_i8", "linear_i
 MAX_COLS = 131071  # SH_I8_MAX_COLS
 TOKEN_ALIGN = 128  # SH_I8_TOKEN_ALIGN
 MAX_LD = 1 << 20  # bytes between rows
+INTEGERS = (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64)
 DTYPE_CODES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}  # enum sh_dtype
 
 
@@ -78,7 +79,7 @@ class Int8Weight:
 
     ``qweight`` is int8 ``(out_features, padded_in)``; ``in_features`` of its columns count (default:
     all). ``scale`` and the optional ``zero_point`` and ``bias`` hold ``out_features`` values; they are
-    constants here (no gradient), kept in fp32. ``qweight`` is used where it lies if its rows start on 128-byte boundaries and its
+    constants here (no gradient), kept in fp32; zero points may be integers. ``qweight`` is used where it lies if its rows start on 128-byte boundaries and its
     memory holds all of the last row; changes of it are then seen by later calls. Otherwise it is copied
     once into such rows. With ``realign=False`` rows that start on 16-byte boundaries are used where
     they lie too: no copy, and 7% slower products of many tokens (4608 x 21504 x 3072: 288 us against
@@ -98,6 +99,8 @@ class Int8Weight:
         align = 128 if realign else 16
         self.qweight = _aligned_rows(qweight[:, :cols], align)
         self.scale = self._per_row(scale, "scale")
+        if zero_point is not None and zero_point.dtype in INTEGERS:
+            zero_point = zero_point.float()
         self.zero_point = None if zero_point is None else self._per_row(zero_point, "zero_point")
         self.bias = None if bias is None else self._per_row(bias, "bias")
         ld = self.qweight.stride(0) if rows > 1 else _round_up(cols, align)

@@ -1,4 +1,5 @@
-"""Int8 linear layers at the ends of their ranges: token scales from 2^-127 to the type's largest. Tolerances as in test_int8_gpu."""
+"""Int8 linear layers at the ends of their ranges: token scales from 2^-127 to the type's largest, integer zero
+points. Tolerances as in test_int8_gpu."""
 from __future__ import annotations
 
 import pytest
@@ -46,3 +47,20 @@ def test_a_sum_of_zero_is_zero_whatever_its_scales(tokens):
     b = torch.randn(70)
     w = Int8Weight(torch.full((70, 64), 5, dtype=torch.int8, device="cuda"), torch.full((70,), 1e10, device="cuda"), bias=b.cuda())
     assert torch.equal(linear_i8(x.cuda(), w).cpu(), b.expand(tokens, 70))
+
+
+def test_integer_zero_points():
+    """A slab may hold its zero points as integers; the dequantising path takes them too."""
+    x, q, s, _, b, _ = make(20, 50, 90, seed=4)
+    z = torch.randint(-100, 100, (50,))
+    for zdt in (torch.int8, torch.int16, torch.int32, torch.int64):
+        zi = z.to(zdt)
+        w = Int8Weight(q.cuda(), s.cuda(), zi.cuda(), b.cuda())
+        check(linear_i8(x.cuda(), w), x, q, s, z.float(), b)
+        ws = Int8Weight.from_squareq({"qweight": q, "scale": s, "zero_point": zi, "bias": b})
+        assert torch.equal(linear_i8(x.cuda(), ws), linear_i8(x.cuda(), w))
+    wu = Int8Weight(q.cuda(), s.cuda(), (z + 100).to(torch.uint8).cuda(), b.cuda())
+    check(linear_i8(x.cuda(), wu), x, q, s, (z + 100).float(), b)
+    for wrong in (torch.ones(50, dtype=torch.bool), torch.ones(50, dtype=torch.complex64)):
+        with pytest.raises(ValueError, match="zero_point"):
+            Int8Weight(q.cuda(), s.cuda(), wrong.cuda())
