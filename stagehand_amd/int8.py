@@ -92,6 +92,7 @@ class Int8Weight:
             raise ValueError(f"qweight must be a 2-D int8 tensor, got {qweight.dim()}-D {qweight.dtype}")
         check_device(qweight, None, "qweight")
         rows, width = qweight.shape
+        _count(rows, "qweight's rows")
         cols = width if in_features is None else int(in_features)
         if not 1 <= cols <= min(width, MAX_COLS):
             raise ValueError(f"in_features {cols} is not in 1 .. {min(width, MAX_COLS)}")
@@ -144,6 +145,13 @@ class Int8Weight:
         return (w * self.scale[:, None]).to(dtype)
 
 
+def _count(n: int, what: str) -> int:
+    """``n`` as the C calls take it, in 32 bits (ctypes would pass on its lower half)."""
+    if n > 0xFFFFFFFF:
+        raise ValueError(f"{what} must be at most {0xFFFFFFFF}, got {n}")
+    return n
+
+
 def _round_up(n: int, m: int) -> int:
     return -(-n // m) * m
 
@@ -182,7 +190,7 @@ def _token_rows(x: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
         x = x.reshape(x.numel() // x.shape[-1] if x.shape[-1] else 0, x.shape[-1])
     if x.shape[1] > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    return x, x.shape[0], x.stride(0)
+    return x, _count(x.shape[0], f"{what}'s tokens"), x.stride(0)
 
 
 def _check_input(x: torch.Tensor, who: str) -> int:
@@ -252,7 +260,7 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
     q, scale, sums, cols, shape = tokens
     if cols != weight.in_features:
         raise ValueError(f"the tokens have {cols} values, the weight takes {weight.in_features}")
-    n = q.shape[0] if q.dim() == 2 else -1
+    n = _count(q.shape[0], "the tokens of tokens.q") if q.dim() == 2 else -1
     width = _round_up(cols, TOKEN_ALIGN)
     if q.dtype != torch.int8 or n < 0 or q.shape[1] < width or (q.numel() and q.stride(1) != 1):
         raise ValueError(f"tokens.q must be int8 rows of {cols} values and zeros up to {width}, got {q.dtype} {tuple(q.shape)}")

@@ -1,5 +1,5 @@
 """Int8 linear layers at the ends of their ranges: token scales from 2^-127 to the type's largest, integer zero
-points. Tolerances as in test_int8_gpu."""
+points, counts past 32 bits. Tolerances as in test_int8_gpu."""
 from __future__ import annotations
 
 import pytest
@@ -64,3 +64,16 @@ def test_integer_zero_points():
     for wrong in (torch.ones(50, dtype=torch.bool), torch.ones(50, dtype=torch.complex64)):
         with pytest.raises(ValueError, match="zero_point"):
             Int8Weight(q.cuda(), s.cuda(), wrong.cuda())
+
+
+def test_counts_past_32_bits_are_refused():
+    """2^32 + 3 tokens (one value seen that often) are not taken for three."""
+    many = 2 ** 32 + 3
+    w = Int8Weight(torch.ones(1, 8, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"))
+    x = torch.ones(1, 8, device="cuda", dtype=torch.bfloat16).expand(many, 8)
+    with pytest.raises(ValueError, match="tokens"):
+        linear_i8(x, w)
+    with pytest.raises(ValueError, match="tokens"):
+        quantize_tokens(x)
+    with pytest.raises(ValueError, match="rows"):
+        Int8Weight(torch.ones(1, 8, dtype=torch.int8, device="cuda").expand(many, 8), torch.ones(1, device="cuda").expand(many))
