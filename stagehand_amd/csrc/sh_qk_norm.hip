@@ -174,7 +174,7 @@ struct Pairs {
     load<(V >= 4 ? 16 : 4 * V)>(shared).values(v0, v1);
   }
 
-  // Cosines and sines of the token at (b, s); NaN where its position has no row.
+  // Cosines and sines of the token at (b, s). Where its position has no row, NaN, also for the values past rot.
   __device__ __forceinline__ void load_angles(const sh_qk_norm_rope_args& a, uint64_t b, uint64_t s, float (&c)[kSlots],
                                               float (&n)[kSlots]) const {
     int64_t row = 0;
@@ -190,8 +190,8 @@ struct Pairs {
       float x[V], y[V];
 #pragma unroll
       for (uint32_t i = 0; i < V; ++i) {
-        x[i] = rotated(j) ? __builtin_nanf("") : 1.0f;
-        y[i] = rotated(j) ? __builtin_nanf("") : 0.0f;
+        x[i] = known ? 1.0f : __builtin_nanf("");
+        y[i] = known ? 0.0f : __builtin_nanf("");
       }
       if (rotated(j) && known) {
         const uint64_t at = (uint64_t)row * a.table_ld + first(j);
