@@ -46,10 +46,14 @@ class _Weight(ctypes.Structure):
                 ("scale", ctypes.c_void_p), ("zero_point", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
 
 
-def on_stream(stream: torch.cuda.Stream | int):
-    """Context in which ``stream`` (a torch stream or a raw handle) is torch's current stream."""
+def on_stream(stream: torch.cuda.Stream | int, t: torch.Tensor):
+    """Context in which ``stream`` (a torch stream, or a raw handle on the device of ``t``) is torch's current
+    stream, for a call that works on ``t``."""
+    check_device(t, None, "a tensor for the stream")
     if isinstance(stream, int):  # ExternalStream(0) would be a new stream
-        stream = torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+        stream = torch.cuda.ExternalStream(stream, t.device) if stream else torch.cuda.default_stream(t.device)
+    elif stream.device != t.device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {t.device}")
     return torch.cuda.stream(stream)
 
 
@@ -230,7 +234,7 @@ def quantize_tokens(x: torch.Tensor, stream: torch.cuda.Stream | int | None = No
     A token with ``a < 2**-120`` counts as zero (q and scale 0). A token with an infinity or a NaN gets
     q = 0 and scale NaN, so every product of it is NaN."""
     if stream is not None:
-        with on_stream(stream):
+        with on_stream(stream, x):
             return quantize_tokens(x)
     code = _check_input(x, "quantize_tokens")
     check_device(x, None, "x")
@@ -255,7 +259,7 @@ def matmul_i8(tokens: Int8Tokens, weight: Int8Weight, out: torch.Tensor | None =
     ``tokens.q`` may be rows of a larger tensor (every second token, the last one of each sequence, some of
     its columns): rows on multiples of 128 bytes, up to 1 MiB apart, are read in place, others are copied."""
     if stream is not None:
-        with on_stream(stream):
+        with on_stream(stream, weight.qweight):
             return matmul_i8(tokens, weight, out, out_dtype)
     q, scale, sums, cols, shape = tokens
     if cols != weight.in_features:
@@ -294,7 +298,7 @@ def linear_i8(x: torch.Tensor, weight: Int8Weight, out: torch.Tensor | None = No
     """``x · weightᵀ + bias`` in the type of ``x``, with the tokens of ``x`` quantised as
     :func:`quantize_tokens` does: the same values as the two calls, in fewer launches."""
     if stream is not None:
-        with on_stream(stream):
+        with on_stream(stream, weight.qweight):
             return linear_i8(x, weight, out)
     code = _check_input(x, "linear_i8")
     index = weight.device.index

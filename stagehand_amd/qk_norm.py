@@ -170,7 +170,7 @@ def qk_norm_rope(
     other memory of the inputs'). A backward pass that needs the old values of ``out`` raises.
     Gradients flow to ``q``, ``k`` and the weights, not to the tables, and not through ``out``."""
     if stream is not None:
-        with on_stream(stream):
+        with on_stream(stream, q):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=positions, start=start,
                                 interleaved=interleaved, eps=eps, out=out)
     device, shape, dtype = q.get_device(), q.shape, q.dtype
