@@ -293,13 +293,12 @@ __device__ __forceinline__ i32x4_t rows_resource(const void* base, uint64_t ld, 
   return r;
 }
 
-// Brings 16 bytes per lane from the resource into LDS, at lds + 16 * lane. Written as assembly: the compiler
+// Brings 16 bytes per lane from the resource into LDS, at lds (in M0) + 16 * lane. Written as assembly: the compiler
 // would wait for the load before the next LDS read, whatever stage that reads. It has no output register;
-// whoever reads the stage waits for it (vmcnt) and for the barrier after that. M0 has no other use here. The
-// whole offset is in the register that the resource's range check covers.
+// whoever reads the stage waits for it (vmcnt) and for the barrier after that. The whole offset is in the register
+// that the resource's range check covers.
 __device__ __forceinline__ void load_to_lds(i32x4_t r, uint32_t lds, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset),
-               "s"(r));
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(lds), "v"(offset), "s"(r));
 }
 
 // Stores N consecutive values, or the first `count` of them. Whole runs are stored as vectors whatever their
