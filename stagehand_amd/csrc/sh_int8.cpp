@@ -13,9 +13,9 @@
 
 namespace {
 
-bool known_dtype(uint32_t d) { return d == SH_DTYPE_BF16 || d == SH_DTYPE_F16 || d == SH_DTYPE_F32; }
-uint32_t dtype_bytes(uint32_t d) { return d == SH_DTYPE_F32 ? 4 : 2; }
-bool misaligned(const void* p, uint32_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+using sh::dtype_bytes;
+using sh::known_dtype;
+using sh::misaligned;
 
 uint64_t token_ld(uint32_t cols) {
   return ((uint64_t)cols + SH_I8_TOKEN_ALIGN - 1) / SH_I8_TOKEN_ALIGN * SH_I8_TOKEN_ALIGN;
@@ -82,9 +82,11 @@ int launch_quantize(const sh::QuantizeArgs& a, hipStream_t stream, const char* w
 }
 
 // The tile of the least estimated time: rounds of tiles over the 256 compute units, times what 128 columns of
-// one round take (MI355X, measured over 64 to 1500 tiles of 3072 and 4096 columns). Larger tiles read LDS and the
-// caches less for each product (8192^3: 256 x 256 415 us, 128 x 256 475, 128 x 128 580, 64 x 64 880), smaller
-// ones leave fewer compute units idle. Around the switches, times in us:
+// one round take (MI355X, measured over 64 to 1500 tiles of 3072 and 4096 columns). The number of columns has no
+// part in it: what a tile's start and its stores take is not in the cost, and products of a few hundred columns,
+// where that counts, were not measured tile by tile (9953 x 949 x 590 takes 20 us, its bytes and operations 5).
+// Larger tiles read LDS and the caches less for each product (8192^3: 256 x 256 415 us, 128 x 256 475, 128 x 128
+// 580, 64 x 64 880), smaller ones leave fewer compute units idle. Around the switches, times in us:
 //   64 x 4096 x 4096     32x32 8.6   64x64 11          1024 x 4096 x 4096   128x128 20   128x256 25   256x256 42
 //   128 x 9216 x 3072    64x64 13.4  32x32 21          2048 x 4096 x 4096   128x256 33   128x128 37   256x256 44
 //   256 x 9216 x 3072    128x128 16  64x64 18          1024 x 12288 x 3072  256x256 41   128x256 45

@@ -20,8 +20,6 @@
 
 namespace {
 
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-
 // A token's factor 127 / a and scale a / 127 from the bits of a = max |x|. The bits order as the
 // values do, with infinities and NaNs last, so their maximum finds a NaN too.
 __device__ __forceinline__ void token_scale(uint32_t amax_bits, float* inv, float* scale) {
@@ -603,8 +601,9 @@ __device__ __forceinline__ void matmul_skinny(const sh::MatmulI8Args& a, uint8_t
 
 namespace {
 
-// As matmul_skinny for up to 16 tokens, which every workgroup quantises for itself into LDS: one launch, and the
-// weight is on its way meanwhile. A wavefront's piece of a token is 512 values; all of them, PIECES / W a
+// As matmul_skinny for up to 16 tokens, which every workgroup quantises for itself into LDS: one launch. The weight's
+// first loads start when the tokens have arrived and their maxima are known, and are on their way while the tokens are
+// rounded: the memory's latency comes twice, one after the other, before the first product. A wavefront's piece of a token is 512 values; all of them, PIECES / W a
 // wavefront, stay in registers between maximum and rounding. In `a`, tq is the tokens as they are, t_ld their
 // distance in elements; t_scale and t_sums are not used.
 template <typename T, uint32_t FN, uint32_t W, uint32_t D, uint32_t PIECES>

@@ -30,6 +30,11 @@ void clear_error();
                         hipGetErrorString(sh_e_), #call);                         \
   } while (0)
 
+// Of the operators' arguments: enum sh_dtype, and an address that is not a multiple of n (a power of two).
+inline bool known_dtype(uint32_t d) { return d == SH_DTYPE_BF16 || d == SH_DTYPE_F16 || d == SH_DTYPE_F32; }
+inline uint32_t dtype_bytes(uint32_t d) { return d == SH_DTYPE_F32 ? 4 : 2; }
+inline bool misaligned(const void* p, uint32_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+
 // Live native objects by kind, for sh_shutdown's report. Each object struct holds a
 // Live<kind> member, so construction and destruction keep the count.
 enum LiveKind : int { kLivePool = 0, kLiveLoader, kLiveSaveback, kLiveTurbo, kLiveVmm, kLiveFile, kLiveKinds };

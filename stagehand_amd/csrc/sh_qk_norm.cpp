@@ -13,9 +13,9 @@
 
 namespace {
 
-bool known_dtype(uint32_t d) { return d == SH_DTYPE_BF16 || d == SH_DTYPE_F16 || d == SH_DTYPE_F32; }
-uint32_t dtype_bytes(uint32_t d) { return d == SH_DTYPE_F32 ? 4 : 2; }
-bool misaligned(const void* p, uint32_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+using sh::dtype_bytes;
+using sh::known_dtype;
+using sh::misaligned;
 
 int check_heads(const sh_heads& v, const char* name, uint32_t heads, uint32_t dtype, const char* who) {
   if (heads == 0) return SH_OK;

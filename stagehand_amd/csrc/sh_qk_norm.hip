@@ -205,8 +205,6 @@ struct Pairs {
   }
 };
 
-// The groups of a wavefront side by side: `abreast` of them share a token and take every abreast-th of its
-// heads, segment by segment; a wavefront's unit is one segment of 64 / lanes / abreast tokens.
 // What a workgroup has to do: the first q_grid take the queries, the others the keys. The groups of a
 // wavefront lie side by side: `abreast` of them share a token and take every abreast-th of its heads, segment by
 // segment; a wavefront's unit is one segment of 64 / lanes / abreast tokens.

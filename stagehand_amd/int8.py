@@ -83,11 +83,11 @@ class Int8Weight:
 
     ``qweight`` is int8 ``(out_features, padded_in)``; ``in_features`` of its columns count (default:
     all). ``scale`` and the optional ``zero_point`` and ``bias`` hold ``out_features`` values; they are
-    constants here (no gradient), kept in fp32; zero points may be integers. ``qweight`` is used where it lies if its rows start on 128-byte boundaries and its
-    memory holds all of the last row; changes of it are then seen by later calls. Otherwise it is copied
-    once into such rows. With ``realign=False`` rows that start on 16-byte boundaries are used where
-    they lie too: no copy, and 7% slower products of many tokens (4608 x 21504 x 3072: 288 us against
-    268), for a weight that is multiplied a few times only.
+    constants here (no gradient), kept in fp32; zero points may be integers. ``qweight`` is used where it
+    lies if its rows start on 128-byte boundaries and its memory holds all of the last row; changes of it
+    are then seen by later calls. Otherwise it is copied once into such rows. With ``realign=False`` rows
+    that start on 16-byte boundaries are used where they lie too: no copy, and 7% slower products of many
+    tokens (4608 x 21504 x 3072: 288 us against 268), for a weight that is multiplied a few times only.
     """
 
     def __init__(self, qweight: torch.Tensor, scale: torch.Tensor, zero_point: torch.Tensor | None = None,
