@@ -507,7 +507,7 @@ def _intersect(x: list[tuple[float, float]], y: list[tuple[float, float]]) -> fl
     return tot
 
 
-def load_gap_causes(trace: dict, top: int = 6) -> list[dict]:
+def load_gap_causes(trace: dict, top: int = 3) -> list[dict]:
     """For the longest gaps between consecutive block loads of a traced step (one copy's end to the
     next copy's start): when the next load was submitted by the host relative to the gap, and the
     host waits (``AsyncTransferEngine.host_wait``) that overlapped the gap before that submit."""
@@ -1784,8 +1784,13 @@ def main() -> int:
         result["train"] = train_leg(args)
 
     log(summary_line(result))
-    print(json.dumps(result), flush=True)
+    print(result_line(result), flush=True)
     return 0
+
+
+def result_line(r: dict) -> str:
+    """The result as one line of JSON, kept under 20,000 characters: what captures the output keeps its end."""
+    return json.dumps(r, separators=(",", ": "))
 
 
 def summary_line(r: dict) -> str:
