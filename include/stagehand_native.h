@@ -822,6 +822,92 @@ int sh_qk_norm_rope_workspace(const sh_qk_norm_rope_args* args, uint64_t* bytes)
 int sh_qk_norm_rope_backward(const sh_qk_norm_rope_args* args, void* workspace, uint64_t workspace_bytes,
                              void* stream);
 
+/* ── Activations in 8 bits, layer norms and weight gradients, for training ──
+ *
+ * An activation kept in 8 bits: rows of `cols` values in groups of
+ * SH_ACT8_GROUP, the last one of a row filled up with zeros. A group shares a
+ * power of two 2^k, the smallest with max |x| <= 127 * 2^k (k = -126 at least);
+ * its values are q * 2^k with q = rint(x * 2^-k), ties to even. Where 64 * 2^k
+ * is no number of the activation's type any more (fp16: k = 10, others: k =
+ * 122), q ends with 63. exponent holds k + 127 for each group, or 255 for a
+ * group with an infinity or a NaN, which is read back as NaNs. What is kept
+ * of a bf16, fp16 or fp32 activation is a number of that type: only q is
+ * rounded. q is 16-byte aligned, tokens * groups * SH_ACT8_GROUP bytes with groups
+ * = cols / SH_ACT8_GROUP, rounded up; exponent tokens * groups bytes. */
+#define SH_ACT8_GROUP 32u
+#define SH_ACT8_MAX_COLS 0x00FFFFFFu
+typedef struct sh_act8 {
+  void* q;
+  void* exponent;
+  uint32_t tokens;
+  uint32_t cols; /* 1 .. SH_ACT8_MAX_COLS */
+} sh_act8;
+/* Rows of x and out are x_ld and out_ld elements apart. */
+int sh_act8_quantize(const void* x, uint32_t dtype, uint64_t x_ld, const sh_act8* kept, void* stream);
+int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype, uint64_t out_ld, void* stream);
+
+/* The gradients of a Linear's weight and bias from its kept input:
+ *   dweight[o][i] = sum_t dy[t][o] kept[t][i],  dbias[o] = sum_t dy[t][o]
+ * over the kept tokens, summed in fp32 in a fixed order and rounded once to
+ * out_dtype. dy is tokens x out_features in `dtype` (rows dy_ld elements apart), the type that
+ * the kept activation had: values kept of bf16 or fp32 need not be fp16 numbers. fp32 gradients are multiplied with
+ * all their bits. dbias may be NULL. The workspace (16-byte aligned device
+ * memory, in use until the call's kernels have run) holds at least
+ * sh_weight_grad_act8_workspace bytes, for `bias` as dbias is given. */
+int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t out_features, uint32_t bias, uint64_t* bytes);
+int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_ld, uint32_t out_features, const sh_act8* kept,
+                        void* dweight, uint32_t out_dtype, uint64_t dw_ld, void* dbias, void* workspace,
+                        uint64_t workspace_bytes, void* stream);
+
+/* Rows of a (batch, seq, cols) tensor with strides in elements; the values of
+ * a row are contiguous. */
+typedef struct sh_rows {
+  void* data;
+  uint64_t batch_stride;
+  uint64_t seq_stride;
+} sh_rows;
+
+/* Layer norm over the cols values of a token:
+ *   n = (x - mean(x)) * r,  r = (var(x) + eps)^(-1/2)
+ *   y = n * weight + bias,  or n * (1 + weight) + bias when `modulate`
+ * weight and bias are NULL (ones, or zeros when `modulate`; zeros), cols values of weight_dtype for all tokens,
+ * or, `per_batch`, such a row for every sequence, *_batch_stride elements
+ * apart. Statistics, products and sums are fp32, outputs are rounded once.
+ *
+ * sh_layer_norm reads x and writes y. With `stats` it writes mean and r of
+ * each token there (two floats, dense); with `q` and `exponent` it keeps x in
+ * 8 bits as sh_act8_quantize does (tokens = batch * seq).
+ * sh_layer_norm_backward reads stats, dy and x, or in the place of x q and exponent, if given, and
+ * writes, of dx, dweight and dbias, those that are not NULL:
+ *   dx = r (g - mean(g) - n mean(g n)),  g = dy * weight (or dy * (1 + weight))
+ *   dweight = sum dy * n,  dbias = sum dy
+ * over all tokens, or those of each sequence when `per_batch` (dense rows of
+ * weight_dtype), in a fixed order. Outputs may not overlap inputs, save y = x
+ * and dx = dy with equal strides. */
+typedef struct sh_layer_norm_args {
+  sh_rows x, y;
+  sh_rows dy, dx;
+  const void* weight;
+  const void* bias;
+  void* dweight;
+  void* dbias;
+  float* stats;
+  void* q;
+  void* exponent;
+  uint64_t weight_batch_stride, bias_batch_stride;
+  uint32_t batch, seq;
+  uint32_t cols; /* 1 .. SH_LAYER_NORM_MAX_COLS */
+  uint32_t dtype, weight_dtype;
+  uint32_t per_batch;
+  uint32_t modulate;
+  float eps;
+} sh_layer_norm_args;
+#define SH_LAYER_NORM_MAX_COLS 16384u
+int sh_layer_norm(const sh_layer_norm_args* args, void* stream);
+/* Bytes of workspace that the backward pass needs; 16-byte aligned device memory. */
+int sh_layer_norm_workspace(const sh_layer_norm_args* args, uint64_t* bytes);
+int sh_layer_norm_backward(const sh_layer_norm_args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,164 @@
+// Activations kept in 8 bits, and the weight gradients that read them (no reference counterpart: the reference
+// leaves activations to torch).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "sh_act8_args.h"
+#include "sh_internal.h"
+#include "stagehand_native.h"
+
+namespace {
+
+using sh::dtype_bytes;
+using sh::known_dtype;
+using sh::misaligned;
+
+uint32_t groups_of(uint32_t cols) { return cols / SH_ACT8_GROUP + (cols % SH_ACT8_GROUP != 0); }
+
+int check_kept(const sh_act8* k, const char* who) {
+  if (k == nullptr) return sh::fail(SH_ERR_INVALID, "%s: kept is NULL", who);
+  if (k->cols == 0 || k->cols > SH_ACT8_MAX_COLS)
+    return sh::fail(SH_ERR_INVALID, "%s: cols %u is not in 1 .. %u", who, k->cols, SH_ACT8_MAX_COLS);
+  if ((uint64_t)k->tokens * groups_of(k->cols) * (SH_ACT8_GROUP / 8) > 0xFFFFFFFFull - sh::kAct8Threads * sh::kAct8Chunks)
+    return sh::fail(SH_ERR_INVALID, "%s: %u tokens of %u values are too many for one launch", who, k->tokens, k->cols);
+  if (k->tokens > 0 && (k->q == nullptr || k->exponent == nullptr))
+    return sh::fail(SH_ERR_INVALID, "%s: q or exponent is NULL", who);
+  if (misaligned(k->q, 16)) return sh::fail(SH_ERR_INVALID, "%s: q is not 16-byte aligned", who);
+  return SH_OK;
+}
+
+int check_values(const void* x, const char* name, uint32_t dtype, uint32_t tokens, const char* who) {
+  if (!known_dtype(dtype)) return sh::fail(SH_ERR_INVALID, "%s: unknown dtype %u", who, dtype);
+  if (tokens == 0) return SH_OK;
+  if (x == nullptr) return sh::fail(SH_ERR_INVALID, "%s: %s is NULL", who, name);
+  if (misaligned(x, dtype_bytes(dtype))) return sh::fail(SH_ERR_INVALID, "%s: %s is not aligned to its type", who, name);
+  return SH_OK;
+}
+
+int check_out_rows(uint64_t ld, uint32_t rows, uint32_t cols, const char* name, const char* who) {
+  if (rows > 1 && ld < cols)
+    return sh::fail(SH_ERR_INVALID, "%s: %s %llu is less than the %u values of a row", who, name, (unsigned long long)ld, cols);
+  return SH_OK;
+}
+
+int launch_act8(const sh_act8* k, void* x, uint64_t x_ld, uint32_t dtype, bool back, hipStream_t stream, const char* who) {
+  static_assert(sh::kKernAct8QuantizeF16 == sh::kKernAct8QuantizeBf16 + 2 && sh::kKernAct8QuantizeF32 == sh::kKernAct8QuantizeBf16 + 4,
+                "two kernels for each type, in the order of enum sh_dtype");
+  if (k->tokens == 0) return SH_OK;
+  sh::Act8Args a{};
+  a.x = x;
+  a.q = k->q;
+  a.exponent = k->exponent;
+  a.x_ld = x_ld;
+  a.row_chunks = groups_of(k->cols) * (SH_ACT8_GROUP / 8);
+  a.chunks = k->tokens * a.row_chunks;
+  a.magic = sh::udiv_magic(a.row_chunks);
+  a.tokens = k->tokens;
+  a.cols = k->cols;
+  constexpr uint32_t per = sh::kAct8Threads * sh::kAct8Chunks;
+  void* args[] = {(void*)&a};
+  return sh::launch_kernel((sh::KernelId)(sh::kKernAct8QuantizeBf16 + (dtype - SH_DTYPE_BF16) * 2 + back), (a.chunks + per - 1) / per,
+                           sh::kAct8Threads, stream, args, who);
+}
+
+struct GradPlan {
+  int tile;
+  uint32_t tiles, splits, split_tokens;
+  uint64_t bytes;
+};
+
+constexpr uint32_t kComputeUnits = 256;
+
+// The tile, and into how many parts the tokens are split where the tiles alone leave compute units idle.
+GradPlan plan_of(const sh_act8* k, uint32_t out, bool bias) {
+  GradPlan p{};
+  auto tiles = [&](int i) {
+    return (uint64_t)((out + sh::kGradTiles[i].out - 1) / sh::kGradTiles[i].out) * ((k->cols + sh::kGradTiles[i].in - 1) / sh::kGradTiles[i].in);
+  };
+  p.tile = out <= 64 ? 0 : tiles(2) >= kComputeUnits / 2 ? 2 : 1;
+  p.tiles = (uint32_t)tiles(p.tile);
+  const uint32_t steps = std::max(1u, (k->tokens + sh::kGradStep - 1) / sh::kGradStep);
+  const uint32_t want = p.tiles >= kComputeUnits ? 1 : 2 * kComputeUnits / std::max(1u, p.tiles);
+  const uint32_t split_steps = std::max(4u, (steps + want - 1) / want);
+  p.splits = (steps + split_steps - 1) / split_steps;
+  p.split_tokens = split_steps * sh::kGradStep;
+  p.bytes = p.splits > 1 ? 4ull * p.splits * ((uint64_t)out * k->cols + (bias ? out : 0)) : 0;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int sh_act8_quantize(const void* x, uint32_t dtype, uint64_t x_ld, const sh_act8* kept, void* stream) {
+  const char* who = "sh_act8_quantize";
+  sh::clear_error();
+  if (int st = check_kept(kept, who)) return st;
+  if (int st = check_values(x, "x", dtype, kept->tokens, who)) return st;
+  return launch_act8(kept, const_cast<void*>(x), x_ld, dtype, false, (hipStream_t)stream, who);
+}
+
+extern "C" int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype, uint64_t out_ld, void* stream) {
+  const char* who = "sh_act8_dequantize";
+  sh::clear_error();
+  if (int st = check_kept(kept, who)) return st;
+  if (int st = check_values(out, "out", dtype, kept->tokens, who)) return st;
+  if (int st = check_out_rows(out_ld, kept->tokens, kept->cols, "out_ld", who)) return st;
+  return launch_act8(kept, out, out_ld, dtype, true, (hipStream_t)stream, who);
+}
+
+extern "C" int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t out_features, uint32_t bias, uint64_t* bytes) {
+  const char* who = "sh_weight_grad_act8_workspace";
+  sh::clear_error();
+  if (bytes == nullptr) return sh::fail(SH_ERR_INVALID, "%s: bytes is NULL", who);
+  if (int st = check_kept(kept, who)) return st;
+  *bytes = plan_of(kept, out_features, bias != 0).bytes;
+  return SH_OK;
+}
+
+extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_ld, uint32_t out_features, const sh_act8* kept,
+                                   void* dweight, uint32_t out_dtype, uint64_t dw_ld, void* dbias, void* workspace,
+                                   uint64_t workspace_bytes, void* stream) {
+  const char* who = "sh_weight_grad_act8";
+  sh::clear_error();
+  if (int st = check_kept(kept, who)) return st;
+  if (int st = check_values(dy, "dy", dtype, out_features == 0 ? 0 : kept->tokens, who)) return st;
+  if (int st = check_values(dweight, "dweight", out_dtype, out_features, who)) return st;
+  if (int st = check_out_rows(dw_ld, out_features, kept->cols, "dw_ld", who)) return st;
+  if (misaligned(dbias, dtype_bytes(out_dtype))) return sh::fail(SH_ERR_INVALID, "%s: dbias is not aligned to its type", who);
+  if (out_features == 0) return SH_OK;
+  const GradPlan p = plan_of(kept, out_features, dbias != nullptr);
+  if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr))
+    return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
+                    (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
+  if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
+  const sh::GradTile& tile = sh::kGradTiles[p.tile];
+  if ((uint64_t)p.tiles * p.splits > 0xFFFFFFFFull / tile.threads)
+    return sh::fail(SH_ERR_INVALID, "%s: %u x %u gradients are too many for one launch", who, out_features, kept->cols);
+  sh::WeightGradArgs a{};
+  a.dy = dy;
+  a.q = kept->q;
+  a.exponent = kept->exponent;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  a.partials = p.splits > 1 ? static_cast<float*>(workspace) : nullptr;
+  a.dy_ld = dy_ld;
+  a.dw_ld = dw_ld;
+  a.tokens = kept->tokens;
+  a.out = out_features;
+  a.cols = kept->cols;
+  a.splits = p.splits;
+  a.split_tokens = p.split_tokens;
+  a.dtype = dtype;
+  a.out_dtype = out_dtype;
+  static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount, "one kernel per type and tile");
+  void* args[] = {(void*)&a};
+  if (int st = sh::launch_kernel((sh::KernelId)(sh::kKernWeightGradBf1632x128 + (dtype - SH_DTYPE_BF16) * sh::kGradTileCount + p.tile),
+                                 p.tiles * p.splits, tile.threads, (hipStream_t)stream, args, who))
+    return st;
+  if (p.splits == 1) return SH_OK;
+  const uint64_t values = (uint64_t)out_features * ((kept->cols + 3) / 4) + (dbias != nullptr ? out_features : 0);
+  const uint64_t blocks = (values + sh::kGradJoinThreads - 1) / sh::kGradJoinThreads;
+  return sh::launch_kernel(sh::kKernWeightGradJoin, (uint32_t)blocks, sh::kGradJoinThreads, (hipStream_t)stream, args, who);
+}

@@ -173,6 +173,80 @@ enum KernelId : int {
   kKernQkNormBackwardF321,
   kKernQkNormBackwardF321Interleaved,
   kKernQkNormDweight,
+  // layer norms: per type and shape of sh_layer_norm_args.h: forward, backward, backward from what was kept
+  kKernLayerNormBf161x1,
+  kKernLayerNormBackwardBf161x1,
+  kKernLayerNormBackwardKeptBf161x1,
+  kKernLayerNormBf161x2,
+  kKernLayerNormBackwardBf161x2,
+  kKernLayerNormBackwardKeptBf161x2,
+  kKernLayerNormBf164x1,
+  kKernLayerNormBackwardBf164x1,
+  kKernLayerNormBackwardKeptBf164x1,
+  kKernLayerNormBf164x2,
+  kKernLayerNormBackwardBf164x2,
+  kKernLayerNormBackwardKeptBf164x2,
+  kKernLayerNormBf168x2,
+  kKernLayerNormBackwardBf168x2,
+  kKernLayerNormBackwardKeptBf168x2,
+  kKernLayerNormBf1616x2,
+  kKernLayerNormBackwardBf1616x2,
+  kKernLayerNormBackwardKeptBf1616x2,
+  kKernLayerNormF161x1,
+  kKernLayerNormBackwardF161x1,
+  kKernLayerNormBackwardKeptF161x1,
+  kKernLayerNormF161x2,
+  kKernLayerNormBackwardF161x2,
+  kKernLayerNormBackwardKeptF161x2,
+  kKernLayerNormF164x1,
+  kKernLayerNormBackwardF164x1,
+  kKernLayerNormBackwardKeptF164x1,
+  kKernLayerNormF164x2,
+  kKernLayerNormBackwardF164x2,
+  kKernLayerNormBackwardKeptF164x2,
+  kKernLayerNormF168x2,
+  kKernLayerNormBackwardF168x2,
+  kKernLayerNormBackwardKeptF168x2,
+  kKernLayerNormF1616x2,
+  kKernLayerNormBackwardF1616x2,
+  kKernLayerNormBackwardKeptF1616x2,
+  kKernLayerNormF321x1,
+  kKernLayerNormBackwardF321x1,
+  kKernLayerNormBackwardKeptF321x1,
+  kKernLayerNormF321x2,
+  kKernLayerNormBackwardF321x2,
+  kKernLayerNormBackwardKeptF321x2,
+  kKernLayerNormF324x1,
+  kKernLayerNormBackwardF324x1,
+  kKernLayerNormBackwardKeptF324x1,
+  kKernLayerNormF324x2,
+  kKernLayerNormBackwardF324x2,
+  kKernLayerNormBackwardKeptF324x2,
+  kKernLayerNormF328x2,
+  kKernLayerNormBackwardF328x2,
+  kKernLayerNormBackwardKeptF328x2,
+  kKernLayerNormF3216x2,
+  kKernLayerNormBackwardF3216x2,
+  kKernLayerNormBackwardKeptF3216x2,
+  kKernLayerNormJoin,
+  // activations in 8 bits and back, per type
+  kKernAct8QuantizeBf16,
+  kKernAct8DequantizeBf16,
+  kKernAct8QuantizeF16,
+  kKernAct8DequantizeF16,
+  kKernAct8QuantizeF32,
+  kKernAct8DequantizeF32,
+  // weight gradients: per type and tile of sh_act8_args.h
+  kKernWeightGradBf1632x128,
+  kKernWeightGradBf16128x128,
+  kKernWeightGradBf16256x256,
+  kKernWeightGradF1632x128,
+  kKernWeightGradF16128x128,
+  kKernWeightGradF16256x256,
+  kKernWeightGradF3232x128,
+  kKernWeightGradF32128x128,
+  kKernWeightGradF32256x256,
+  kKernWeightGradJoin,
   kKernelCount
 };
 // Launches kernel `id` of the current device: a 1-D grid of `grid` workgroups of `block`

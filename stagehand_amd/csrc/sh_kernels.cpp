@@ -26,11 +26,14 @@ extern const unsigned char sh_co_unpack[];
 extern const unsigned char sh_co_digest[];
 extern const unsigned char sh_co_int8[];
 extern const unsigned char sh_co_qk_norm[];
+extern const unsigned char sh_co_layer_norm[];
+extern const unsigned char sh_co_act8[];
+extern const unsigned char sh_co_weight_grad[];
 }
 
 namespace {
 
-enum ModuleId : int { kModUnpack = 0, kModDigest, kModInt8, kModQkNorm, kModules };
+enum ModuleId : int { kModUnpack = 0, kModDigest, kModInt8, kModQkNorm, kModLayerNorm, kModAct8, kModWeightGrad, kModules };
 
 struct ModuleSpec {
   const unsigned char* image;
@@ -38,12 +41,15 @@ struct ModuleSpec {
   int set;  // modules of one set load together
 };
 
-constexpr int kSets = 3;
+constexpr int kSets = 6;
 const ModuleSpec kModuleSpecs[kModules] = {
     {sh_co_unpack, "unpack", 0},
     {sh_co_digest, "digest", 0},
     {sh_co_int8, "int8", 1},
     {sh_co_qk_norm, "qk_norm", 2},
+    {sh_co_layer_norm, "layer_norm", 3},
+    {sh_co_act8, "act8", 4},
+    {sh_co_weight_grad, "weight_grad", 5},
 };
 
 struct KernelSpec {
@@ -142,6 +148,77 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModQkNorm, "sh_qk_norm_backward_f32_1_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f32_1_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_1x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_1x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_4x1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_4x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_8x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_join_kernel"},
+    {kModAct8, "sh_act8_quantize_bf16_kernel"},
+    {kModAct8, "sh_act8_dequantize_bf16_kernel"},
+    {kModAct8, "sh_act8_quantize_f16_kernel"},
+    {kModAct8, "sh_act8_dequantize_f16_kernel"},
+    {kModAct8, "sh_act8_quantize_f32_kernel"},
+    {kModAct8, "sh_act8_dequantize_f32_kernel"},
+    {kModWeightGrad, "sh_weight_grad_bf16_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_bf16_128x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_bf16_256x256_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f16_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f16_128x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f16_256x256_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f32_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f32_128x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f32_256x256_kernel"},
+    {kModWeightGrad, "sh_weight_grad_join_kernel"},
 };
 
 struct DeviceKernels {

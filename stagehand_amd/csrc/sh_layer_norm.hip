@@ -1,0 +1,339 @@
+// Layer norm, forward and backward, for gfx950 (device code only; the checks and the launches are in
+// sh_layer_norm.cpp).
+//
+// With n = (x - mean) r, r = (var + eps)^(-1/2), and a gain w (1 + w when modulated): y = n w + b. For a gradient dy,
+// with g = dy w: dx = r (g - mean(g) - n mean(g n)), dw = sum of dy n and db = sum of dy over the tokens that share w, b.
+//
+// Bound by HBM: each value is read once and written once (backward: x and dy read, dx written). A team of wavefronts
+// holds a row in registers, so mean and variance take two passes over registers and one over memory: the variance is a
+// sum of squares of differences, not a difference of sums. The forward leaves mean and r of each token for the backward
+// pass. The gradients of w and b are summed in registers over a workgroup's tokens and joined by a second kernel,
+// always in the same order.
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sh_act8_device.h"
+#include "sh_layer_norm_args.h"
+
+namespace {
+
+template <int CTRL>
+__device__ __forceinline__ float add_moved(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+// The sum over a wavefront, in all of it: halves of 2, 4, 8 and 16 by data-parallel moves, 32 and 64 by shuffles.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = add_moved<0xB1>(v);   // quad_perm 1,0,3,2
+  v = add_moved<0x4E>(v);   // quad_perm 2,3,0,1
+  v = add_moved<0x141>(v);  // row_half_mirror
+  v = add_moved<0x140>(v);  // row_mirror
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  return v;
+}
+
+// Sums over a team of W wavefronts. Two sets of slots in turn: a set is written again only after the barrier of the
+// other, which everyone reaches after reading it.
+template <uint32_t W, uint32_t N>
+struct TeamSum {
+  float (*slots)[N][W];  // [2][N][W] of LDS
+  uint32_t turn = 0;
+
+  __device__ __forceinline__ void operator()(float (&v)[N]) {
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if constexpr (W > 1) {
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) slots[turn][i][threadIdx.x / 64] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (uint32_t i = 0; i < N; ++i) {
+        v[i] = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) v[i] += slots[turn][i][w];
+      }
+      turn ^= 1;
+    }
+  }
+};
+
+// 8 values of a weight or bias at p, 0 behind `count`.
+__device__ __forceinline__ void load_params(const void* p, uint32_t dtype, uint64_t at, uint32_t count, float (&v)[8]) {
+  auto values = [&](auto zero) {
+    using T = decltype(zero);
+    const auto raw = Values8<T>::load(static_cast<const T*>(p) + at, count);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = (float)raw[i];
+  };
+  if (dtype == SH_DTYPE_BF16) values(__bf16{});
+  else if (dtype == SH_DTYPE_F16) values(_Float16{});
+  else values(float{});
+}
+
+__device__ __forceinline__ void store_params(void* p, uint32_t dtype, uint64_t at, uint32_t count, const float (&v)[8]) {
+  if (dtype == SH_DTYPE_BF16) Values8<__bf16>::store(static_cast<__bf16*>(p) + at, v, count);
+  else if (dtype == SH_DTYPE_F16) Values8<_Float16>::store(static_cast<_Float16*>(p) + at, v, count);
+  else Values8<float>::store(static_cast<float*>(p) + at, v, count);
+}
+
+// A work-item's share of the rows: chunks of 8 values, and the team's tokens of a group.
+template <uint32_t W, uint32_t C>
+struct Mine {
+  static constexpr uint32_t kTeams = sh::norm_teams(W);
+  uint32_t item;               // in the team
+  uint32_t group, first, step;  // tokens first, first + step .. of the group
+  uint32_t cols;
+
+  __device__ __forceinline__ Mine(const sh::LayerNormKernelArgs& ka) : cols(ka.a.cols) {
+    const uint32_t team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * W));
+    item = threadIdx.x - team * 64 * W;
+    group = blockIdx.x / ka.per_group;
+    first = (blockIdx.x - group * ka.per_group) * kTeams + team;
+    step = ka.per_group * kTeams;
+  }
+  __device__ __forceinline__ uint32_t chunk(uint32_t j) const { return j * W * 64 + item; }
+  __device__ __forceinline__ uint32_t col(uint32_t j) const { return chunk(j) * 8; }
+  __device__ __forceinline__ uint32_t count(uint32_t j) const { return col(j) < cols ? min(cols - col(j), 8u) : 0; }
+};
+
+struct Token {
+  uint64_t b, s, row;
+
+  __device__ __forceinline__ Token(const sh_layer_norm_args& a, uint32_t group, uint32_t t) {
+    if (a.per_batch) b = group, s = t;
+    else b = t / a.seq, s = t - (uint32_t)b * a.seq;
+    row = b * a.seq + s;
+  }
+  __device__ __forceinline__ uint64_t at(const sh_rows& r) const { return b * r.batch_stride + s * r.seq_stride; }
+};
+
+template <typename T, uint32_t W, uint32_t C>
+__device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
+  const sh_layer_norm_args& a = ka.a;
+  const Mine<W, C> m(ka);
+  __shared__ float slots[2][1][W];
+  TeamSum<W, 1> team_sum{slots};
+  const float rcols = 1.0f / (float)a.cols;
+  const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
+  float w[C][8], b[C][8];
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f, b[j][i] = 0.0f;
+    if (a.weight != nullptr) load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
+    if (a.bias != nullptr) load_params(a.bias, a.weight_dtype, m.group * a.bias_batch_stride + m.col(j), m.count(j), b[j]);
+    if (a.modulate) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) w[j][i] += 1.0f;
+    }
+  }
+  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+    const Token token(a, m.group, t);
+    const T* x = static_cast<const T*>(a.x.data) + token.at(a.x);
+    T* y = static_cast<T*>(a.y.data) + token.at(a.y);
+    float v[C][8], sum[1] = {0.0f};
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+      const auto raw = Values8<T>::load(x + m.col(j), m.count(j));
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) v[j][i] = (float)raw[i];
+    }
+    if (a.q != nullptr) {
+#pragma unroll
+      for (uint32_t j = 0; j < C; ++j) {
+        if (m.chunk(j) >= row_chunks) continue;  // whole groups of four work-items
+        const uint32_t e = group_exponent(v[j]);
+        const uint64_t at = token.row * row_chunks + m.chunk(j);
+        static_cast<uint2*>(a.q)[at] = quantize8<T>(v[j], e);
+        if (m.item % 4 == 0) static_cast<uint8_t*>(a.exponent)[at / 4] = (uint8_t)e;
+      }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) sum[0] += v[j][i];
+    team_sum(sum);
+    const float mean = sum[0] * rcols;
+    sum[0] = 0.0f;
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        v[j][i] = i < m.count(j) ? v[j][i] - mean : 0.0f;
+        sum[0] = __builtin_fmaf(v[j][i], v[j][i], sum[0]);
+      }
+    }
+    team_sum(sum);
+    const float r = 1.0f / __builtin_sqrtf(sum[0] * rcols + a.eps);
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+      float out[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) out[i] = __builtin_fmaf(v[j][i] * r, w[j][i], b[j][i]);
+      Values8<T>::store(y + m.col(j), out, m.count(j));
+    }
+    if (a.stats != nullptr && m.item == 0) {
+      a.stats[2 * token.row] = mean;
+      a.stats[2 * token.row + 1] = r;
+    }
+  }
+}
+
+template <typename T, uint32_t W, uint32_t C, bool KEPT>
+__device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
+  const sh_layer_norm_args& a = ka.a;
+  const Mine<W, C> m(ka);
+  constexpr uint32_t kTeams = Mine<W, C>::kTeams;
+  __shared__ float slots[2][2][W];
+  TeamSum<W, 2> team_sum{slots};
+  const float rcols = 1.0f / (float)a.cols;
+  const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
+  float w[C][8], dw[C][8] = {}, db[C][8] = {};
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f;
+    if (a.weight != nullptr) load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
+    if (a.modulate) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) w[j][i] += 1.0f;
+    }
+  }
+  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+    const Token token(a, m.group, t);
+    const T* dy = static_cast<const T*>(a.dy.data) + token.at(a.dy);
+    const float mean = a.stats[2 * token.row], r = a.stats[2 * token.row + 1];
+    float n[C][8], g[C][8], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+      if constexpr (KEPT) {
+        if (m.chunk(j) < row_chunks) {
+          const uint64_t at = token.row * row_chunks + m.chunk(j);
+          dequantize8(static_cast<const uint2*>(a.q)[at], group_scale(static_cast<const uint8_t*>(a.exponent)[at / 4]), n[j]);
+        } else {
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) n[j][i] = 0.0f;
+        }
+      } else {
+        const auto raw = Values8<T>::load(static_cast<const T*>(a.x.data) + token.at(a.x) + m.col(j), m.count(j));
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) n[j][i] = (float)raw[i];
+      }
+      const auto raw = Values8<T>::load(dy + m.col(j), m.count(j));  // zeros past the row add nothing below
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) g[j][i] = (float)raw[i];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        n[j][i] = (n[j][i] - mean) * r;
+        dw[j][i] = __builtin_fmaf(g[j][i], n[j][i], dw[j][i]);
+        db[j][i] += g[j][i];
+        g[j][i] *= w[j][i];
+        sum[0] += g[j][i];
+        sum[1] = __builtin_fmaf(g[j][i], n[j][i], sum[1]);
+      }
+    }
+    if (a.dx.data == nullptr) continue;
+    team_sum(sum);
+    const float mean_g = sum[0] * rcols, mean_gn = sum[1] * rcols;
+    T* dx = static_cast<T*>(a.dx.data) + token.at(a.dx);
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+      float out[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) out[i] = r * (g[j][i] - mean_g - n[j][i] * mean_gn);
+      Values8<T>::store(dx + m.col(j), out, m.count(j));
+    }
+  }
+  if (a.dweight == nullptr && a.dbias == nullptr) return;
+  if constexpr (kTeams > 1) {  // the teams' sums, in their order
+    __shared__ alignas(16) float part[kTeams][2][C][8][64];
+    const uint32_t team = threadIdx.x / 64;
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) part[team][0][j][i][m.item] = dw[j][i], part[team][1][j][i][m.item] = db[j][i];
+    __syncthreads();
+    if (team != 0) return;
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+#pragma unroll
+        for (uint32_t k = 1; k < kTeams; ++k) dw[j][i] += part[k][0][j][i][m.item], db[j][i] += part[k][1][j][i][m.item];
+      }
+    }
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) {
+    if (ka.partials == nullptr) {  // the workgroup has all of the group's tokens
+      const uint64_t at = (uint64_t)m.group * a.cols + m.col(j);
+      if (a.dweight != nullptr) store_params(a.dweight, a.weight_dtype, at, m.count(j), dw[j]);
+      if (a.dbias != nullptr) store_params(a.dbias, a.weight_dtype, at, m.count(j), db[j]);
+    } else {
+      float* p = ka.partials + (uint64_t)blockIdx.x * 2 * a.cols + m.col(j);
+      Values8<float>::store(p, dw[j], m.count(j));
+      Values8<float>::store(p + a.cols, db[j], m.count(j));
+    }
+  }
+}
+
+}  // namespace
+
+#define SH_NORM(name, T, W, C)                                                                                    \
+  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_##name##_##W##x##C##_kernel(    \
+      sh::LayerNormKernelArgs ka) {                                                                               \
+    forward<T, W, C>(ka);                                                                                         \
+  }                                                                                                               \
+  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_backward_##name##_##W##x##C##_kernel( \
+      sh::LayerNormKernelArgs ka) {                                                                               \
+    backward<T, W, C, false>(ka);                                                                                 \
+  }                                                                                                               \
+  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_backward_kept_##name##_##W##x##C##_kernel( \
+      sh::LayerNormKernelArgs ka) {                                                                               \
+    backward<T, W, C, true>(ka);                                                                                  \
+  }
+#define SH_NORM_SHAPES(name, T) \
+  SH_NORM(name, T, 1, 1)        \
+  SH_NORM(name, T, 1, 2)        \
+  SH_NORM(name, T, 4, 1)        \
+  SH_NORM(name, T, 4, 2)        \
+  SH_NORM(name, T, 8, 2)        \
+  SH_NORM(name, T, 16, 2)
+SH_NORM_SHAPES(bf16, __bf16)
+SH_NORM_SHAPES(f16, _Float16)
+SH_NORM_SHAPES(f32, float)
+
+// The gradients of a group's weight and bias from its workgroups' sums: 32 values a workgroup, each added up by 32
+// work-items, every 32nd sum each, that are joined in order.
+extern "C" __global__ __launch_bounds__(sh::kNormJoinThreads) void sh_layer_norm_join_kernel(sh::LayerNormKernelArgs ka) {
+  constexpr uint32_t kCols = sh::kNormJoinCols, kRows = sh::kNormJoinThreads / kCols;
+  const sh_layer_norm_args& a = ka.a;
+  const uint32_t blocks = (a.cols + kCols - 1) / kCols;
+  const uint32_t which = blockIdx.x / blocks % 2, group = blockIdx.x / blocks / 2;
+  const uint32_t col = blockIdx.x % blocks * kCols + threadIdx.x % kCols;
+  void* out = which == 0 ? a.dweight : a.dbias;
+  if (out == nullptr) return;
+  __shared__ float part[kRows][kCols];
+  float v = 0.0f;
+  if (col < a.cols) {
+    const float* p = ka.partials + ((uint64_t)group * ka.per_group * 2 + which) * a.cols + col;
+#pragma unroll 8
+    for (uint32_t k = threadIdx.x / kCols; k < ka.per_group; k += kRows) v += p[(uint64_t)k * 2 * a.cols];
+  }
+  part[threadIdx.x / kCols][threadIdx.x % kCols] = v;
+  __syncthreads();
+  if (threadIdx.x >= kCols || col >= a.cols) return;
+  v = 0.0f;
+  for (uint32_t k = 0; k < kRows; ++k) v += part[k][threadIdx.x];
+  const uint64_t at = (uint64_t)group * a.cols + col;
+  if (a.weight_dtype == SH_DTYPE_BF16) static_cast<__bf16*>(out)[at] = (__bf16)v;
+  else if (a.weight_dtype == SH_DTYPE_F16) static_cast<_Float16*>(out)[at] = (_Float16)v;
+  else static_cast<float*>(out)[at] = v;
+}
