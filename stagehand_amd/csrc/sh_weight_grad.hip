@@ -129,9 +129,10 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
         for (uint32_t part = 0; part < kParts; ++part) {
           Out8 v;
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) {
-            v[i] = (E)rest[i];
-            rest[i] -= (float)v[i];  // exact
+          for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits; all of an infinity
+            const float head = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xFFFF0000u);
+            v[i] = (E)head;
+            rest[i] = rest[i] == head ? 0.0f : rest[i] - head;
           }
           *reinterpret_cast<Out8*>(at + part * kDy) = v;
         }
