@@ -854,7 +854,8 @@ int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype, uint64_t 
  * all their bits. dbias may be NULL. The workspace (16-byte aligned device
  * memory, in use until the call's kernels have run) holds at least
  * sh_weight_grad_act8_workspace bytes, for `bias` as dbias is given. */
-int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t out_features, uint32_t bias, uint64_t* bytes);
+int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t dtype, uint32_t out_features, uint32_t bias,
+                                  uint64_t* bytes);
 int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_ld, uint32_t out_features, const sh_act8* kept,
                         void* dweight, uint32_t out_dtype, uint64_t dw_ld, void* dbias, void* workspace,
                         uint64_t workspace_bytes, void* stream);

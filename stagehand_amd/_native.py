@@ -233,7 +233,7 @@ _SIGNATURES: dict[str, list] = {
     "sh_qk_norm_rope_backward": [_vp, _vp, ctypes.c_uint64, _vp],
     "sh_act8_quantize": [_vp, _u32, ctypes.c_uint64, _vp, _vp],
     "sh_act8_dequantize": [_vp, _vp, _u32, ctypes.c_uint64, _vp],
-    "sh_weight_grad_act8_workspace": [_vp, _u32, _u32, ctypes.POINTER(ctypes.c_uint64)],
+    "sh_weight_grad_act8_workspace": [_vp, _u32, _u32, _u32, ctypes.POINTER(ctypes.c_uint64)],
     "sh_weight_grad_act8": [_vp, _u32, ctypes.c_uint64, _u32, _vp, _vp, _u32, ctypes.c_uint64, _vp, _vp, ctypes.c_uint64, _vp],
     "sh_layer_norm": [_vp, _vp],
     "sh_layer_norm_workspace": [_vp, ctypes.POINTER(ctypes.c_uint64)],

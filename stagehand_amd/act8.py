@@ -144,16 +144,20 @@ def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False,
     device = kept.q.device
     check_device(dy, device, "dy")
     out, features = dy.shape[-1], kept.features
-    if out > 0xFFFFFF:
-        raise ValueError(f"dy must have at most {0xFFFFFF} features, got {out}")
-    rows, _, ld = _token_rows(dy, "dy")
+    if out > MAX_COLS:
+        raise ValueError(f"dy must have at most {MAX_COLS} features, got {out}")
+    rows, tokens, ld = _token_rows(dy, "dy")
+    if tokens > 1 and ld > MAX_COLS:
+        rows, ld = rows.contiguous(), out
+    elif tokens <= 1:
+        ld = out
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return weight_grad_act8(dy, kept, bias=bias, out_dtype=out_dtype)
     dw = torch.empty((out, features), dtype=out_dtype, device=device)
     db = torch.empty(out, dtype=out_dtype, device=device) if bias else None
     lib, need = _native.lib(), ctypes.c_uint64()
-    _native.check(lib.sh_weight_grad_act8_workspace(args, out, bool(bias), ctypes.byref(need)))
+    _native.check(lib.sh_weight_grad_act8_workspace(args, DTYPE_CODES[dy.dtype], out, bool(bias), ctypes.byref(need)))
     ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
     _native.check(lib.sh_weight_grad_act8(rows.data_ptr(), DTYPE_CODES[dy.dtype], ld, out, args, dw.data_ptr(), DTYPE_CODES[out_dtype],
                                           features, None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),

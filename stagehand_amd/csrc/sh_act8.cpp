@@ -73,12 +73,12 @@ struct GradPlan {
 constexpr uint32_t kComputeUnits = 256;
 
 // The tile, and into how many parts the tokens are split where the tiles alone leave compute units idle.
-GradPlan plan_of(const sh_act8* k, uint32_t out, bool bias) {
+GradPlan plan_of(const sh_act8* k, uint32_t out, uint32_t dtype, bool bias) {
   GradPlan p{};
   auto tiles = [&](int i) {
     return (uint64_t)((out + sh::kGradTiles[i].out - 1) / sh::kGradTiles[i].out) * ((k->cols + sh::kGradTiles[i].in - 1) / sh::kGradTiles[i].in);
   };
-  p.tile = out <= 64 ? 0 : tiles(2) >= kComputeUnits / 2 ? 2 : 1;
+  p.tile = out <= 64 ? 0 : dtype != SH_DTYPE_F32 && tiles(2) >= kComputeUnits / 2 ? 2 : 1;
   p.tiles = (uint32_t)tiles(p.tile);
   const uint32_t steps = std::max(1u, (k->tokens + sh::kGradStep - 1) / sh::kGradStep);
   const uint32_t want = p.tiles >= kComputeUnits ? 1 : 2 * kComputeUnits / std::max(1u, p.tiles);
@@ -108,12 +108,13 @@ extern "C" int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype
   return launch_act8(kept, out, out_ld, dtype, true, (hipStream_t)stream, who);
 }
 
-extern "C" int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t out_features, uint32_t bias, uint64_t* bytes) {
+extern "C" int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t dtype, uint32_t out_features, uint32_t bias, uint64_t* bytes) {
   const char* who = "sh_weight_grad_act8_workspace";
   sh::clear_error();
   if (bytes == nullptr) return sh::fail(SH_ERR_INVALID, "%s: bytes is NULL", who);
   if (int st = check_kept(kept, who)) return st;
-  *bytes = plan_of(kept, out_features, bias != 0).bytes;
+  if (!known_dtype(dtype)) return sh::fail(SH_ERR_INVALID, "%s: unknown dtype %u", who, dtype);
+  *bytes = plan_of(kept, out_features, dtype, bias != 0).bytes;
   return SH_OK;
 }
 
@@ -124,11 +125,14 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   sh::clear_error();
   if (int st = check_kept(kept, who)) return st;
   if (int st = check_values(dy, "dy", dtype, out_features == 0 ? 0 : kept->tokens, who)) return st;
+  if (out_features > SH_ACT8_MAX_COLS || dy_ld > SH_ACT8_MAX_COLS)
+    return sh::fail(SH_ERR_INVALID, "%s: out_features %u or dy_ld %llu is more than %u", who, out_features, (unsigned long long)dy_ld,
+                    SH_ACT8_MAX_COLS);
   if (int st = check_values(dweight, "dweight", out_dtype, out_features, who)) return st;
   if (int st = check_out_rows(dw_ld, out_features, kept->cols, "dw_ld", who)) return st;
   if (misaligned(dbias, dtype_bytes(out_dtype))) return sh::fail(SH_ERR_INVALID, "%s: dbias is not aligned to its type", who);
   if (out_features == 0) return SH_OK;
-  const GradPlan p = plan_of(kept, out_features, dbias != nullptr);
+  const GradPlan p = plan_of(kept, out_features, dtype, dbias != nullptr);
   if (workspace_bytes < p.bytes || (p.bytes > 0 && workspace == nullptr))
     return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
                     (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
@@ -152,7 +156,8 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   a.split_tokens = p.split_tokens;
   a.dtype = dtype;
   a.out_dtype = out_dtype;
-  static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount, "one kernel per type and tile");
+  a.dy_words = !misaligned(dy, 4) && dy_ld * dtype_bytes(dtype) % 4 == 0 && (uint64_t)out_features * dtype_bytes(dtype) % 4 == 0;
+  static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount - 1, "one kernel per type and tile");
   void* args[] = {(void*)&a};
   if (int st = sh::launch_kernel((sh::KernelId)(sh::kKernWeightGradBf1632x128 + (dtype - SH_DTYPE_BF16) * sh::kGradTileCount + p.tile),
                                  p.tiles * p.splits, tile.threads, (hipStream_t)stream, args, who))

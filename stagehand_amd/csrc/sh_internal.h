@@ -236,7 +236,7 @@ enum KernelId : int {
   kKernAct8DequantizeF16,
   kKernAct8QuantizeF32,
   kKernAct8DequantizeF32,
-  // weight gradients: per type and tile of sh_act8_args.h
+  // weight gradients: per type and tile of sh_act8_args.h, without the largest for fp32
   kKernWeightGradBf1632x128,
   kKernWeightGradBf16128x128,
   kKernWeightGradBf16256x256,
@@ -245,7 +245,6 @@ enum KernelId : int {
   kKernWeightGradF16256x256,
   kKernWeightGradF3232x128,
   kKernWeightGradF32128x128,
-  kKernWeightGradF32256x256,
   kKernWeightGradJoin,
   kKernelCount
 };

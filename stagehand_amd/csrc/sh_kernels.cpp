@@ -217,7 +217,6 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModWeightGrad, "sh_weight_grad_f16_256x256_kernel"},
     {kModWeightGrad, "sh_weight_grad_f32_32x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_f32_128x128_kernel"},
-    {kModWeightGrad, "sh_weight_grad_f32_256x256_kernel"},
     {kModWeightGrad, "sh_weight_grad_join_kernel"},
 };
 

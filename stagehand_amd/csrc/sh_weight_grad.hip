@@ -59,14 +59,38 @@ __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t t) {
 
 typedef __attribute__((address_space(3))) s16x4_t* LdsRead;
 
+// Where a lane's reads of unit 0 start. Unit u lies at this ^ 16 u: the other parts of the place have no bits there.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t read_place() {
+  const uint32_t lane = threadIdx.x & 63, t = lane / 16 * 8 + lane % 16 / 4;
+  return t * N + swizzle<N>(t) * 16 + lane % 4 * 4;
+}
+
 // The fragment of unit u: lane l gets values of column l % 16, tokens 8 (l / 16) .. + 7.
 template <uint32_t N>
-__device__ __forceinline__ s16x8_t read_fragment(const short* stage, uint32_t u) {
-  const uint32_t lane = threadIdx.x & 63, t = lane / 16 * 8 + lane % 16 / 4;
-  const short* p = stage + t * N + (u ^ swizzle<N>(t)) * 16 + lane % 4 * 4;
+__device__ __forceinline__ s16x8_t read_fragment(const short* stage, uint32_t place, uint32_t u) {
+  const short* p = stage + (place ^ u * 16);
   const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRead)p);
   const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsRead)(p + 4 * N));
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Buffer resource of `rows` rows from p on, `ld` bytes apart, of which the last ends after `width` bytes: reads past that give 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_resource(const void* p, uint32_t ld, uint32_t rows, uint32_t width) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, rows > 0 ? (rows - 1) * ld + width : 0, 0x00020000);
+}
+
+// f(0), f(1) .. f(N - 1) with constants for the compiler.
+template <uint32_t I>
+struct Constant {
+  static constexpr uint32_t value = I;
+};
+template <uint32_t N, uint32_t I = 0, typename F>
+__device__ __forceinline__ void each(const F& f) {
+  if constexpr (I < N) {
+    f(Constant<I>{});
+    each<N, I + 1>(f);
+  }
 }
 
 template <typename T, uint32_t TO, uint32_t TI, uint32_t WO, uint32_t WI>
@@ -75,7 +99,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   constexpr uint32_t kParts = Multiplied<T>::kParts, kStep = sh::kGradStep;
   constexpr uint32_t kThreads = WO * WI * 64, FO = TO / WO / 16, FI = TI / WI / 16;
   static_assert(FI == 4, "a wavefront's inputs are one group of 64 permuted ones");
-  constexpr uint32_t kDy = kStep * TO, kStage = kParts * kDy + kStep * TI;
+  constexpr uint32_t kDy = kStep * TO, kStage = kParts * kDy + kStep * TI, kGroups64 = TI / 64;
   constexpr uint32_t ND = (kDy / 8 + kThreads - 1) / kThreads, NX = (kStep * TI / 16 + kThreads - 1) / kThreads;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wo = wave / WI, wi = wave % WI;
@@ -89,105 +113,178 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   const uint32_t t_begin = split * a.split_tokens, t_end = min(a.tokens, t_begin + a.split_tokens);
   const uint32_t groups = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP;
 
-  typename Values8<T>::Vec dy[ND];
-  uint4 q[NX];
-  uint32_t e[NX];
-  auto load = [&](uint32_t t0) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t j = 0; j < ND; ++j) {
-      const uint32_t c = j * kThreads + threadIdx.x, t = t0 + c / (TO / 8), o = o0 + c % (TO / 8) * 8;
-      dy[j] = Values8<T>::zero();
-      if (c < kDy / 8 && t < t_end && o < a.out) dy[j] = Values8<T>::load(static_cast<const T*>(a.dy) + t * a.dy_ld + o, a.out - o);
-    }
+  // A stage on its way to LDS. The next one that is loaded starts at dy_at, q_at and e_at and has `left` tokens at most.
+  struct Staged {
+    typename Values8<T>::Vec dy[ND];
+    uint4 q[NX];
+    uint32_t e[NX];
+  };
+  const T* dy_at = static_cast<const T*>(a.dy) + t_begin * a.dy_ld + o0;
+  const uint8_t* q_at = static_cast<const uint8_t*>(a.q) + (uint64_t)t_begin * groups * SH_ACT8_GROUP + i0;
+  const uint8_t* e_at = static_cast<const uint8_t*>(a.exponent) + (uint64_t)t_begin * groups + i0 / SH_ACT8_GROUP;
+  uint32_t left = t_begin < t_end ? t_end - t_begin : 0;
+  const uint32_t dy_ld = (uint32_t)a.dy_ld * sizeof(T), q_ld = groups * SH_ACT8_GROUP;
+  const uint32_t dy_t = threadIdx.x / (TO / 8), dy_o = threadIdx.x % (TO / 8) * 8;
+  const uint32_t q_t = threadIdx.x / (TI / 16), q_i = threadIdx.x % (TI / 16) * 16;
+  const uint32_t dy_off = dy_t * dy_ld + dy_o * sizeof(T), q_off = q_t * q_ld + q_i, e_off = q_t * groups + q_i / SH_ACT8_GROUP;
+  constexpr uint32_t kDyRows = kThreads / (TO / 8), kQRows = kThreads / (TI / 16);
+  auto load = [&](Staged& v) __attribute__((always_inline)) {
+    const uint32_t rows = min(left, kStep);
+    const auto qr = rows_resource(q_at, q_ld, rows, q_ld - i0), er = rows_resource(e_at, groups, rows, groups - i0 / SH_ACT8_GROUP);
 #pragma unroll
     for (uint32_t j = 0; j < NX; ++j) {
-      const uint32_t c = j * kThreads + threadIdx.x, t = t0 + c / (TI / 16), i = i0 + c % (TI / 16) * 16;
-      q[j] = make_uint4(0, 0, 0, 0);
-      e[j] = 1;
-      if (c < kStep * TI / 16 && t < t_end && i < groups * SH_ACT8_GROUP) {
-        const uint64_t at = (uint64_t)t * groups * SH_ACT8_GROUP + i;
-        q[j] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + at);
-        e[j] = static_cast<const uint8_t*>(a.exponent)[at / SH_ACT8_GROUP];
+      v.q[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(qr, q_off + j * kQRows * q_ld, 0, 0));
+      v.e[j] = __builtin_amdgcn_raw_buffer_load_b8(er, e_off + j * kQRows * groups, 0, 0);
+    }
+    if (a.dy_words) {
+      const auto dr = rows_resource(dy_at, dy_ld, rows, (a.out - o0) * (uint32_t)sizeof(T));
+#pragma unroll
+      for (uint32_t j = 0; j < ND; ++j) {
+        typedef uint32_t Words __attribute__((ext_vector_type(4 * sizeof(T) / 2)));
+        Words w;
+#pragma unroll
+        for (uint32_t k = 0; k < sizeof(T) / 2; ++k) {
+          const auto part = __builtin_amdgcn_raw_buffer_load_b128(dr, dy_off + j * kDyRows * dy_ld + k * 16, 0, 0);
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) w[k * 4 + i] = part[i];
+        }
+        v.dy[j] = __builtin_bit_cast(typename Values8<T>::Vec, w);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < ND; ++j) {
+        v.dy[j] = Values8<T>::zero();
+        const uint32_t t = dy_t + j * kDyRows;
+        if (t < rows && o0 + dy_o < a.out) v.dy[j] = Values8<T>::load(dy_at + t * a.dy_ld + dy_o, a.out - o0 - dy_o);
       }
     }
+    dy_at += kStep * a.dy_ld;
+    q_at += kStep * q_ld;
+    e_at += kStep * groups;
+    left -= rows;
   };
   typedef E Out4 __attribute__((ext_vector_type(4)));
   typedef E Out8 __attribute__((ext_vector_type(8)));
-  auto put = [&](short* stage) __attribute__((always_inline)) {
+  // Sums over the tokens that a work-item stages: always of the same 8 outputs.
+  const bool with_bias = a.dbias != nullptr && i0 == 0;
+  float bias[8] = {};
+  const uint32_t dy_place = dy_t * TO + ((dy_o / 16) ^ swizzle<TO>(dy_t)) * 16 + dy_o % 16;
+  static_assert(kDyRows % 16 == 0 || ND == 1, "a work-item's rows have one swizzle");
+  auto put_dy = [&](const Staged& v, short* stage) __attribute__((always_inline)) {
+    if (kDy / 8 < kThreads && threadIdx.x >= kDy / 8) return;
+    if (with_bias) {
+#pragma unroll
+      for (uint32_t j = 0; j < ND; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) bias[i] += (float)v.dy[j][i];
+    }
 #pragma unroll
     for (uint32_t j = 0; j < ND; ++j) {
-      const uint32_t c = j * kThreads + threadIdx.x, t = c / (TO / 8), c8 = c % (TO / 8);
-      if (c >= kDy / 8) continue;
-      short* at = stage + t * TO + ((c8 / 2) ^ swizzle<TO>(t)) * 16 + c8 % 2 * 8;
+      short* at = stage + dy_place + j * kDyRows * TO;
       if constexpr (kParts == 1) {
-        *reinterpret_cast<typename Values8<T>::Vec*>(at) = dy[j];
+        *reinterpret_cast<typename Values8<T>::Vec*>(at) = v.dy[j];
       } else {
         float rest[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) rest[i] = dy[j][i];
+        for (uint32_t i = 0; i < 8; ++i) rest[i] = v.dy[j][i];
 #pragma unroll
         for (uint32_t part = 0; part < kParts; ++part) {
-          Out8 v;
+          Out8 out;
 #pragma unroll
           for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits; all of an infinity
             const float head = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xFFFF0000u);
-            v[i] = (E)head;
+            out[i] = (E)head;
             rest[i] = rest[i] == head ? 0.0f : rest[i] - head;
           }
-          *reinterpret_cast<Out8*>(at + part * kDy) = v;
+          *reinterpret_cast<Out8*>(at + part * kDy) = out;
         }
       }
     }
+  };
+  // Column 64 g + 16 p + 4 f + m of x^ is column 4 p + m of the unit f * kGroups64 + g, fragment f of the group g: a lane
+  // of the product then has 16 consecutive inputs.
+  static_assert(kQRows % 16 == 0 || NX == 1, "a work-item's rows have one swizzle");
+  const uint32_t x_place = q_t * TI + ((q_i / 64) ^ swizzle<TI>(q_t)) * 16 + q_i % 64 / 4;
+  auto put_x = [&](const Staged& v, short* stage) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t j = 0; j < NX; ++j) {
-      const uint32_t c = j * kThreads + threadIdx.x, t = c / (TI / 16), c16 = c % (TI / 16);
-      if (c >= kStep * TI / 16) continue;
-      const float scale = group_scale(e[j]);
-      const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+      const float scale = group_scale(v.e[j]);
+      const uint32_t words[4] = {v.q[j].x, v.q[j].y, v.q[j].z, v.q[j].w};
 #pragma unroll
-      for (uint32_t f = 0; f < 4; ++f) {  // column c16 * 16 + f * 4 + m is column c16 % 4 * 4 + m of fragment f
-        float v[4];
-        dequantize4(words[f], scale, v);
+      for (uint32_t f = 0; f < 4; ++f) {
+        float x[4];
+        dequantize4(words[f], scale, x);
         Out4 out;
 #pragma unroll
-        for (uint32_t m = 0; m < 4; ++m) out[m] = (E)v[m];
-        *reinterpret_cast<Out4*>(stage + kParts * kDy + t * TI + ((c16 / 4 * 4 + f) ^ swizzle<TI>(t)) * 16 + c16 % 4 * 4) = out;
+        for (uint32_t m = 0; m < 4; ++m) out[m] = (E)x[m];
+        *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = out;
       }
     }
   };
+  static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
+  const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
+  auto read_x = [&](const short* stage, uint32_t j) __attribute__((always_inline)) {
+    return read_fragment<TI>(stage + kParts * kDy, x_read, j * kGroups64);
+  };
+  // Fragment b of dy: of part b / FO.
+  auto read_dy = [&](const short* stage, uint32_t b) __attribute__((always_inline)) {
+    return read_fragment<TO>(stage + b / FO * kDy, dy_read, b % FO);
+  };
 
-  f32x4_t acc[FO][FI] = {}, bias[FO] = {};
-  const bool with_bias = a.dbias != nullptr && i0 == 0 && wi == 0;
-  s16x8_t ones;
-  {
-    Out8 v;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) v[i] = (E)1.0f;
-    ones = __builtin_bit_cast(s16x8_t, v);
-  }
-  load(t_begin);
-  put(lds);
-  uint32_t s = 0;
-  for (uint32_t t0 = t_begin; t0 < t_end; t0 += kStep) {
-    __syncthreads();  // stage s is written, and read the one that is written next
-    const bool more = t0 + kStep < t_end;
-    if (more) load(t0 + kStep);
+  f32x4_t acc[FO][FI] = {};
+  constexpr uint32_t NB = kParts * FO, kAhead = NB < 2 ? NB : 2;
+  Staged staged[2];
+  s16x8_t x[2][FI], d[NB + kAhead];
+  // One stage: fragment b of dy is multiplied while fragment b + 2 is read. The first half also writes the next stage to
+  // LDS and starts the loads of the one after the next two; after the barrier in its middle, the second half reads the
+  // next stage's first fragments. A third stage of LDS is written while the other two are read.
+  auto multiply = [&](auto turn, uint32_t s) __attribute__((always_inline)) {
+    constexpr uint32_t V = decltype(turn)::value;
     const short* stage = lds + s * kStage;
-    s16x8_t x[FI];
-#pragma unroll
-    for (uint32_t j = 0; j < FI; ++j) x[j] = read_fragment<TI>(stage + kParts * kDy, wi * FI + j);
-#pragma unroll
-    for (uint32_t part = 0; part < kParts; ++part) {
-#pragma unroll
-      for (uint32_t i = 0; i < FO; ++i) {
-        const s16x8_t d = read_fragment<TO>(stage + part * kDy, wo * FO + i);
-#pragma unroll
-        for (uint32_t j = 0; j < FI; ++j) acc[i][j] = mfma<E>(x[j], d, acc[i][j]);
-        if (with_bias) bias[i] = mfma<E>(ones, d, bias[i]);
+    short* next = lds + (s == 2 ? 0 : s + 1) * kStage;
+    each<NB>([&](auto block) __attribute__((always_inline)) {
+      constexpr uint32_t B = decltype(block)::value;
+      if constexpr (B == 0) put_x(staged[V ^ 1], next);
+      if constexpr (B == (NB > 2 ? 1 : 0)) {
+        put_dy(staged[V ^ 1], next);
+        load(staged[V ^ 1]);
       }
-    }
-    s ^= 1;
-    if (more) put(lds + s * kStage);
+      if constexpr (B + kAhead < NB) d[B + kAhead] = read_dy(stage, B + kAhead);
+      if constexpr (B == NB / 2) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if constexpr (B >= NB / 2) {
+        constexpr uint32_t kFrom = (B - NB / 2) * FI / (NB - NB / 2), kTo = (B - NB / 2 + 1) * FI / (NB - NB / 2);
+        each<kTo, kFrom>([&](auto j) __attribute__((always_inline)) { x[V ^ 1][decltype(j)::value] = read_x(next, decltype(j)::value); });
+      }
+      if constexpr (B + kAhead >= NB) d[B + kAhead] = read_dy(next, B + kAhead - NB);
+      each<FI>([&](auto j) __attribute__((always_inline)) {
+        constexpr uint32_t J = decltype(j)::value;
+        acc[B % FO][J] = mfma<E>(x[V][J], d[B], acc[B % FO][J]);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+#pragma unroll
+    for (uint32_t b = 0; b < kAhead; ++b) d[b] = d[NB + b];
+  };
+  load(staged[0]);
+  put_x(staged[0], lds);
+  put_dy(staged[0], lds);
+  load(staged[1]);
+  load(staged[0]);
+  __syncthreads();
+#pragma unroll
+  for (uint32_t j = 0; j < FI; ++j) x[0][j] = read_x(lds, j);
+#pragma unroll
+  for (uint32_t b = 0; b < kAhead; ++b) d[b] = read_dy(lds, b);
+  uint32_t s = 0;
+  for (uint32_t t0 = t_begin; t0 < t_end; t0 += 2 * kStep) {
+    multiply(Constant<0>{}, s);
+    s = s == 2 ? 0 : s + 1;
+    multiply(Constant<1>{}, s);
+    s = s == 2 ? 0 : s + 1;
   }
 
   // lane: output l % 16 of each fragment of outputs, 16 consecutive inputs
@@ -214,12 +311,27 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
         else Values8<float>::store(static_cast<float*>(a.dweight) + at, v[h], n);
       }
     }
-    if (with_bias && lane < 16) {  // every row of the product with ones
-      if (sums != nullptr) sums[(uint64_t)a.out * a.cols + o] = bias[f][0];
-      else if (a.out_dtype == SH_DTYPE_BF16) static_cast<__bf16*>(a.dbias)[o] = (__bf16)bias[f][0];
-      else if (a.out_dtype == SH_DTYPE_F16) static_cast<_Float16*>(a.dbias)[o] = (_Float16)bias[f][0];
-      else static_cast<float*>(a.dbias)[o] = bias[f][0];
-    }
+  }
+  if (!with_bias) return;
+  // an output's sums, in their order
+  __syncthreads();  // the stages are not read any more
+  float* sum = reinterpret_cast<float*>(lds);
+  if (kDy / 8 >= kThreads || threadIdx.x < kDy / 8) {
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) sum[dy_t * TO + dy_o + k] = bias[k];
+  }
+  __syncthreads();
+  constexpr uint32_t kSums = kDyRows < kStep ? kDyRows : kStep;
+  for (uint32_t k = threadIdx.x; k < TO; k += kThreads) {
+    const uint32_t o = o0 + k;
+    if (o >= a.out) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (uint32_t r = 0; r < kSums; ++r) v += sum[r * TO + k];
+    if (sums != nullptr) sums[(uint64_t)a.out * a.cols + o] = v;
+    else if (a.out_dtype == SH_DTYPE_BF16) static_cast<__bf16*>(a.dbias)[o] = (__bf16)v;
+    else if (a.out_dtype == SH_DTYPE_F16) static_cast<_Float16*>(a.dbias)[o] = (_Float16)v;
+    else static_cast<float*>(a.dbias)[o] = v;
   }
 }
 
@@ -227,17 +339,18 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
 
 // The tiles of sh_act8_args.h.
 #define SH_WEIGHT_GRAD(name, T, TO, TI, WO, WI)                                                                   \
-  extern "C" __global__ __launch_bounds__(WO * WI * 64) void sh_weight_grad_##name##_##TO##x##TI##_kernel(sh::WeightGradArgs a) { \
-    __shared__ alignas(16) short lds[2 * sh::kGradStep * (Multiplied<T>::kParts * TO + TI)];                      \
+  extern "C" __global__ __launch_bounds__(WO * WI * 64, 2) void sh_weight_grad_##name##_##TO##x##TI##_kernel(sh::WeightGradArgs a) { \
+    __shared__ alignas(16) short lds[3 * sh::kGradStep * (Multiplied<T>::kParts * TO + TI)];                      \
     weight_grad<T, TO, TI, WO, WI>(a, lds);                                                                       \
   }
-#define SH_WEIGHT_GRAD_TILES(name, T)       \
-  SH_WEIGHT_GRAD(name, T, 32, 128, 2, 2)    \
-  SH_WEIGHT_GRAD(name, T, 128, 128, 2, 2)   \
-  SH_WEIGHT_GRAD(name, T, 256, 256, 2, 4)
-SH_WEIGHT_GRAD_TILES(bf16, __bf16)
-SH_WEIGHT_GRAD_TILES(f16, _Float16)
-SH_WEIGHT_GRAD_TILES(f32, float)
+SH_WEIGHT_GRAD(bf16, __bf16, 32, 128, 2, 2)
+SH_WEIGHT_GRAD(bf16, __bf16, 128, 128, 2, 2)
+SH_WEIGHT_GRAD(bf16, __bf16, 256, 256, 2, 4)
+SH_WEIGHT_GRAD(f16, _Float16, 32, 128, 2, 2)
+SH_WEIGHT_GRAD(f16, _Float16, 128, 128, 2, 2)
+SH_WEIGHT_GRAD(f16, _Float16, 256, 256, 2, 4)
+SH_WEIGHT_GRAD(f32, float, 32, 128, 2, 2)
+SH_WEIGHT_GRAD(f32, float, 128, 128, 2, 2)
 
 // dweight and dbias from the sums of the splits, in their order: four values a work-item, then the biases.
 extern "C" __global__ __launch_bounds__(sh::kGradJoinThreads) void sh_weight_grad_join_kernel(sh::WeightGradArgs a) {
