@@ -156,7 +156,6 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   a.split_tokens = p.split_tokens;
   a.dtype = dtype;
   a.out_dtype = out_dtype;
-  a.dy_words = !misaligned(dy, 4) && dy_ld * dtype_bytes(dtype) % 4 == 0 && (uint64_t)out_features * dtype_bytes(dtype) % 4 == 0;
   static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount - 1, "one kernel per type and tile");
   void* args[] = {(void*)&a};
   if (int st = sh::launch_kernel((sh::KernelId)(sh::kKernWeightGradBf1632x128 + (dtype - SH_DTYPE_BF16) * sh::kGradTileCount + p.tile),

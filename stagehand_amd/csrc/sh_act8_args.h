@@ -34,7 +34,6 @@ struct WeightGradArgs {
   uint32_t splits;        // parts of the tokens, each summed by workgroups of its own
   uint32_t split_tokens;  // tokens of a part, a multiple of kGradStep
   uint32_t dtype, out_dtype;
-  uint32_t dy_words;  // whether dy's rows start and end on multiples of 4 bytes
 };
 
 constexpr uint32_t kGradStep = 32;  // tokens that are staged at a time

@@ -104,12 +104,15 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wo = wave / WI, wi = wave % WI;
 
-  // XCDs take consecutive runs of tiles, an XCD's L2 then serves neighbouring ones
+  // XCDs take consecutive runs of tiles, which run down groups of kGroup tiles of outputs: an XCD's L2 then serves a block of
+  // 8 x 4 tiles.
+  constexpr uint32_t kGroup = 8;
   const uint32_t tiles_o = (a.out + TO - 1) / TO, tiles_i = (a.cols + TI - 1) / TI, tiles = tiles_o * tiles_i;
   const uint32_t all = tiles * a.splits, xcd = blockIdx.x % 8;
   const uint32_t p = xcd * (all / 8) + min(xcd, all % 8) + blockIdx.x / 8;
   const uint32_t split = p / tiles, tile = p % tiles;
-  const uint32_t o0 = tile % tiles_o * TO, i0 = tile / tiles_o * TI;
+  const uint32_t group = tile / (kGroup * tiles_i), in_group = tile % (kGroup * tiles_i), g_rows = min(tiles_o - group * kGroup, kGroup);
+  const uint32_t o0 = (group * kGroup + in_group % g_rows) * TO, i0 = in_group / g_rows * TI;
   const uint32_t t_begin = split * a.split_tokens, t_end = min(a.tokens, t_begin + a.split_tokens);
   const uint32_t groups = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP;
 
@@ -127,6 +130,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   const uint32_t dy_t = threadIdx.x / (TO / 8), dy_o = threadIdx.x % (TO / 8) * 8;
   const uint32_t q_t = threadIdx.x / (TI / 16), q_i = threadIdx.x % (TI / 16) * 16;
   const uint32_t dy_off = dy_t * dy_ld + dy_o * sizeof(T), q_off = q_t * q_ld + q_i, e_off = q_t * groups + q_i / SH_ACT8_GROUP;
+  const bool dy_odd = sizeof(T) == 2 && a.out % 2 != 0;
   constexpr uint32_t kDyRows = kThreads / (TO / 8), kQRows = kThreads / (TI / 16);
   auto load = [&](Staged& v) __attribute__((always_inline)) {
     const uint32_t rows = min(left, kStep);
@@ -136,26 +140,30 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
       v.q[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(qr, q_off + j * kQRows * q_ld, 0, 0));
       v.e[j] = __builtin_amdgcn_raw_buffer_load_b8(er, e_off + j * kQRows * groups, 0, 0);
     }
-    if (a.dy_words) {
-      const auto dr = rows_resource(dy_at, dy_ld, rows, (a.out - o0) * (uint32_t)sizeof(T));
+    // An odd number of 16-bit values ends within a word, which is not read past the resource's end: where another row
+    // follows, the resource ends after that word.
+    const auto dr = rows_resource(dy_at, dy_ld, rows, (a.out - o0) * (uint32_t)sizeof(T) + (dy_odd && left > kStep ? 2 : 0));
 #pragma unroll
-      for (uint32_t j = 0; j < ND; ++j) {
-        typedef uint32_t Words __attribute__((ext_vector_type(4 * sizeof(T) / 2)));
-        Words w;
+    for (uint32_t j = 0; j < ND; ++j) {
+      typedef uint32_t Words __attribute__((ext_vector_type(4 * sizeof(T) / 2)));
+      Words w;
 #pragma unroll
-        for (uint32_t k = 0; k < sizeof(T) / 2; ++k) {
-          const auto part = __builtin_amdgcn_raw_buffer_load_b128(dr, dy_off + j * kDyRows * dy_ld + k * 16, 0, 0);
+      for (uint32_t k = 0; k < sizeof(T) / 2; ++k) {
+        const auto part = __builtin_amdgcn_raw_buffer_load_b128(dr, dy_off + j * kDyRows * dy_ld + k * 16, 0, 0);
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) w[k * 4 + i] = part[i];
-        }
-        v.dy[j] = __builtin_bit_cast(typename Values8<T>::Vec, w);
+        for (uint32_t i = 0; i < 4; ++i) w[k * 4 + i] = part[i];
       }
-    } else {
+      v.dy[j] = __builtin_bit_cast(typename Values8<T>::Vec, w);
+    }
+    if (dy_odd && left <= kStep) {  // the last value of all is read by itself
 #pragma unroll
       for (uint32_t j = 0; j < ND; ++j) {
-        v.dy[j] = Values8<T>::zero();
-        const uint32_t t = dy_t + j * kDyRows;
-        if (t < rows && o0 + dy_o < a.out) v.dy[j] = Values8<T>::load(dy_at + t * a.dy_ld + dy_o, a.out - o0 - dy_o);
+        const uint32_t t = dy_t + j * kDyRows, last = a.out - 1 - o0 - dy_o;
+        if (t + 1 != rows || last >= 8) continue;
+        const T value = dy_at[t * a.dy_ld + dy_o + last];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+          if (i == last) v.dy[j][i] = value;
       }
     }
     dy_at += kStep * a.dy_ld;
@@ -170,16 +178,16 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   float bias[8] = {};
   const uint32_t dy_place = dy_t * TO + ((dy_o / 16) ^ swizzle<TO>(dy_t)) * 16 + dy_o % 16;
   static_assert(kDyRows % 16 == 0 || ND == 1, "a work-item's rows have one swizzle");
-  auto put_dy = [&](const Staged& v, short* stage) __attribute__((always_inline)) {
+  auto add_bias = [&](const Staged& v) __attribute__((always_inline)) {
+    if (!with_bias) return;
+#pragma unroll
+    for (uint32_t j = 0; j < ND; ++j)
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) bias[i] += (float)v.dy[j][i];
+  };
+  auto put_dy = [&](const Staged& v, short* stage, uint32_t j) __attribute__((always_inline)) {
     if (kDy / 8 < kThreads && threadIdx.x >= kDy / 8) return;
-    if (with_bias) {
-#pragma unroll
-      for (uint32_t j = 0; j < ND; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) bias[i] += (float)v.dy[j][i];
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < ND; ++j) {
+    {
       short* at = stage + dy_place + j * kDyRows * TO;
       if constexpr (kParts == 1) {
         *reinterpret_cast<typename Values8<T>::Vec*>(at) = v.dy[j];
@@ -205,21 +213,14 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   // of the product then has 16 consecutive inputs.
   static_assert(kQRows % 16 == 0 || NX == 1, "a work-item's rows have one swizzle");
   const uint32_t x_place = q_t * TI + ((q_i / 64) ^ swizzle<TI>(q_t)) * 16 + q_i % 64 / 4;
-  auto put_x = [&](const Staged& v, short* stage) __attribute__((always_inline)) {
+  auto put_x = [&](const Staged& v, short* stage, uint32_t j, uint32_t f) __attribute__((always_inline)) {
+    const uint32_t words[4] = {v.q[j].x, v.q[j].y, v.q[j].z, v.q[j].w};
+    float x[4];
+    dequantize4(words[f], group_scale(v.e[j]), x);
+    Out4 out;
 #pragma unroll
-    for (uint32_t j = 0; j < NX; ++j) {
-      const float scale = group_scale(v.e[j]);
-      const uint32_t words[4] = {v.q[j].x, v.q[j].y, v.q[j].z, v.q[j].w};
-#pragma unroll
-      for (uint32_t f = 0; f < 4; ++f) {
-        float x[4];
-        dequantize4(words[f], scale, x);
-        Out4 out;
-#pragma unroll
-        for (uint32_t m = 0; m < 4; ++m) out[m] = (E)x[m];
-        *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = out;
-      }
-    }
+    for (uint32_t m = 0; m < 4; ++m) out[m] = (E)x[m];
+    *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = out;
   };
   static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
   const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
@@ -237,17 +238,23 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   s16x8_t x[2][FI], d[NB + kAhead];
   // One stage: fragment b of dy is multiplied while fragment b + 2 is read. The first half also writes the next stage to
   // LDS and starts the loads of the one after the next two; after the barrier in its middle, the second half reads the
-  // next stage's first fragments. A third stage of LDS is written while the other two are read.
+  // next stage's first fragments. A third stage of LDS is written while the other two are read. The instructions of a
+  // part are spread between its products: all at once they would hold up the products of both wavefronts of a SIMD.
+  constexpr uint32_t kHalf = NB / 2 > 0 ? NB / 2 : 1, kWrites = NX * 4 + ND;
   auto multiply = [&](auto turn, uint32_t s) __attribute__((always_inline)) {
     constexpr uint32_t V = decltype(turn)::value;
     const short* stage = lds + s * kStage;
     short* next = lds + (s == 2 ? 0 : s + 1) * kStage;
     each<NB>([&](auto block) __attribute__((always_inline)) {
       constexpr uint32_t B = decltype(block)::value;
-      if constexpr (B == 0) put_x(staged[V ^ 1], next);
-      if constexpr (B == (NB > 2 ? 1 : 0)) {
-        put_dy(staged[V ^ 1], next);
-        load(staged[V ^ 1]);
+      if constexpr (B == 0) add_bias(staged[V ^ 1]);
+      if constexpr (B < kHalf) {
+        each<(B + 1) * kWrites / kHalf, B * kWrites / kHalf>([&](auto w) __attribute__((always_inline)) {
+          constexpr uint32_t I = decltype(w)::value;
+          if constexpr (I < NX * 4) put_x(staged[V ^ 1], next, I / 4, I % 4);
+          else put_dy(staged[V ^ 1], next, I - NX * 4);
+        });
+        if constexpr (B == kHalf - 1) load(staged[V ^ 1]);
       }
       if constexpr (B + kAhead < NB) d[B + kAhead] = read_dy(stage, B + kAhead);
       if constexpr (B == NB / 2) {
@@ -264,14 +271,22 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
         constexpr uint32_t J = decltype(j)::value;
         acc[B % FO][J] = mfma<E>(x[V][J], d[B], acc[B % FO][J]);
       });
+      each<FI>([&](auto) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+        __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // an LDS write
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a load
+      });
       __builtin_amdgcn_sched_barrier(0);
     });
 #pragma unroll
     for (uint32_t b = 0; b < kAhead; ++b) d[b] = d[NB + b];
   };
   load(staged[0]);
-  put_x(staged[0], lds);
-  put_dy(staged[0], lds);
+  add_bias(staged[0]);
+  each<NX * 4>([&](auto i) __attribute__((always_inline)) { put_x(staged[0], lds, decltype(i)::value / 4, decltype(i)::value % 4); });
+  each<ND>([&](auto j) __attribute__((always_inline)) { put_dy(staged[0], lds, decltype(j)::value); });
   load(staged[1]);
   load(staged[0]);
   __syncthreads();
