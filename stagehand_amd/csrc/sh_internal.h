@@ -174,60 +174,51 @@ enum KernelId : int {
   kKernQkNormBackwardF321Interleaved,
   kKernQkNormDweight,
   // layer norms: per type and shape of sh_layer_norm_args.h: forward, backward, backward from what was kept
-  kKernLayerNormBf161x1,
-  kKernLayerNormBackwardBf161x1,
-  kKernLayerNormBackwardKeptBf161x1,
-  kKernLayerNormBf161x2,
-  kKernLayerNormBackwardBf161x2,
-  kKernLayerNormBackwardKeptBf161x2,
-  kKernLayerNormBf164x1,
-  kKernLayerNormBackwardBf164x1,
-  kKernLayerNormBackwardKeptBf164x1,
-  kKernLayerNormBf164x2,
-  kKernLayerNormBackwardBf164x2,
-  kKernLayerNormBackwardKeptBf164x2,
-  kKernLayerNormBf168x2,
-  kKernLayerNormBackwardBf168x2,
-  kKernLayerNormBackwardKeptBf168x2,
-  kKernLayerNormBf1616x2,
-  kKernLayerNormBackwardBf1616x2,
-  kKernLayerNormBackwardKeptBf1616x2,
-  kKernLayerNormF161x1,
-  kKernLayerNormBackwardF161x1,
-  kKernLayerNormBackwardKeptF161x1,
-  kKernLayerNormF161x2,
-  kKernLayerNormBackwardF161x2,
-  kKernLayerNormBackwardKeptF161x2,
-  kKernLayerNormF164x1,
-  kKernLayerNormBackwardF164x1,
-  kKernLayerNormBackwardKeptF164x1,
-  kKernLayerNormF164x2,
-  kKernLayerNormBackwardF164x2,
-  kKernLayerNormBackwardKeptF164x2,
-  kKernLayerNormF168x2,
-  kKernLayerNormBackwardF168x2,
-  kKernLayerNormBackwardKeptF168x2,
-  kKernLayerNormF1616x2,
-  kKernLayerNormBackwardF1616x2,
-  kKernLayerNormBackwardKeptF1616x2,
-  kKernLayerNormF321x1,
-  kKernLayerNormBackwardF321x1,
-  kKernLayerNormBackwardKeptF321x1,
-  kKernLayerNormF321x2,
-  kKernLayerNormBackwardF321x2,
-  kKernLayerNormBackwardKeptF321x2,
-  kKernLayerNormF324x1,
-  kKernLayerNormBackwardF324x1,
-  kKernLayerNormBackwardKeptF324x1,
-  kKernLayerNormF324x2,
-  kKernLayerNormBackwardF324x2,
-  kKernLayerNormBackwardKeptF324x2,
-  kKernLayerNormF328x2,
-  kKernLayerNormBackwardF328x2,
-  kKernLayerNormBackwardKeptF328x2,
-  kKernLayerNormF3216x2,
-  kKernLayerNormBackwardF3216x2,
-  kKernLayerNormBackwardKeptF3216x2,
+  kKernLayerNormBf16Wave1,
+  kKernLayerNormBackwardBf16Wave1,
+  kKernLayerNormBackwardKeptBf16Wave1,
+  kKernLayerNormBf16Wave2,
+  kKernLayerNormBackwardBf16Wave2,
+  kKernLayerNormBackwardKeptBf16Wave2,
+  kKernLayerNormBf16Team1,
+  kKernLayerNormBackwardBf16Team1,
+  kKernLayerNormBackwardKeptBf16Team1,
+  kKernLayerNormBf16Team2,
+  kKernLayerNormBackwardBf16Team2,
+  kKernLayerNormBackwardKeptBf16Team2,
+  kKernLayerNormBf16Team4,
+  kKernLayerNormBackwardBf16Team4,
+  kKernLayerNormBackwardKeptBf16Team4,
+  kKernLayerNormF16Wave1,
+  kKernLayerNormBackwardF16Wave1,
+  kKernLayerNormBackwardKeptF16Wave1,
+  kKernLayerNormF16Wave2,
+  kKernLayerNormBackwardF16Wave2,
+  kKernLayerNormBackwardKeptF16Wave2,
+  kKernLayerNormF16Team1,
+  kKernLayerNormBackwardF16Team1,
+  kKernLayerNormBackwardKeptF16Team1,
+  kKernLayerNormF16Team2,
+  kKernLayerNormBackwardF16Team2,
+  kKernLayerNormBackwardKeptF16Team2,
+  kKernLayerNormF16Team4,
+  kKernLayerNormBackwardF16Team4,
+  kKernLayerNormBackwardKeptF16Team4,
+  kKernLayerNormF32Wave1,
+  kKernLayerNormBackwardF32Wave1,
+  kKernLayerNormBackwardKeptF32Wave1,
+  kKernLayerNormF32Wave2,
+  kKernLayerNormBackwardF32Wave2,
+  kKernLayerNormBackwardKeptF32Wave2,
+  kKernLayerNormF32Team1,
+  kKernLayerNormBackwardF32Team1,
+  kKernLayerNormBackwardKeptF32Team1,
+  kKernLayerNormF32Team2,
+  kKernLayerNormBackwardF32Team2,
+  kKernLayerNormBackwardKeptF32Team2,
+  kKernLayerNormF32Team4,
+  kKernLayerNormBackwardF32Team4,
+  kKernLayerNormBackwardKeptF32Team4,
   kKernLayerNormJoin,
   // activations in 8 bits and back, per type
   kKernAct8QuantizeBf16,

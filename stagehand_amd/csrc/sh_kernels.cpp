@@ -148,60 +148,51 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModQkNorm, "sh_qk_norm_backward_f32_1_kernel"},
     {kModQkNorm, "sh_qk_norm_backward_f32_1_interleaved_kernel"},
     {kModQkNorm, "sh_qk_norm_dweight_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_1x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_1x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_4x1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_4x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_8x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_16x2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_16x2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_bf16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_bf16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_wave1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_wave2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_team1_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_team2_kernel"},
+    {kModLayerNorm, "sh_layer_norm_f32_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_f32_team4_kernel"},
+    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_team4_kernel"},
     {kModLayerNorm, "sh_layer_norm_join_kernel"},
     {kModAct8, "sh_act8_quantize_bf16_kernel"},
     {kModAct8, "sh_act8_dequantize_bf16_kernel"},

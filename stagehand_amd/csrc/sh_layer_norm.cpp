@@ -71,8 +71,10 @@ sh::LayerNormKernelArgs kernel_args(const sh_layer_norm_args* a, bool backward) 
   ka.groups = a->per_batch ? a->batch : 1;
   ka.tokens = a->per_batch ? a->seq : a->batch * a->seq;
   const sh::NormShape shape = sh::kNormShapes[shape_of(a->cols)];
-  const uint32_t teams = sh::norm_teams(shape.waves);
-  const uint32_t most = kComputeUnits * (backward ? kBackwardWaves : kForwardWaves) / (shape.waves * teams);
+  const uint32_t teams = shape.team ? 1 : sh::kNormTeams, of_wave = 64 * 8 * shape.chunks;
+  const uint32_t waves = shape.team ? (a->cols + of_wave - 1) / of_wave : teams;
+  ka.threads = waves * 64;
+  const uint32_t most = kComputeUnits * std::max(1u, (backward ? kBackwardWaves : kForwardWaves) / waves);
   const uint32_t useful = (ka.tokens + teams - 1) / teams;
   ka.per_group = std::max(1u, std::min(useful, most / std::max(1u, std::min(ka.groups, most))));
   return ka;
@@ -87,14 +89,13 @@ uint64_t partial_bytes(const sh::LayerNormKernelArgs& ka) {
 
 // Three kernels for each type and shape: forward, backward, backward from what was kept.
 sh::KernelId kernel_of(const sh_layer_norm_args* a, int pass) {
-  static_assert(sh::kKernLayerNormJoin - sh::kKernLayerNormBf161x1 == 3 * sh::kNormShapeCount * 3, "one kernel per variant");
-  return (sh::KernelId)(sh::kKernLayerNormBf161x1 + ((a->dtype - SH_DTYPE_BF16) * sh::kNormShapeCount + shape_of(a->cols)) * 3 + pass);
+  static_assert(sh::kKernLayerNormJoin - sh::kKernLayerNormBf16Wave1 == 3 * sh::kNormShapeCount * 3, "one kernel per variant");
+  return (sh::KernelId)(sh::kKernLayerNormBf16Wave1 + ((a->dtype - SH_DTYPE_BF16) * sh::kNormShapeCount + shape_of(a->cols)) * 3 + pass);
 }
 
 int launch(const sh::LayerNormKernelArgs& ka, int pass, hipStream_t stream, const char* who) {
   void* list[] = {(void*)&ka};
-  return sh::launch_kernel(kernel_of(&ka.a, pass), ka.groups * ka.per_group,
-                           sh::norm_threads(sh::kNormShapes[shape_of(ka.a.cols)].waves), stream, list, who);
+  return sh::launch_kernel(kernel_of(&ka.a, pass), ka.groups * ka.per_group, ka.threads, stream, list, who);
 }
 
 }  // namespace

@@ -23,28 +23,41 @@ template <int CTRL>
 __device__ __forceinline__ float add_moved(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
-// The sum over a wavefront, in all of it: halves of 2, 4, 8 and 16 by data-parallel moves, 32 and 64 by shuffles.
+// The sum over a wavefront, in all of it: halves of 2, 4, 8 and 16 by data-parallel moves, 32 and 64 by exchanges of rows.
 __device__ __forceinline__ float wave_sum(float v) {
   v = add_moved<0xB1>(v);   // quad_perm 1,0,3,2
   v = add_moved<0x4E>(v);   // quad_perm 2,3,0,1
   v = add_moved<0x141>(v);  // row_half_mirror
   v = add_moved<0x140>(v);  // row_mirror
-  v += __shfl_xor(v, 16);
-  v += __shfl_xor(v, 32);
-  return v;
+  // Two copies of v exchange rows of 16 (then halves): each has one half of the sum everywhere. As assembly: the compiler
+  // takes both results of its builtin to be one where both arguments are.
+  float other = v;
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(other));
+  v += other;
+  other = v;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(other));
+  return v + other;
 }
 
-// Sums over a team of W wavefronts. Two sets of slots in turn: a set is written again only after the barrier of the
-// other, which everyone reaches after reading it.
-template <uint32_t W, uint32_t N>
-struct TeamSum {
-  float (*slots)[N][W];  // [2][N][W] of LDS
+constexpr uint32_t kMostWaves = sh::kNormMostWaves;
+
+// Sums over the wavefronts of a workgroup, if it is one TEAM. Two sets of slots in turn: a set is written again only
+// after the barrier of the other, which everyone reaches after reading it. Slots that no wavefront has hold zeros.
+template <bool TEAM, uint32_t N>
+struct RowSum {
+  float (*slots)[N][kMostWaves];  // [2][N][kMostWaves] of LDS
   uint32_t turn = 0;
 
+  __device__ __forceinline__ RowSum(float (*slots)[N][kMostWaves]) : slots(slots) {
+    if constexpr (TEAM) {
+      if (threadIdx.x < 2 * N * kMostWaves) (&slots[0][0][0])[threadIdx.x] = 0.0f;
+      __syncthreads();
+    }
+  }
   __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
     for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
-    if constexpr (W > 1) {
+    if constexpr (TEAM) {
       if ((threadIdx.x & 63) == 0) {
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) slots[turn][i][threadIdx.x / 64] = v[i];
@@ -54,7 +67,7 @@ struct TeamSum {
       for (uint32_t i = 0; i < N; ++i) {
         v[i] = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < W; ++w) v[i] += slots[turn][i][w];
+        for (uint32_t w = 0; w < kMostWaves; ++w) v[i] += slots[turn][i][w];
       }
       turn ^= 1;
     }
@@ -80,22 +93,23 @@ __device__ __forceinline__ void store_params(void* p, uint32_t dtype, uint64_t a
   else Values8<float>::store(static_cast<float*>(p) + at, v, count);
 }
 
-// A work-item's share of the rows: chunks of 8 values, and the team's tokens of a group.
-template <uint32_t W, uint32_t C>
+// A work-item's share of the rows: chunks of 8 values, and the tokens of a group that its team takes: the workgroup, or a
+// wavefront by itself.
+template <bool TEAM, uint32_t C>
 struct Mine {
-  static constexpr uint32_t kTeams = sh::norm_teams(W);
-  uint32_t item;               // in the team
+  uint32_t item, items;         // in the team
   uint32_t group, first, step;  // tokens first, first + step .. of the group
   uint32_t cols;
 
   __device__ __forceinline__ Mine(const sh::LayerNormKernelArgs& ka) : cols(ka.a.cols) {
-    const uint32_t team = kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * W));
-    item = threadIdx.x - team * 64 * W;
+    const uint32_t team = TEAM ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64), teams = TEAM ? 1 : sh::kNormTeams;
+    items = TEAM ? ka.threads : 64;
+    item = threadIdx.x - team * 64;
     group = blockIdx.x / ka.per_group;
-    first = (blockIdx.x - group * ka.per_group) * kTeams + team;
-    step = ka.per_group * kTeams;
+    first = (blockIdx.x - group * ka.per_group) * teams + team;
+    step = ka.per_group * teams;
   }
-  __device__ __forceinline__ uint32_t chunk(uint32_t j) const { return j * W * 64 + item; }
+  __device__ __forceinline__ uint32_t chunk(uint32_t j) const { return j * items + item; }
   __device__ __forceinline__ uint32_t col(uint32_t j) const { return chunk(j) * 8; }
   __device__ __forceinline__ uint32_t count(uint32_t j) const { return col(j) < cols ? min(cols - col(j), 8u) : 0; }
 };
@@ -111,37 +125,52 @@ struct Token {
   __device__ __forceinline__ uint64_t at(const sh_rows& r) const { return b * r.batch_stride + s * r.seq_stride; }
 };
 
-template <typename T, uint32_t W, uint32_t C>
-__device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
-  const sh_layer_norm_args& a = ka.a;
-  const Mine<W, C> m(ka);
-  __shared__ float slots[2][1][W];
-  TeamSum<W, 1> team_sum{slots};
-  const float rcols = 1.0f / (float)a.cols;
-  const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
-  float w[C][8], b[C][8];
+// The gain of a work-item's values.
+template <bool TEAM, uint32_t C>
+__device__ __forceinline__ void load_gain(const sh_layer_norm_args& a, const Mine<TEAM, C>& m, float (&w)[C][8]) {
 #pragma unroll
   for (uint32_t j = 0; j < C; ++j) {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f, b[j][i] = 0.0f;
+    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f;
     if (a.weight != nullptr) load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
-    if (a.bias != nullptr) load_params(a.bias, a.weight_dtype, m.group * a.bias_batch_stride + m.col(j), m.count(j), b[j]);
     if (a.modulate) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) w[j][i] += 1.0f;
     }
   }
+}
+
+template <typename T, bool TEAM, uint32_t C>
+__device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
+  const sh_layer_norm_args& a = ka.a;
+  const Mine<TEAM, C> m(ka);
+  __shared__ alignas(16) float slots[2][1][kMostWaves];
+  RowSum<TEAM, 1> row_sum(slots);
+  const float rcols = 1.0f / (float)a.cols;
+  const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
+  typename Values8<T>::Vec next[C];
+  auto load = [&](uint32_t t) __attribute__((always_inline)) {
+    const T* x = static_cast<const T*>(a.x.data) + Token(a, m.group, t).at(a.x);
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) next[j] = Values8<T>::load(x + m.col(j), m.count(j));
+  };
+  if (m.first < ka.tokens) load(m.first);
+  float w[C][8], b[C][8];
+  load_gain(a, m, w);
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) b[j][i] = 0.0f;
+    if (a.bias != nullptr) load_params(a.bias, a.weight_dtype, m.group * a.bias_batch_stride + m.col(j), m.count(j), b[j]);
+  }
   for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
     const Token token(a, m.group, t);
-    const T* x = static_cast<const T*>(a.x.data) + token.at(a.x);
-    T* y = static_cast<T*>(a.y.data) + token.at(a.y);
     float v[C][8], sum[1] = {0.0f};
 #pragma unroll
-    for (uint32_t j = 0; j < C; ++j) {
-      const auto raw = Values8<T>::load(x + m.col(j), m.count(j));
+    for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) v[j][i] = (float)raw[i];
-    }
+      for (uint32_t i = 0; i < 8; ++i) v[j][i] = (float)next[j][i];
+    if (t + m.step < ka.tokens) load(t + m.step);  // on its way while this row is worked on
     if (a.q != nullptr) {
 #pragma unroll
       for (uint32_t j = 0; j < C; ++j) {
@@ -156,7 +185,7 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
     for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) sum[0] += v[j][i];
-    team_sum(sum);
+    row_sum(sum);
     const float mean = sum[0] * rcols;
     sum[0] = 0.0f;
 #pragma unroll
@@ -167,8 +196,9 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
         sum[0] = __builtin_fmaf(v[j][i], v[j][i], sum[0]);
       }
     }
-    team_sum(sum);
+    row_sum(sum);
     const float r = 1.0f / __builtin_sqrtf(sum[0] * rcols + a.eps);
+    T* y = static_cast<T*>(a.y.data) + token.at(a.y);
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
       float out[8];
@@ -183,50 +213,75 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
   }
 }
 
-template <typename T, uint32_t W, uint32_t C, bool KEPT>
-__device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
-  const sh_layer_norm_args& a = ka.a;
-  const Mine<W, C> m(ka);
-  constexpr uint32_t kTeams = Mine<W, C>::kTeams;
-  __shared__ float slots[2][2][W];
-  TeamSum<W, 2> team_sum{slots};
-  const float rcols = 1.0f / (float)a.cols;
-  const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
-  float w[C][8], dw[C][8] = {}, db[C][8] = {};
+// A row of the input as it lies in memory, or as it was kept.
+template <typename T, bool TEAM, uint32_t C, bool KEPT>
+struct InputRow {
+  typename Values8<T>::Vec raw[C];
+
+  __device__ __forceinline__ void load(const sh_layer_norm_args& a, const Mine<TEAM, C>& m, const Token& token) {
+    const T* x = static_cast<const T*>(a.x.data) + token.at(a.x);
 #pragma unroll
-  for (uint32_t j = 0; j < C; ++j) {
+    for (uint32_t j = 0; j < C; ++j) raw[j] = Values8<T>::load(x + m.col(j), m.count(j));
+  }
+  __device__ __forceinline__ void values(uint32_t j, float (&v)[8]) const {
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f;
-    if (a.weight != nullptr) load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
-    if (a.modulate) {
+    for (uint32_t i = 0; i < 8; ++i) v[i] = (float)raw[j][i];
+  }
+};
+template <typename T, bool TEAM, uint32_t C>
+struct InputRow<T, TEAM, C, true> {
+  uint2 q[C];
+  uint32_t e[C];
+
+  __device__ __forceinline__ void load(const sh_layer_norm_args& a, const Mine<TEAM, C>& m, const Token& token) {
+    const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) w[j][i] += 1.0f;
+    for (uint32_t j = 0; j < C; ++j) {
+      q[j] = make_uint2(0, 0);
+      e[j] = 1;
+      if (m.chunk(j) >= row_chunks) continue;
+      const uint64_t at = token.row * row_chunks + m.chunk(j);
+      q[j] = static_cast<const uint2*>(a.q)[at];
+      e[j] = static_cast<const uint8_t*>(a.exponent)[at / 4];
     }
   }
-  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+  __device__ __forceinline__ void values(uint32_t j, float (&v)[8]) const { dequantize8(q[j], group_scale(e[j]), v); }
+};
+
+template <typename T, bool TEAM, uint32_t C, bool KEPT>
+__device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
+  const sh_layer_norm_args& a = ka.a;
+  const Mine<TEAM, C> m(ka);
+  __shared__ alignas(16) float slots[2][2][kMostWaves];
+  RowSum<TEAM, 2> row_sum(slots);
+  const float rcols = 1.0f / (float)a.cols;
+  InputRow<T, TEAM, C, KEPT> next_x;
+  typename Values8<T>::Vec next_dy[C];
+  float next_mean = 0.0f, next_r = 0.0f;
+  auto load = [&](uint32_t t) __attribute__((always_inline)) {
     const Token token(a, m.group, t);
+    next_x.load(a, m, token);
     const T* dy = static_cast<const T*>(a.dy.data) + token.at(a.dy);
-    const float mean = a.stats[2 * token.row], r = a.stats[2 * token.row + 1];
+#pragma unroll
+    for (uint32_t j = 0; j < C; ++j) next_dy[j] = Values8<T>::load(dy + m.col(j), m.count(j));  // zeros past the row add nothing below
+    next_mean = a.stats[2 * token.row];
+    next_r = a.stats[2 * token.row + 1];
+  };
+  constexpr bool kAhead = C < 4;  // longer rows' registers do not hold another row
+  if (kAhead && m.first < ka.tokens) load(m.first);
+  float w[C][8], dw[C][8] = {}, db[C][8] = {};
+  load_gain(a, m, w);
+  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+    if (!kAhead) load(t);
+    const float mean = next_mean, r = next_r;
     float n[C][8], g[C][8], sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
-      if constexpr (KEPT) {
-        if (m.chunk(j) < row_chunks) {
-          const uint64_t at = token.row * row_chunks + m.chunk(j);
-          dequantize8(static_cast<const uint2*>(a.q)[at], group_scale(static_cast<const uint8_t*>(a.exponent)[at / 4]), n[j]);
-        } else {
+      next_x.values(j, n[j]);
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) n[j][i] = 0.0f;
-        }
-      } else {
-        const auto raw = Values8<T>::load(static_cast<const T*>(a.x.data) + token.at(a.x) + m.col(j), m.count(j));
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) n[j][i] = (float)raw[i];
-      }
-      const auto raw = Values8<T>::load(dy + m.col(j), m.count(j));  // zeros past the row add nothing below
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) g[j][i] = (float)raw[i];
+      for (uint32_t i = 0; i < 8; ++i) g[j][i] = (float)next_dy[j][i];
     }
+    if (kAhead && t + m.step < ka.tokens) load(t + m.step);  // on its way while this row is worked on
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
 #pragma unroll
@@ -240,9 +295,9 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
       }
     }
     if (a.dx.data == nullptr) continue;
-    team_sum(sum);
+    row_sum(sum);
     const float mean_g = sum[0] * rcols, mean_gn = sum[1] * rcols;
-    T* dx = static_cast<T*>(a.dx.data) + token.at(a.dx);
+    T* dx = static_cast<T*>(a.dx.data) + Token(a, m.group, t).at(a.dx);
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
       float out[8];
@@ -252,21 +307,21 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
     }
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  if constexpr (kTeams > 1) {  // the teams' sums, in their order
-    __shared__ alignas(16) float part[kTeams][2][C][8][64];
-    const uint32_t team = threadIdx.x / 64;
+  if constexpr (!TEAM) {  // the wavefronts' sums, in their order
+    __shared__ float part[sh::kNormTeams][2][C][8][64];
+    const uint32_t wave = threadIdx.x / 64;
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) part[team][0][j][i][m.item] = dw[j][i], part[team][1][j][i][m.item] = db[j][i];
+      for (uint32_t i = 0; i < 8; ++i) part[wave][0][j][i][m.item] = dw[j][i], part[wave][1][j][i][m.item] = db[j][i];
     __syncthreads();
-    if (team != 0) return;
+    if (wave != 0) return;
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
 #pragma unroll
-        for (uint32_t k = 1; k < kTeams; ++k) dw[j][i] += part[k][0][j][i][m.item], db[j][i] += part[k][1][j][i][m.item];
+        for (uint32_t k = 1; k < sh::kNormTeams; ++k) dw[j][i] += part[k][0][j][i][m.item], db[j][i] += part[k][1][j][i][m.item];
       }
     }
   }
@@ -286,26 +341,26 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
 
 }  // namespace
 
-#define SH_NORM(name, T, W, C)                                                                                    \
-  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_##name##_##W##x##C##_kernel(    \
-      sh::LayerNormKernelArgs ka) {                                                                               \
-    forward<T, W, C>(ka);                                                                                         \
-  }                                                                                                               \
-  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_backward_##name##_##W##x##C##_kernel( \
-      sh::LayerNormKernelArgs ka) {                                                                               \
-    backward<T, W, C, false>(ka);                                                                                 \
-  }                                                                                                               \
-  extern "C" __global__ __launch_bounds__(sh::norm_threads(W)) void sh_layer_norm_backward_kept_##name##_##W##x##C##_kernel( \
-      sh::LayerNormKernelArgs ka) {                                                                               \
-    backward<T, W, C, true>(ka);                                                                                  \
+// The shapes of sh_layer_norm_args.h.
+#define SH_NORM(name, T, shape, TEAM, C)                                                                                      \
+  extern "C" __global__ __launch_bounds__(sh::norm_most_threads(TEAM)) void sh_layer_norm_##name##_##shape##_kernel(          \
+      sh::LayerNormKernelArgs ka) {                                                                                           \
+    forward<T, TEAM, C>(ka);                                                                                                  \
+  }                                                                                                                           \
+  extern "C" __global__ __launch_bounds__(sh::norm_most_threads(TEAM)) void sh_layer_norm_backward_##name##_##shape##_kernel( \
+      sh::LayerNormKernelArgs ka) {                                                                                           \
+    backward<T, TEAM, C, false>(ka);                                                                                          \
+  }                                                                                                                           \
+  extern "C" __global__ __launch_bounds__(sh::norm_most_threads(TEAM)) void sh_layer_norm_backward_kept_##name##_##shape##_kernel( \
+      sh::LayerNormKernelArgs ka) {                                                                                           \
+    backward<T, TEAM, C, true>(ka);                                                                                           \
   }
-#define SH_NORM_SHAPES(name, T) \
-  SH_NORM(name, T, 1, 1)        \
-  SH_NORM(name, T, 1, 2)        \
-  SH_NORM(name, T, 4, 1)        \
-  SH_NORM(name, T, 4, 2)        \
-  SH_NORM(name, T, 8, 2)        \
-  SH_NORM(name, T, 16, 2)
+#define SH_NORM_SHAPES(name, T)          \
+  SH_NORM(name, T, wave1, false, 1)      \
+  SH_NORM(name, T, wave2, false, 2)      \
+  SH_NORM(name, T, team1, true, 1)       \
+  SH_NORM(name, T, team2, true, 2)       \
+  SH_NORM(name, T, team4, true, 4)
 SH_NORM_SHAPES(bf16, __bf16)
 SH_NORM_SHAPES(f16, _Float16)
 SH_NORM_SHAPES(f32, float)

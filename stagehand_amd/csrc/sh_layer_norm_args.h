@@ -14,17 +14,20 @@ struct LayerNormKernelArgs {
   uint32_t groups;    // of tokens that share weight and bias
   uint32_t tokens;    // of a group
   uint32_t per_group;  // workgroups
+  uint32_t threads;    // of a workgroup
 };
 
-// Rows are held by teams of wavefronts, 8 values a work-item and chunk.
+// A row is held by a wavefront, kNormTeams of them in a workgroup, or by a workgroup of up to kNormMostWaves; `chunks` times
+// 8 values a work-item.
 struct NormShape {
-  uint32_t waves, chunks;
+  bool team;
+  uint32_t chunks;
 };
-constexpr NormShape kNormShapes[] = {{1, 1}, {1, 2}, {4, 1}, {4, 2}, {8, 2}, {16, 2}};
+constexpr NormShape kNormShapes[] = {{false, 1}, {false, 2}, {true, 1}, {true, 2}, {true, 4}};
 constexpr int kNormShapeCount = sizeof(kNormShapes) / sizeof(kNormShapes[0]);
-constexpr uint32_t norm_capacity(NormShape s) { return s.waves * 64 * 8 * s.chunks; }
-constexpr uint32_t norm_teams(uint32_t waves) { return waves == 1 ? 4 : 1; }  // of a workgroup
-constexpr uint32_t norm_threads(uint32_t waves) { return waves * norm_teams(waves) * 64; }
+constexpr uint32_t kNormTeams = 4, kNormMostWaves = 8;
+constexpr uint32_t norm_capacity(NormShape s) { return (s.team ? kNormMostWaves : 1) * 64 * 8 * s.chunks; }
+constexpr uint32_t norm_most_threads(bool team) { return 64 * (team ? kNormMostWaves : kNormTeams); }
 static_assert(norm_capacity(kNormShapes[kNormShapeCount - 1]) == SH_LAYER_NORM_MAX_COLS, "the last shape holds the longest rows");
 
 constexpr uint32_t kNormJoinThreads = 1024, kNormJoinCols = 32;
