@@ -180,9 +180,6 @@ enum KernelId : int {
   kKernLayerNormBf16Wave2,
   kKernLayerNormBackwardBf16Wave2,
   kKernLayerNormBackwardKeptBf16Wave2,
-  kKernLayerNormBf16Team1,
-  kKernLayerNormBackwardBf16Team1,
-  kKernLayerNormBackwardKeptBf16Team1,
   kKernLayerNormBf16Team2,
   kKernLayerNormBackwardBf16Team2,
   kKernLayerNormBackwardKeptBf16Team2,
@@ -195,9 +192,6 @@ enum KernelId : int {
   kKernLayerNormF16Wave2,
   kKernLayerNormBackwardF16Wave2,
   kKernLayerNormBackwardKeptF16Wave2,
-  kKernLayerNormF16Team1,
-  kKernLayerNormBackwardF16Team1,
-  kKernLayerNormBackwardKeptF16Team1,
   kKernLayerNormF16Team2,
   kKernLayerNormBackwardF16Team2,
   kKernLayerNormBackwardKeptF16Team2,
@@ -210,9 +204,6 @@ enum KernelId : int {
   kKernLayerNormF32Wave2,
   kKernLayerNormBackwardF32Wave2,
   kKernLayerNormBackwardKeptF32Wave2,
-  kKernLayerNormF32Team1,
-  kKernLayerNormBackwardF32Team1,
-  kKernLayerNormBackwardKeptF32Team1,
   kKernLayerNormF32Team2,
   kKernLayerNormBackwardF32Team2,
   kKernLayerNormBackwardKeptF32Team2,

@@ -154,9 +154,6 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModLayerNorm, "sh_layer_norm_bf16_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_bf16_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_wave2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_bf16_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_bf16_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_team1_kernel"},
     {kModLayerNorm, "sh_layer_norm_bf16_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_bf16_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_bf16_team2_kernel"},
@@ -169,9 +166,6 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModLayerNorm, "sh_layer_norm_f16_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_f16_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_f16_wave2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f16_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f16_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f16_team1_kernel"},
     {kModLayerNorm, "sh_layer_norm_f16_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_f16_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_f16_team2_kernel"},
@@ -184,9 +178,6 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModLayerNorm, "sh_layer_norm_f32_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_f32_wave2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_f32_wave2_kernel"},
-    {kModLayerNorm, "sh_layer_norm_f32_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_f32_team1_kernel"},
-    {kModLayerNorm, "sh_layer_norm_backward_kept_f32_team1_kernel"},
     {kModLayerNorm, "sh_layer_norm_f32_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_f32_team2_kernel"},
     {kModLayerNorm, "sh_layer_norm_backward_kept_f32_team2_kernel"},

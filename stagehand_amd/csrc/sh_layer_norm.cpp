@@ -55,9 +55,6 @@ int check(const sh_layer_norm_args* a, bool backward, const char* who) {
 }
 
 constexpr uint32_t kComputeUnits = 256;
-// Wavefronts at most, a compute unit: what runs at a time, so that a workgroup loads the weights once and, in the
-// backward pass, leaves one set of sums for many tokens.
-constexpr uint32_t kForwardWaves = 32, kBackwardWaves = 16;
 
 int shape_of(uint32_t cols) {
   int i = 0;
@@ -71,12 +68,26 @@ sh::LayerNormKernelArgs kernel_args(const sh_layer_norm_args* a, bool backward) 
   ka.groups = a->per_batch ? a->batch : 1;
   ka.tokens = a->per_batch ? a->seq : a->batch * a->seq;
   const sh::NormShape shape = sh::kNormShapes[shape_of(a->cols)];
-  const uint32_t teams = shape.team ? 1 : sh::kNormTeams, of_wave = 64 * 8 * shape.chunks;
-  const uint32_t waves = shape.team ? (a->cols + of_wave - 1) / of_wave : teams;
-  ka.threads = waves * 64;
-  const uint32_t most = kComputeUnits * std::max(1u, (backward ? kBackwardWaves : kForwardWaves) / waves);
+  const uint32_t chunks = (a->cols + 7) / 8;
+  uint32_t teams = 1;  // of a workgroup
+  if (shape.team) {
+    ka.lanes = (chunks + 64 * shape.chunks - 1) / (64 * shape.chunks) * 64;
+  } else {
+    for (ka.lanes = 4; ka.lanes < 64 && ka.lanes < chunks;) ka.lanes *= 2;
+    teams = sh::kNormThreads / ka.lanes;
+  }
+  const uint32_t threads = shape.team ? ka.lanes : sh::kNormThreads, groups = std::max(1u, ka.groups);
   const uint32_t useful = (ka.tokens + teams - 1) / teams;
-  ka.per_group = std::max(1u, std::min(useful, most / std::max(1u, std::min(ka.groups, most))));
+  uint32_t per_group;
+  if (!backward) {
+    per_group = kComputeUnits * ((shape.chunks == 1 ? 1536 : 1024) / threads) / groups;
+  } else {
+    // Every workgroup leaves a set of sums, that is written and read once more: 16 MB of them at most, and no team has fewer
+    // than three tokens.
+    const uint32_t fit = (16u << 20) / (8 * a->cols) / kComputeUnits;
+    per_group = std::min(kComputeUnits * (shape.team ? std::min(std::max(fit, 1u), 4u) : 3) / groups, (useful + 2) / 3);
+  }
+  ka.per_group = std::max(1u, std::min(per_group, useful));
   return ka;
 }
 
@@ -95,7 +106,8 @@ sh::KernelId kernel_of(const sh_layer_norm_args* a, int pass) {
 
 int launch(const sh::LayerNormKernelArgs& ka, int pass, hipStream_t stream, const char* who) {
   void* list[] = {(void*)&ka};
-  return sh::launch_kernel(kernel_of(&ka.a, pass), ka.groups * ka.per_group, ka.threads, stream, list, who);
+  return sh::launch_kernel(kernel_of(&ka.a, pass), ka.groups * ka.per_group,
+                           sh::kNormShapes[shape_of(ka.a.cols)].team ? ka.lanes : sh::kNormThreads, stream, list, who);
 }
 
 }  // namespace

@@ -23,40 +23,46 @@ template <int CTRL>
 __device__ __forceinline__ float add_moved(float v) {
   return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
-// The sum over a wavefront, in all of it: halves of 2, 4, 8 and 16 by data-parallel moves, 32 and 64 by exchanges of rows.
-__device__ __forceinline__ float wave_sum(float v) {
-  v = add_moved<0xB1>(v);   // quad_perm 1,0,3,2
-  v = add_moved<0x4E>(v);   // quad_perm 2,3,0,1
-  v = add_moved<0x141>(v);  // row_half_mirror
-  v = add_moved<0x140>(v);  // row_mirror
-  // Two copies of v exchange rows of 16 (then halves): each has one half of the sum everywhere. As assembly: the compiler
-  // takes both results of its builtin to be one where both arguments are.
-  float other = v;
-  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(other));
-  v += other;
-  other = v;
-  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(other));
-  return v + other;
+// The sum over groups of `lanes` (a power of two from 4 on) neighbouring work-items, in all of them: halves of 2, 4, 8 and
+// 16 by data-parallel moves (each adds a half that already agrees), 32 and 64 by exchanges: two copies of v exchange rows
+// of 16 (then halves), so that each has one half of the sum everywhere. These are assembly: the compiler takes both
+// results of its builtin to be one where both arguments are.
+__device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
+  v = add_moved<0xB1>(v);                    // quad_perm 1,0,3,2
+  v = add_moved<0x4E>(v);                    // quad_perm 2,3,0,1
+  if (lanes >= 8) v = add_moved<0x141>(v);   // row_half_mirror
+  if (lanes >= 16) v = add_moved<0x140>(v);  // row_mirror
+  if (lanes >= 32) {
+    float other = v;
+    asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(other));
+    v += other;
+  }
+  if (lanes >= 64) {
+    float other = v;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(other));
+    v += other;
+  }
+  return v;
 }
 
 constexpr uint32_t kMostWaves = sh::kNormMostWaves;
 
-// Sums over the wavefronts of a workgroup, if it is one TEAM. Two sets of slots in turn: a set is written again only
-// after the barrier of the other, which everyone reaches after reading it. Slots that no wavefront has hold zeros.
+// Sums over a team, in all of it: the workgroup if TEAM, else groups of `lanes` work-items. Two sets of slots in turn: a
+// set is written again only after the barrier of the other, which everyone reaches after reading it. Slots that no
+// wavefront has hold zeros.
 template <bool TEAM, uint32_t N>
-struct RowSum {
+struct TeamSum {
   float (*slots)[N][kMostWaves];  // [2][N][kMostWaves] of LDS
-  uint32_t turn = 0;
+  uint32_t lanes, turn = 0;
 
-  __device__ __forceinline__ RowSum(float (*slots)[N][kMostWaves]) : slots(slots) {
-    if constexpr (TEAM) {
-      if (threadIdx.x < 2 * N * kMostWaves) (&slots[0][0][0])[threadIdx.x] = 0.0f;
-      __syncthreads();
+  __device__ __forceinline__ TeamSum(float (*slots)[N][kMostWaves], uint32_t lanes) : slots(slots), lanes(lanes) {
+    if constexpr (TEAM) {  // by the wavefront that is before the first barrier with the others
+      if (threadIdx.x < 2 * N * kMostWaves && threadIdx.x % kMostWaves >= blockDim.x / 64) (&slots[0][0][0])[threadIdx.x] = 0.0f;
     }
   }
   __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    for (uint32_t i = 0; i < N; ++i) v[i] = group_sum(v[i], TEAM ? 64 : lanes);
     if constexpr (TEAM) {
       if ((threadIdx.x & 63) == 0) {
 #pragma unroll
@@ -74,11 +80,11 @@ struct RowSum {
   }
 };
 
-// 8 values of a weight or bias at p, 0 behind `count`.
+// 8 values of a weight or bias at p; 0 behind `count` and without one.
 __device__ __forceinline__ void load_params(const void* p, uint32_t dtype, uint64_t at, uint32_t count, float (&v)[8]) {
   auto values = [&](auto zero) {
     using T = decltype(zero);
-    const auto raw = Values8<T>::load(static_cast<const T*>(p) + at, count);
+    const auto raw = Values8<T>::load(static_cast<const T*>(p) + at, p != nullptr ? count : 0);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) v[i] = (float)raw[i];
   };
@@ -87,27 +93,33 @@ __device__ __forceinline__ void load_params(const void* p, uint32_t dtype, uint6
   else values(float{});
 }
 
+// A weight as a gain: 1 without one.
+__device__ __forceinline__ void as_gain(const sh_layer_norm_args& a, float (&w)[8]) {
+  if (!a.modulate && a.weight != nullptr) return;
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) w[i] += 1.0f;
+}
+
 __device__ __forceinline__ void store_params(void* p, uint32_t dtype, uint64_t at, uint32_t count, const float (&v)[8]) {
   if (dtype == SH_DTYPE_BF16) Values8<__bf16>::store(static_cast<__bf16*>(p) + at, v, count);
   else if (dtype == SH_DTYPE_F16) Values8<_Float16>::store(static_cast<_Float16*>(p) + at, v, count);
   else Values8<float>::store(static_cast<float*>(p) + at, v, count);
 }
 
-// A work-item's share of the rows: chunks of 8 values, and the tokens of a group that its team takes: the workgroup, or a
-// wavefront by itself.
+// A work-item's share of the rows: chunks of 8 values, and the tokens of a group that its team takes.
 template <bool TEAM, uint32_t C>
 struct Mine {
-  uint32_t item, items;         // in the team
-  uint32_t group, first, step;  // tokens first, first + step .. of the group
+  uint32_t item, items;  // in the team
+  uint32_t group, team, teams;  // of the group
   uint32_t cols;
 
   __device__ __forceinline__ Mine(const sh::LayerNormKernelArgs& ka) : cols(ka.a.cols) {
-    const uint32_t team = TEAM ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64), teams = TEAM ? 1 : sh::kNormTeams;
-    items = TEAM ? ka.threads : 64;
-    item = threadIdx.x - team * 64;
+    items = ka.lanes;
+    item = TEAM ? threadIdx.x : threadIdx.x & (items - 1);
     group = blockIdx.x / ka.per_group;
-    first = (blockIdx.x - group * ka.per_group) * teams + team;
-    step = ka.per_group * teams;
+    const uint32_t block = blockIdx.x - group * ka.per_group, of_block = TEAM ? 1 : sh::kNormThreads / items;
+    team = block * of_block + (TEAM ? 0 : threadIdx.x / items);
+    teams = ka.per_group * of_block;
   }
   __device__ __forceinline__ uint32_t chunk(uint32_t j) const { return j * items + item; }
   __device__ __forceinline__ uint32_t col(uint32_t j) const { return chunk(j) * 8; }
@@ -118,34 +130,19 @@ struct Token {
   uint64_t b, s, row;
 
   __device__ __forceinline__ Token(const sh_layer_norm_args& a, uint32_t group, uint32_t t) {
-    if (a.per_batch) b = group, s = t;
+    if (a.per_batch || a.batch == 1) b = group, s = t;
     else b = t / a.seq, s = t - (uint32_t)b * a.seq;
     row = b * a.seq + s;
   }
   __device__ __forceinline__ uint64_t at(const sh_rows& r) const { return b * r.batch_stride + s * r.seq_stride; }
 };
 
-// The gain of a work-item's values.
-template <bool TEAM, uint32_t C>
-__device__ __forceinline__ void load_gain(const sh_layer_norm_args& a, const Mine<TEAM, C>& m, float (&w)[C][8]) {
-#pragma unroll
-  for (uint32_t j = 0; j < C; ++j) {
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) w[j][i] = a.modulate ? 0.0f : 1.0f;
-    if (a.weight != nullptr) load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
-    if (a.modulate) {
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) w[j][i] += 1.0f;
-    }
-  }
-}
-
 template <typename T, bool TEAM, uint32_t C>
 __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
   const sh_layer_norm_args& a = ka.a;
   const Mine<TEAM, C> m(ka);
   __shared__ alignas(16) float slots[2][1][kMostWaves];
-  RowSum<TEAM, 1> row_sum(slots);
+  TeamSum<TEAM, 1> team_sum(slots, ka.lanes);
   const float rcols = 1.0f / (float)a.cols;
   const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
   typename Values8<T>::Vec next[C];
@@ -154,23 +151,22 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) next[j] = Values8<T>::load(x + m.col(j), m.count(j));
   };
-  if (m.first < ka.tokens) load(m.first);
+  if (m.team < ka.tokens) load(m.team);
   float w[C][8], b[C][8];
-  load_gain(a, m, w);
 #pragma unroll
   for (uint32_t j = 0; j < C; ++j) {
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) b[j][i] = 0.0f;
-    if (a.bias != nullptr) load_params(a.bias, a.weight_dtype, m.group * a.bias_batch_stride + m.col(j), m.count(j), b[j]);
+    load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
+    load_params(a.bias, a.weight_dtype, m.group * a.bias_batch_stride + m.col(j), m.count(j), b[j]);
+    as_gain(a, w[j]);
   }
-  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+  for (uint32_t t = m.team; t < ka.tokens; t += m.teams) {
     const Token token(a, m.group, t);
     float v[C][8], sum[1] = {0.0f};
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) v[j][i] = (float)next[j][i];
-    if (t + m.step < ka.tokens) load(t + m.step);  // on its way while this row is worked on
+    if (t + m.teams < ka.tokens) load(t + m.teams);  // on its way while this row is worked on
     if (a.q != nullptr) {
 #pragma unroll
       for (uint32_t j = 0; j < C; ++j) {
@@ -185,7 +181,7 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
     for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) sum[0] += v[j][i];
-    row_sum(sum);
+    team_sum(sum);
     const float mean = sum[0] * rcols;
     sum[0] = 0.0f;
 #pragma unroll
@@ -196,7 +192,7 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
         sum[0] = __builtin_fmaf(v[j][i], v[j][i], sum[0]);
       }
     }
-    row_sum(sum);
+    team_sum(sum);
     const float r = 1.0f / __builtin_sqrtf(sum[0] * rcols + a.eps);
     T* y = static_cast<T*>(a.y.data) + token.at(a.y);
 #pragma unroll
@@ -253,7 +249,7 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
   const sh_layer_norm_args& a = ka.a;
   const Mine<TEAM, C> m(ka);
   __shared__ alignas(16) float slots[2][2][kMostWaves];
-  RowSum<TEAM, 2> row_sum(slots);
+  TeamSum<TEAM, 2> team_sum(slots, ka.lanes);
   const float rcols = 1.0f / (float)a.cols;
   InputRow<T, TEAM, C, KEPT> next_x;
   typename Values8<T>::Vec next_dy[C];
@@ -268,10 +264,14 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
     next_r = a.stats[2 * token.row + 1];
   };
   constexpr bool kAhead = C < 4;  // longer rows' registers do not hold another row
-  if (kAhead && m.first < ka.tokens) load(m.first);
+  if (kAhead && m.team < ka.tokens) load(m.team);
   float w[C][8], dw[C][8] = {}, db[C][8] = {};
-  load_gain(a, m, w);
-  for (uint32_t t = m.first; t < ka.tokens; t += m.step) {
+#pragma unroll
+  for (uint32_t j = 0; j < C; ++j) {
+    load_params(a.weight, a.weight_dtype, m.group * a.weight_batch_stride + m.col(j), m.count(j), w[j]);
+    as_gain(a, w[j]);
+  }
+  for (uint32_t t = m.team; t < ka.tokens; t += m.teams) {
     if (!kAhead) load(t);
     const float mean = next_mean, r = next_r;
     float n[C][8], g[C][8], sum[2] = {0.0f, 0.0f};
@@ -281,7 +281,7 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) g[j][i] = (float)next_dy[j][i];
     }
-    if (kAhead && t + m.step < ka.tokens) load(t + m.step);  // on its way while this row is worked on
+    if (kAhead && t + m.teams < ka.tokens) load(t + m.teams);  // on its way while this row is worked on
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
 #pragma unroll
@@ -295,7 +295,7 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
       }
     }
     if (a.dx.data == nullptr) continue;
-    row_sum(sum);
+    team_sum(sum);
     const float mean_g = sum[0] * rcols, mean_gn = sum[1] * rcols;
     T* dx = static_cast<T*>(a.dx.data) + Token(a, m.group, t).at(a.dx);
 #pragma unroll
@@ -307,22 +307,20 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
     }
   }
   if (a.dweight == nullptr && a.dbias == nullptr) return;
-  if constexpr (!TEAM) {  // the wavefronts' sums, in their order
-    __shared__ float part[sh::kNormTeams][2][C][8][64];
-    const uint32_t wave = threadIdx.x / 64;
+  if constexpr (!TEAM) {  // the teams' sums, in their order
+    constexpr uint32_t kThreads = sh::kNormThreads;
+    __shared__ float part[2][C][8][kThreads];
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) part[wave][0][j][i][m.item] = dw[j][i], part[wave][1][j][i][m.item] = db[j][i];
+      for (uint32_t i = 0; i < 8; ++i) part[0][j][i][threadIdx.x] = dw[j][i], part[1][j][i][threadIdx.x] = db[j][i];
     __syncthreads();
-    if (wave != 0) return;
+    if (threadIdx.x >= m.items) return;
+    for (uint32_t k = threadIdx.x + m.items; k < kThreads; k += m.items) {
 #pragma unroll
-    for (uint32_t j = 0; j < C; ++j) {
+      for (uint32_t j = 0; j < C; ++j)
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) {
-#pragma unroll
-        for (uint32_t k = 1; k < sh::kNormTeams; ++k) dw[j][i] += part[k][0][j][i][m.item], db[j][i] += part[k][1][j][i][m.item];
-      }
+        for (uint32_t i = 0; i < 8; ++i) dw[j][i] += part[0][j][i][k], db[j][i] += part[1][j][i][k];
     }
   }
 #pragma unroll
@@ -358,7 +356,6 @@ __device__ __forceinline__ void backward(const sh::LayerNormKernelArgs& ka) {
 #define SH_NORM_SHAPES(name, T)          \
   SH_NORM(name, T, wave1, false, 1)      \
   SH_NORM(name, T, wave2, false, 2)      \
-  SH_NORM(name, T, team1, true, 1)       \
   SH_NORM(name, T, team2, true, 2)       \
   SH_NORM(name, T, team4, true, 4)
 SH_NORM_SHAPES(bf16, __bf16)

@@ -14,20 +14,20 @@ struct LayerNormKernelArgs {
   uint32_t groups;    // of tokens that share weight and bias
   uint32_t tokens;    // of a group
   uint32_t per_group;  // workgroups
-  uint32_t threads;    // of a workgroup
+  uint32_t lanes;      // work-items that share a row: the workgroup's, or a power of two of them from 4 to 64
 };
 
-// A row is held by a wavefront, kNormTeams of them in a workgroup, or by a workgroup of up to kNormMostWaves; `chunks` times
-// 8 values a work-item.
+// A row is held by up to 64 work-items of a workgroup of kNormThreads, or by a `team`: a workgroup of up to kNormMostWaves
+// wavefronts; `chunks` times 8 values a work-item.
 struct NormShape {
   bool team;
   uint32_t chunks;
 };
-constexpr NormShape kNormShapes[] = {{false, 1}, {false, 2}, {true, 1}, {true, 2}, {true, 4}};
+constexpr NormShape kNormShapes[] = {{false, 1}, {false, 2}, {true, 2}, {true, 4}};
 constexpr int kNormShapeCount = sizeof(kNormShapes) / sizeof(kNormShapes[0]);
-constexpr uint32_t kNormTeams = 4, kNormMostWaves = 8;
+constexpr uint32_t kNormThreads = 256, kNormMostWaves = 8;
 constexpr uint32_t norm_capacity(NormShape s) { return (s.team ? kNormMostWaves : 1) * 64 * 8 * s.chunks; }
-constexpr uint32_t norm_most_threads(bool team) { return 64 * (team ? kNormMostWaves : kNormTeams); }
+constexpr uint32_t norm_most_threads(bool team) { return team ? 64 * kNormMostWaves : kNormThreads; }
 static_assert(norm_capacity(kNormShapes[kNormShapeCount - 1]) == SH_LAYER_NORM_MAX_COLS, "the last shape holds the longest rows");
 
 constexpr uint32_t kNormJoinThreads = 1024, kNormJoinCols = 32;
