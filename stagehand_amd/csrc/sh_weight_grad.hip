@@ -213,14 +213,17 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   // of the product then has 16 consecutive inputs.
   static_assert(kQRows % 16 == 0 || NX == 1, "a work-item's rows have one swizzle");
   const uint32_t x_place = q_t * TI + ((q_i / 64) ^ swizzle<TI>(q_t)) * 16 + q_i % 64 / 4;
-  auto put_x = [&](const Staged& v, short* stage, uint32_t j, uint32_t f) __attribute__((always_inline)) {
+  // In two steps, as their instructions hide behind products of different halves of a stage.
+  Out4 packed[NX][4];
+  auto convert_x = [&](const Staged& v, uint32_t j, uint32_t f) __attribute__((always_inline)) {
     const uint32_t words[4] = {v.q[j].x, v.q[j].y, v.q[j].z, v.q[j].w};
     float x[4];
     dequantize4(words[f], group_scale(v.e[j]), x);
-    Out4 out;
 #pragma unroll
-    for (uint32_t m = 0; m < 4; ++m) out[m] = (E)x[m];
-    *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = out;
+    for (uint32_t m = 0; m < 4; ++m) packed[j][f][m] = (E)x[m];
+  };
+  auto put_x = [&](short* stage, uint32_t j, uint32_t f) __attribute__((always_inline)) {
+    *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = packed[j][f];
   };
   static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
   const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
@@ -251,7 +254,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
       if constexpr (B < kHalf) {
         each<(B + 1) * kWrites / kHalf, B * kWrites / kHalf>([&](auto w) __attribute__((always_inline)) {
           constexpr uint32_t I = decltype(w)::value;
-          if constexpr (I < NX * 4) put_x(staged[V ^ 1], next, I / 4, I % 4);
+          if constexpr (I < NX * 4) put_x(next, I / 4, I % 4);
           else put_dy(staged[V ^ 1], next, I - NX * 4);
         });
         if constexpr (B == kHalf - 1) load(staged[V ^ 1]);
@@ -265,6 +268,8 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
       if constexpr (B >= NB / 2) {
         constexpr uint32_t kFrom = (B - NB / 2) * FI / (NB - NB / 2), kTo = (B - NB / 2 + 1) * FI / (NB - NB / 2);
         each<kTo, kFrom>([&](auto j) __attribute__((always_inline)) { x[V ^ 1][decltype(j)::value] = read_x(next, decltype(j)::value); });
+        constexpr uint32_t kFirst = (B - NB / 2) * NX * 4 / (NB - NB / 2), kLast = (B - NB / 2 + 1) * NX * 4 / (NB - NB / 2);
+        each<kLast, kFirst>([&](auto c) __attribute__((always_inline)) { convert_x(staged[V], decltype(c)::value / 4, decltype(c)::value % 4); });
       }
       if constexpr (B + kAhead >= NB) d[B + kAhead] = read_dy(next, B + kAhead - NB);
       each<FI>([&](auto j) __attribute__((always_inline)) {
@@ -285,10 +290,15 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   };
   load(staged[0]);
   add_bias(staged[0]);
-  each<NX * 4>([&](auto i) __attribute__((always_inline)) { put_x(staged[0], lds, decltype(i)::value / 4, decltype(i)::value % 4); });
+  auto convert_all = [&](const Staged& v) __attribute__((always_inline)) {
+    each<NX * 4>([&](auto i) __attribute__((always_inline)) { convert_x(v, decltype(i)::value / 4, decltype(i)::value % 4); });
+  };
+  convert_all(staged[0]);
+  each<NX * 4>([&](auto i) __attribute__((always_inline)) { put_x(lds, decltype(i)::value / 4, decltype(i)::value % 4); });
   each<ND>([&](auto j) __attribute__((always_inline)) { put_dy(staged[0], lds, decltype(j)::value); });
   load(staged[1]);
   load(staged[0]);
+  convert_all(staged[1]);
   __syncthreads();
 #pragma unroll
   for (uint32_t j = 0; j < FI; ++j) x[0][j] = read_x(lds, j);
