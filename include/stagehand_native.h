@@ -836,6 +836,7 @@ int sh_qk_norm_rope_backward(const sh_qk_norm_rope_args* args, void* workspace, 
  * = cols / SH_ACT8_GROUP, rounded up; exponent tokens * groups bytes. */
 #define SH_ACT8_GROUP 32u
 #define SH_ACT8_MAX_COLS 0x00FFFFFFu
+#define SH_WEIGHT_GRAD_MAX_OUT 0x003FFFFFu
 typedef struct sh_act8 {
   void* q;
   void* exponent;
@@ -849,7 +850,8 @@ int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype, uint64_t 
 /* The gradients of a Linear's weight and bias from its kept input:
  *   dweight[o][i] = sum_t dy[t][o] kept[t][i],  dbias[o] = sum_t dy[t][o]
  * over the kept tokens, summed in fp32 in a fixed order and rounded once to
- * out_dtype. dy is tokens x out_features in `dtype` (rows dy_ld elements apart), the type that
+ * out_dtype. dy is tokens x out_features in `dtype` (rows dy_ld elements apart,
+ * out_features and dy_ld at most SH_WEIGHT_GRAD_MAX_OUT), the type that
  * the kept activation had: values kept of bf16 or fp32 need not be fp16 numbers. fp32 gradients are multiplied with
  * all their bits. dbias may be NULL. The workspace (16-byte aligned device
  * memory, in use until the call's kernels have run) holds at least

@@ -24,6 +24,7 @@ allocated on that stream. There is no CPU path.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from typing import Any, Callable, NamedTuple
 
@@ -39,6 +40,7 @@ __all__ = ["Activation8", "quantize_activation", "weight_grad_act8", "linear_act
 
 GROUP = 32  # SH_ACT8_GROUP
 MAX_COLS = 0x00FFFFFF  # SH_ACT8_MAX_COLS
+MAX_OUT = 0x003FFFFF  # SH_WEIGHT_GRAD_MAX_OUT
 
 _KEPT = struct.Struct("<2Q2I")  # mirror of `struct sh_act8`
 
@@ -66,30 +68,36 @@ class Activation8(NamedTuple):
             dtype = self.dtype if out is None else out.dtype
         if dtype not in DTYPE_CODES:
             raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-        args = _kept_args(self)
-        with torch.cuda.device(self.q.device):
+        args, index = _kept_args(self)
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                return self.dequantize(dtype, out)
+        if out is None:
+            y, ld = self.q.new_empty((*self.shape, self.features), dtype=dtype), self.features
+        else:
             y, ld = _output(out, (*self.shape, self.features), dtype, self.q.device)
-            _native.call("sh_act8_dequantize", args, y.data_ptr(), DTYPE_CODES[dtype], ld, current_stream_handle())
+        _native.check(_native.lib().sh_act8_dequantize(args, y.data_ptr(), DTYPE_CODES[dtype], ld, current_stream_handle()))
         if out is not None:
             increment_version(out)
         return y
 
 
-def _kept_args(kept: Activation8) -> bytes:
-    """``struct sh_act8``, after a look at what the tuple holds."""
+def _kept_args(kept: Activation8) -> tuple[bytes, int]:
+    """(``struct sh_act8``, the device's index), after a look at what the tuple holds."""
     q, exponent, features, shape, dtype = kept
     if not 1 <= features <= MAX_COLS:
         raise ValueError(f"a token must have 1 .. {MAX_COLS} features, got {features}")
-    groups, tokens = -(-features // GROUP), torch.Size(shape).numel()
+    groups, tokens = -(-features // GROUP), math.prod(shape)
+    index = q.get_device()
+    if index < 0 or exponent.get_device() != index:
+        raise ValueError(f"kept.q and kept.exponent must be on one device, got {q.device} and {exponent.device}")
     if q.dtype != torch.int8 or exponent.dtype != torch.uint8 or q.shape != (tokens, groups * GROUP) or \
             exponent.shape != (tokens, groups) or not q.is_contiguous() or not exponent.is_contiguous():
         raise ValueError(f"kept must hold contiguous int8 {(tokens, groups * GROUP)} and uint8 {(tokens, groups)}, got {q.dtype} "
                          f"{tuple(q.shape)} and {exponent.dtype} {tuple(exponent.shape)}")
     if dtype not in DTYPE_CODES:
         raise ValueError(f"kept.dtype must be bfloat16, float16 or float32, got {dtype}")
-    check_device(q, None, "kept.q")
-    check_device(exponent, q.device, "kept.exponent")
-    return _KEPT.pack(q.data_ptr(), exponent.data_ptr(), tokens, features)
+    return _KEPT.pack(q.data_ptr(), exponent.data_ptr(), tokens, features), index
 
 
 def quantize_activation(x: torch.Tensor, stream: torch.cuda.Stream | int | None = None) -> Activation8:
@@ -105,18 +113,22 @@ def quantize_activation(x: torch.Tensor, stream: torch.cuda.Stream | int | None 
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("quantize_activation has no gradient: call it under torch.no_grad(), or on x.detach()")
     check_no_tangent("quantize_activation", x)
-    check_device(x, None, "x")
+    index, shape = x.get_device(), x.shape
+    if index < 0:
+        raise ValueError(f"x must be a device tensor, got {x.device}")
     rows, tokens, ld = _token_rows(x, "x")
     features = rows.shape[1]
     if not 1 <= features <= MAX_COLS:
         raise ValueError(f"a token must have 1 .. {MAX_COLS} features, got {features}")
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return quantize_activation(x)
     groups = -(-features // GROUP)
-    with torch.cuda.device(x.device):
-        q = torch.empty((tokens, groups * GROUP), dtype=torch.int8, device=x.device)
-        exponent = torch.empty((tokens, groups), dtype=torch.uint8, device=x.device)
-        kept = _KEPT.pack(q.data_ptr(), exponent.data_ptr(), tokens, features)
-        _native.call("sh_act8_quantize", rows.data_ptr(), code, ld, kept, current_stream_handle())
-    return Activation8(q, exponent, features, x.shape[:-1], x.dtype)
+    q = x.new_empty((tokens, groups * GROUP), dtype=torch.int8)
+    exponent = x.new_empty((tokens, groups), dtype=torch.uint8)
+    kept = _KEPT.pack(q.data_ptr(), exponent.data_ptr(), tokens, features)
+    _native.check(_native.lib().sh_act8_quantize(rows.data_ptr(), code, ld, kept, current_stream_handle()))
+    return Activation8(q, exponent, features, shape[:-1], x.dtype)
 
 
 def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False, out_dtype: torch.dtype | None = None,
@@ -129,10 +141,10 @@ def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False,
     if stream is not None:
         with on_stream(stream, kept.q):
             return weight_grad_act8(dy, kept, bias=bias, out_dtype=out_dtype)
-    args = _kept_args(kept)
+    args, index = _kept_args(kept)
     if dy.dtype != kept.dtype:
         raise ValueError(f"dy must have the kept activation's type {kept.dtype}, got {dy.dtype}")
-    if dy.dim() == 0 or dy.shape[:-1] != torch.Size(kept.shape):
+    if dy.dim() == 0 or dy.shape[:-1] != kept.shape:
         raise ValueError(f"dy must have the kept activation's leading dims {tuple(kept.shape)}, got {tuple(dy.shape)}")
     if out_dtype is None:
         out_dtype = dy.dtype
@@ -141,26 +153,27 @@ def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False,
     if dy.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("weight_grad_act8 has no gradient: call it under torch.no_grad(), or on dy.detach()")
     check_no_tangent("weight_grad_act8", dy)
-    device = kept.q.device
-    check_device(dy, device, "dy")
+    if dy.get_device() != index:
+        raise ValueError(f"dy must be on {kept.q.device}, got {dy.device}")
     out, features = dy.shape[-1], kept.features
-    if out > MAX_COLS:
-        raise ValueError(f"dy must have at most {MAX_COLS} features, got {out}")
+    if out > MAX_OUT:
+        raise ValueError(f"dy must have at most {MAX_OUT} features, got {out}")
     rows, tokens, ld = _token_rows(dy, "dy")
-    if tokens > 1 and ld > MAX_COLS:
+    if tokens > 1 and ld > MAX_OUT:
         rows, ld = rows.contiguous(), out
     elif tokens <= 1:
         ld = out
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return weight_grad_act8(dy, kept, bias=bias, out_dtype=out_dtype)
-    dw = torch.empty((out, features), dtype=out_dtype, device=device)
-    db = torch.empty(out, dtype=out_dtype, device=device) if bias else None
+    code = DTYPE_CODES[dy.dtype]
+    dw = dy.new_empty((out, features), dtype=out_dtype)
+    db = dy.new_empty(out, dtype=out_dtype) if bias else None
     lib, need = _native.lib(), ctypes.c_uint64()
-    _native.check(lib.sh_weight_grad_act8_workspace(args, DTYPE_CODES[dy.dtype], out, bool(bias), ctypes.byref(need)))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-    _native.check(lib.sh_weight_grad_act8(rows.data_ptr(), DTYPE_CODES[dy.dtype], ld, out, args, dw.data_ptr(), DTYPE_CODES[out_dtype],
-                                          features, None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+    _native.check(lib.sh_weight_grad_act8_workspace(args, code, out, bool(bias), ctypes.byref(need)))
+    ws = dy.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    _native.check(lib.sh_weight_grad_act8(rows.data_ptr(), code, ld, out, args, dw.data_ptr(), DTYPE_CODES[out_dtype], features,
+                                          None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
                                           need.value, current_stream_handle()))
     return dw, db
 

@@ -66,27 +66,41 @@ int launch_act8(const sh_act8* k, void* x, uint64_t x_ld, uint32_t dtype, bool b
 
 struct GradPlan {
   int tile;
-  uint32_t tiles, splits, split_tokens;
+  uint64_t tiles;
+  uint32_t splits, split_tokens;
   uint64_t bytes;
 };
 
 constexpr uint32_t kComputeUnits = 256;
 
-// The tile, and into how many parts the tokens are split where the tiles alone leave compute units idle.
+// The tile, and into how many parts the tokens are split, of the least estimated time: rounds of workgroups over the
+// compute units, one on each, times the steps of a part; and the parts' sums, written and read once at 3.5 TB/s, with a launch of
+// 3 us. Around the switches, times in us (tile, parts):
+//   1013 x 1000 x 1155    128x128 1: 19   2: 22   256x256 1: 39     4096 x 2048 x 2048   128x128 1: 61   256x256 1: 113   4: 66
+//   16384 x 1024 x 1024   128x128 1: 190  4: 68   256x256 4: 124    4608 x 4096 x 4096   256x256 1: 145  128x128 1: 297
+//   4096 x 32 x 4096      32x128 4: 17    8: 14   16: 21
 GradPlan plan_of(const sh_act8* k, uint32_t out, uint32_t dtype, bool bias) {
-  GradPlan p{};
-  auto tiles = [&](int i) {
-    return (uint64_t)((out + sh::kGradTiles[i].out - 1) / sh::kGradTiles[i].out) * ((k->cols + sh::kGradTiles[i].in - 1) / sh::kGradTiles[i].in);
-  };
-  p.tile = out <= 64 ? 0 : dtype != SH_DTYPE_F32 && tiles(2) >= kComputeUnits / 2 ? 2 : 1;
-  p.tiles = (uint32_t)tiles(p.tile);
-  const uint32_t steps = std::max(1u, (k->tokens + sh::kGradStep - 1) / sh::kGradStep);
-  const uint32_t want = p.tiles >= kComputeUnits ? 1 : 2 * kComputeUnits / std::max(1u, p.tiles);
-  const uint32_t split_steps = std::max(4u, (steps + want - 1) / want);
-  p.splits = (steps + split_steps - 1) / split_steps;
-  p.split_tokens = split_steps * sh::kGradStep;
-  p.bytes = p.splits > 1 ? 4ull * p.splits * ((uint64_t)out * k->cols + (bias ? out : 0)) : 0;
-  return p;
+  const bool wide = dtype == SH_DTYPE_F32;
+  const uint64_t sums = (uint64_t)out * k->cols + (bias ? out : 0);
+  GradPlan best{};
+  double best_cost = 0;
+  for (int i = 0; i < sh::kGradTileCount; ++i) {
+    const sh::GradTile& t = sh::kGradTiles[i];
+    const uint32_t step = t.of[wide].step;
+    if (step == 0) continue;
+    const uint64_t tiles = ((uint64_t)out + t.out - 1) / t.out * (((uint64_t)k->cols + t.in - 1) / t.in);
+    const uint32_t steps = std::max(1u, (k->tokens + step - 1) / step);
+    for (uint32_t parts = 1; parts <= steps && (parts == 1 || tiles * parts <= 2 * kComputeUnits); parts *= 2) {
+      const uint32_t part_steps = (steps + parts - 1) / parts, splits = (steps + part_steps - 1) / part_steps;
+      const double rounds = (double)((tiles * splits + kComputeUnits - 1) / kComputeUnits);
+      const double join = splits > 1 ? 300 + (double)sums * 8 * splits / 35e3 : 0;
+      const double cost = rounds * part_steps * t.of[wide].cost + join;
+      if (best.tiles != 0 && cost >= best_cost) continue;
+      best_cost = cost;
+      best = {i, tiles, splits, part_steps * step, splits > 1 ? 4 * sums * splits : 0};
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -125,9 +139,9 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   sh::clear_error();
   if (int st = check_kept(kept, who)) return st;
   if (int st = check_values(dy, "dy", dtype, out_features == 0 ? 0 : kept->tokens, who)) return st;
-  if (out_features > SH_ACT8_MAX_COLS || dy_ld > SH_ACT8_MAX_COLS)
+  if (out_features > SH_WEIGHT_GRAD_MAX_OUT || dy_ld > SH_WEIGHT_GRAD_MAX_OUT)
     return sh::fail(SH_ERR_INVALID, "%s: out_features %u or dy_ld %llu is more than %u", who, out_features, (unsigned long long)dy_ld,
-                    SH_ACT8_MAX_COLS);
+                    SH_WEIGHT_GRAD_MAX_OUT);
   if (int st = check_values(dweight, "dweight", out_dtype, out_features, who)) return st;
   if (int st = check_out_rows(dw_ld, out_features, kept->cols, "dw_ld", who)) return st;
   if (misaligned(dbias, dtype_bytes(out_dtype))) return sh::fail(SH_ERR_INVALID, "%s: dbias is not aligned to its type", who);
@@ -137,8 +151,8 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
     return sh::fail(SH_ERR_INVALID, "%s: the workspace holds %llu bytes, %llu are needed", who,
                     (unsigned long long)workspace_bytes, (unsigned long long)p.bytes);
   if (misaligned(workspace, 16)) return sh::fail(SH_ERR_INVALID, "%s: workspace is not 16-byte aligned", who);
-  const sh::GradTile& tile = sh::kGradTiles[p.tile];
-  if ((uint64_t)p.tiles * p.splits > 0xFFFFFFFFull / tile.threads)
+  const uint32_t threads = sh::kGradTiles[p.tile].of[dtype == SH_DTYPE_F32].threads;
+  if (p.tiles * p.splits > 0xFFFFFFFFull / threads)
     return sh::fail(SH_ERR_INVALID, "%s: %u x %u gradients are too many for one launch", who, out_features, kept->cols);
   sh::WeightGradArgs a{};
   a.dy = dy;
@@ -159,7 +173,7 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount - 1, "one kernel per type and tile");
   void* args[] = {(void*)&a};
   if (int st = sh::launch_kernel((sh::KernelId)(sh::kKernWeightGradBf1632x128 + (dtype - SH_DTYPE_BF16) * sh::kGradTileCount + p.tile),
-                                 p.tiles * p.splits, tile.threads, (hipStream_t)stream, args, who))
+                                 (uint32_t)(p.tiles * p.splits), threads, (hipStream_t)stream, args, who))
     return st;
   if (p.splits == 1) return SH_OK;
   const uint64_t values = (uint64_t)out_features * ((kept->cols + 3) / 4) + (dbias != nullptr ? out_features : 0);

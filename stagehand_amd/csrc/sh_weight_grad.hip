@@ -48,7 +48,7 @@ __device__ __forceinline__ f32x4_t mfma(s16x8_t a, s16x8_t b, f32x4_t c) {
   else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, vb, c, 0, 0, 0);
 }
 
-// A stage holds kGradStep tokens' rows of N 16-bit values. The 16 values of unit u lie in unit u ^ swizzle(t): the
+// A stage holds the rows of N 16-bit values of some tokens. The 16 values of unit u lie in unit u ^ swizzle(t): the
 // rows that a transposing read takes together, 4 of every 8, then lie in different LDS banks.
 template <uint32_t N>
 __device__ __forceinline__ constexpr uint32_t swizzle(uint32_t t) {
@@ -93,10 +93,10 @@ __device__ __forceinline__ void each(const F& f) {
   }
 }
 
-template <typename T, uint32_t TO, uint32_t TI, uint32_t WO, uint32_t WI>
+template <typename T, uint32_t TO, uint32_t TI, uint32_t WO, uint32_t WI, uint32_t kStep>
 __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* lds) {
   using E = typename Multiplied<T>::Type;
-  constexpr uint32_t kParts = Multiplied<T>::kParts, kStep = sh::kGradStep;
+  constexpr uint32_t kParts = Multiplied<T>::kParts;
   constexpr uint32_t kThreads = WO * WI * 64, FO = TO / WO / 16, FI = TI / WI / 16;
   static_assert(FI == 4, "a wavefront's inputs are one group of 64 permuted ones");
   constexpr uint32_t kDy = kStep * TO, kStage = kParts * kDy + kStep * TI, kGroups64 = TI / 64;
@@ -105,8 +105,8 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   const uint32_t wo = wave / WI, wi = wave % WI;
 
   // XCDs take consecutive runs of tiles, which run down groups of kGroup tiles of outputs: an XCD's L2 then serves a block of
-  // 8 x 4 tiles.
-  constexpr uint32_t kGroup = 8;
+  // 4 x 8 tiles.
+  constexpr uint32_t kGroup = 4;
   const uint32_t tiles_o = (a.out + TO - 1) / TO, tiles_i = (a.cols + TI - 1) / TI, tiles = tiles_o * tiles_i;
   const uint32_t all = tiles * a.splits, xcd = blockIdx.x % 8;
   const uint32_t p = xcd * (all / 8) + min(xcd, all % 8) + blockIdx.x / 8;
@@ -227,54 +227,64 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   };
   static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
   const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
-  auto read_x = [&](const short* stage, uint32_t j) __attribute__((always_inline)) {
-    return read_fragment<TI>(stage + kParts * kDy, x_read, j * kGroups64);
+  // Fragment j of x^, of the stage's tokens 32 k .. 32 k + 31.
+  auto read_x = [&](const short* stage, uint32_t k, uint32_t j) __attribute__((always_inline)) {
+    return read_fragment<TI>(stage + kParts * kDy + k * 32 * TI, x_read, j * kGroups64);
   };
-  // Fragment b of dy: of part b / FO.
+  // Fragment b of dy: of tokens 32 (b / kOf32) on, of part b % kOf32 / FO.
+  constexpr uint32_t kOf32 = kParts * FO;
   auto read_dy = [&](const short* stage, uint32_t b) __attribute__((always_inline)) {
-    return read_fragment<TO>(stage + b / FO * kDy, dy_read, b % FO);
+    return read_fragment<TO>(stage + b % kOf32 / FO * kDy + b / kOf32 * 32 * TO, dy_read, b % FO);
   };
 
   f32x4_t acc[FO][FI] = {};
-  constexpr uint32_t NB = kParts * FO, kAhead = NB < 2 ? NB : 2;
+  // A stage's products go in NB blocks, one for each fragment of dy, which is read kAhead blocks before. The blocks before
+  // block kBarrier also write the next stage to LDS and start the loads of the one after the next two. After the barrier the
+  // next stage's first fragments are read and the inputs of the one after it converted. A third stage of LDS is written
+  // while the other two are read. The instructions of a block are spread between its products: all at once they would
+  // hold up the products of both wavefronts of a SIMD.
+  constexpr uint32_t K32 = kStep / 32, NB = K32 * kOf32, kBarrier = K32 == 1 ? NB / 2 : NB - kOf32;
+  constexpr uint32_t kAhead = NB - kBarrier < 2 ? NB - kBarrier : 2, kFirstHalf = kBarrier > 0 ? kBarrier : 1, kWrites = NX * 4 + ND;
+  static_assert(K32 == 1 || K32 % 2 == 0, "stages start with the same half of x");
   Staged staged[2];
   s16x8_t x[2][FI], d[NB + kAhead];
-  // One stage: fragment b of dy is multiplied while fragment b + 2 is read. The first half also writes the next stage to
-  // LDS and starts the loads of the one after the next two; after the barrier in its middle, the second half reads the
-  // next stage's first fragments. A third stage of LDS is written while the other two are read. The instructions of a
-  // part are spread between its products: all at once they would hold up the products of both wavefronts of a SIMD.
-  constexpr uint32_t kHalf = NB / 2 > 0 ? NB / 2 : 1, kWrites = NX * 4 + ND;
   auto multiply = [&](auto turn, uint32_t s) __attribute__((always_inline)) {
     constexpr uint32_t V = decltype(turn)::value;
     const short* stage = lds + s * kStage;
     short* next = lds + (s == 2 ? 0 : s + 1) * kStage;
     each<NB>([&](auto block) __attribute__((always_inline)) {
-      constexpr uint32_t B = decltype(block)::value;
+      constexpr uint32_t B = decltype(block)::value, K = B / kOf32, X = K32 == 1 ? V : K % 2;
       if constexpr (B == 0) add_bias(staged[V ^ 1]);
-      if constexpr (B < kHalf) {
-        each<(B + 1) * kWrites / kHalf, B * kWrites / kHalf>([&](auto w) __attribute__((always_inline)) {
+      if constexpr (B < kFirstHalf) {
+        each<(B + 1) * kWrites / kFirstHalf, B * kWrites / kFirstHalf>([&](auto w) __attribute__((always_inline)) {
           constexpr uint32_t I = decltype(w)::value;
           if constexpr (I < NX * 4) put_x(next, I / 4, I % 4);
           else put_dy(staged[V ^ 1], next, I - NX * 4);
         });
-        if constexpr (B == kHalf - 1) load(staged[V ^ 1]);
+        if constexpr (B == kFirstHalf - 1) load(staged[V ^ 1]);
       }
       if constexpr (B + kAhead < NB) d[B + kAhead] = read_dy(stage, B + kAhead);
-      if constexpr (B == NB / 2) {
+      if constexpr (B == kBarrier) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      if constexpr (B >= NB / 2) {
-        constexpr uint32_t kFrom = (B - NB / 2) * FI / (NB - NB / 2), kTo = (B - NB / 2 + 1) * FI / (NB - NB / 2);
-        each<kTo, kFrom>([&](auto j) __attribute__((always_inline)) { x[V ^ 1][decltype(j)::value] = read_x(next, decltype(j)::value); });
-        constexpr uint32_t kFirst = (B - NB / 2) * NX * 4 / (NB - NB / 2), kLast = (B - NB / 2 + 1) * NX * 4 / (NB - NB / 2);
+      // the other half of x: of the next 32 tokens, or of the next stage
+      constexpr uint32_t kLead = K + 1 < K32 ? K * kOf32 : kBarrier, kOf = (K + 1 < K32 ? kLead + kOf32 : NB) - kLead;
+      if constexpr (B >= kLead) {
+        each<(B - kLead + 1) * FI / kOf, (B - kLead) * FI / kOf>([&](auto j) __attribute__((always_inline)) {
+          constexpr uint32_t J = decltype(j)::value;
+          x[X ^ 1][J] = K + 1 < K32 ? read_x(stage, K + 1, J) : read_x(next, 0, J);
+        });
+      }
+      if constexpr (B >= kBarrier) {
+        constexpr uint32_t kFirst = (B - kBarrier) * NX * 4 / (NB - kBarrier), kLast = (B - kBarrier + 1) * NX * 4 / (NB - kBarrier);
         each<kLast, kFirst>([&](auto c) __attribute__((always_inline)) { convert_x(staged[V], decltype(c)::value / 4, decltype(c)::value % 4); });
       }
       if constexpr (B + kAhead >= NB) d[B + kAhead] = read_dy(next, B + kAhead - NB);
       each<FI>([&](auto j) __attribute__((always_inline)) {
         constexpr uint32_t J = decltype(j)::value;
-        acc[B % FO][J] = mfma<E>(x[V][J], d[B], acc[B % FO][J]);
+        acc[B % FO][J] = mfma<E>(x[X][J], d[B], acc[B % FO][J]);
       });
       each<FI>([&](auto) __attribute__((always_inline)) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // an LDS read
@@ -301,7 +311,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   convert_all(staged[1]);
   __syncthreads();
 #pragma unroll
-  for (uint32_t j = 0; j < FI; ++j) x[0][j] = read_x(lds, j);
+  for (uint32_t j = 0; j < FI; ++j) x[0][j] = read_x(lds, 0, j);
 #pragma unroll
   for (uint32_t b = 0; b < kAhead; ++b) d[b] = read_dy(lds, b);
   uint32_t s = 0;
@@ -346,7 +356,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
     for (uint32_t k = 0; k < 8; ++k) sum[dy_t * TO + dy_o + k] = bias[k];
   }
   __syncthreads();
-  constexpr uint32_t kSums = kDyRows < kStep ? kDyRows : kStep;
+  constexpr uint32_t kSums = kDyRows < kStep ? kDyRows : kStep;  // work-items that staged an output
   for (uint32_t k = threadIdx.x; k < TO; k += kThreads) {
     const uint32_t o = o0 + k;
     if (o >= a.out) continue;
@@ -363,19 +373,19 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
 }  // namespace
 
 // The tiles of sh_act8_args.h.
-#define SH_WEIGHT_GRAD(name, T, TO, TI, WO, WI)                                                                   \
+#define SH_WEIGHT_GRAD(name, T, TO, TI, WO, WI, STEP)                                                             \
   extern "C" __global__ __launch_bounds__(WO * WI * 64, 2) void sh_weight_grad_##name##_##TO##x##TI##_kernel(sh::WeightGradArgs a) { \
-    __shared__ alignas(16) short lds[3 * sh::kGradStep * (Multiplied<T>::kParts * TO + TI)];                      \
-    weight_grad<T, TO, TI, WO, WI>(a, lds);                                                                       \
+    __shared__ alignas(16) short lds[3 * STEP * (Multiplied<T>::kParts * TO + TI)];                               \
+    weight_grad<T, TO, TI, WO, WI, STEP>(a, lds);                                                                 \
   }
-SH_WEIGHT_GRAD(bf16, __bf16, 32, 128, 2, 2)
-SH_WEIGHT_GRAD(bf16, __bf16, 128, 128, 2, 2)
-SH_WEIGHT_GRAD(bf16, __bf16, 256, 256, 2, 4)
-SH_WEIGHT_GRAD(f16, _Float16, 32, 128, 2, 2)
-SH_WEIGHT_GRAD(f16, _Float16, 128, 128, 2, 2)
-SH_WEIGHT_GRAD(f16, _Float16, 256, 256, 2, 4)
-SH_WEIGHT_GRAD(f32, float, 32, 128, 2, 2)
-SH_WEIGHT_GRAD(f32, float, 128, 128, 2, 2)
+SH_WEIGHT_GRAD(bf16, __bf16, 32, 128, 2, 2, 128)
+SH_WEIGHT_GRAD(bf16, __bf16, 128, 128, 4, 2, 64)
+SH_WEIGHT_GRAD(bf16, __bf16, 256, 256, 2, 4, 32)
+SH_WEIGHT_GRAD(f16, _Float16, 32, 128, 2, 2, 128)
+SH_WEIGHT_GRAD(f16, _Float16, 128, 128, 4, 2, 64)
+SH_WEIGHT_GRAD(f16, _Float16, 256, 256, 2, 4, 32)
+SH_WEIGHT_GRAD(f32, float, 32, 128, 2, 2, 64)
+SH_WEIGHT_GRAD(f32, float, 128, 128, 2, 2, 32)
 
 // dweight and dbias from the sums of the splits, in their order: four values a work-item, then the biases.
 extern "C" __global__ __launch_bounds__(sh::kGradJoinThreads) void sh_weight_grad_join_kernel(sh::WeightGradArgs a) {
