@@ -12,9 +12,8 @@
 
 namespace {
 
-// Groups whose sums are joined in one launch, with SH_LAYER_NORM_MAX_COLS values each.
-constexpr uint32_t kMostGroups =
-    0xFFFFFFFFu / (2 * sh::kNormJoinThreads * (SH_LAYER_NORM_MAX_COLS / sh::kNormJoinCols));
+// Sequences with a weight of their own, a workgroup each at least, in one launch of under 2^32 work-items.
+constexpr uint32_t kMostGroups = 0xFFFFFFFFu / sh::norm_most_threads(true);
 
 using sh::dtype_bytes;
 using sh::known_dtype;
