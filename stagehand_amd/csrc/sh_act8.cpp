@@ -90,7 +90,7 @@ GradPlan plan_of(const sh_act8* k, uint32_t out, uint32_t dtype, bool bias) {
     if (step == 0) continue;
     const uint64_t tiles = ((uint64_t)out + t.out - 1) / t.out * (((uint64_t)k->cols + t.in - 1) / t.in);
     const uint32_t steps = std::max(1u, (k->tokens + step - 1) / step);
-    for (uint32_t parts = 1; parts <= steps && (parts == 1 || tiles * parts <= 2 * kComputeUnits); parts *= 2) {
+    for (uint32_t parts = 1; parts <= steps && (parts == 1 || tiles * parts <= 2 * kComputeUnits); parts += parts < 16 ? 1 : parts) {
       const uint32_t part_steps = (steps + parts - 1) / parts, splits = (steps + part_steps - 1) / part_steps;
       const double rounds = (double)((tiles * splits + kComputeUnits - 1) / kComputeUnits);
       const double join = splits > 1 ? 300 + (double)sums * 8 * splits / 35e3 : 0;

@@ -46,6 +46,7 @@ struct GradTile {
 };
 constexpr GradTile kGradTiles[] = {
     {32, 128, {{256, 128, 120}, {256, 64, 100}}},
+    {64, 128, {{512, 64, 60}, {256, 32, 70}}},
     {128, 128, {{512, 64, 85}, {256, 32, 118}}},
     {256, 256, {{512, 32, 93}, {0, 0, 0}}},
 };

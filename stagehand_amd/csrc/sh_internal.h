@@ -220,12 +220,15 @@ enum KernelId : int {
   kKernAct8DequantizeF32,
   // weight gradients: per type and tile of sh_act8_args.h, without the largest for fp32
   kKernWeightGradBf1632x128,
+  kKernWeightGradBf1664x128,
   kKernWeightGradBf16128x128,
   kKernWeightGradBf16256x256,
   kKernWeightGradF1632x128,
+  kKernWeightGradF1664x128,
   kKernWeightGradF16128x128,
   kKernWeightGradF16256x256,
   kKernWeightGradF3232x128,
+  kKernWeightGradF3264x128,
   kKernWeightGradF32128x128,
   kKernWeightGradJoin,
   kKernelCount

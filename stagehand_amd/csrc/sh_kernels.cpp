@@ -192,12 +192,15 @@ constexpr KernelSpec kKernelSpecs[sh::kKernelCount] = {
     {kModAct8, "sh_act8_quantize_f32_kernel"},
     {kModAct8, "sh_act8_dequantize_f32_kernel"},
     {kModWeightGrad, "sh_weight_grad_bf16_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_bf16_64x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_bf16_128x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_bf16_256x256_kernel"},
     {kModWeightGrad, "sh_weight_grad_f16_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f16_64x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_f16_128x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_f16_256x256_kernel"},
     {kModWeightGrad, "sh_weight_grad_f32_32x128_kernel"},
+    {kModWeightGrad, "sh_weight_grad_f32_64x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_f32_128x128_kernel"},
     {kModWeightGrad, "sh_weight_grad_join_kernel"},
 };

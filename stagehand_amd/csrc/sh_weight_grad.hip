@@ -80,6 +80,23 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_resource(const void* p, u
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, rows > 0 ? (rows - 1) * ld + width : 0, 0x00020000);
 }
 
+// Stores N neighbouring values, or the first `count` of them.
+template <typename T, uint32_t N>
+__device__ __forceinline__ void store_run(T* out, const float (&v)[N], uint32_t count) {
+  typedef T Run __attribute__((ext_vector_type(N)));
+  typedef Run Any __attribute__((aligned(2)));
+  if (count >= N) {
+    Run x;
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) x[j] = (T)v[j];
+    *reinterpret_cast<Any*>(out) = x;
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j)
+      if (j < count) out[j] = (T)v[j];
+  }
+}
+
 // f(0), f(1) .. f(N - 1) with constants for the compiler.
 template <uint32_t I>
 struct Constant {
@@ -209,10 +226,15 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
       }
     }
   };
-  // Column 64 g + 16 p + 4 f + m of x^ is column 4 p + m of the unit f * kGroups64 + g, fragment f of the group g: a lane
-  // of the product then has 16 consecutive inputs.
+  // Unit j * kGroups64 + g is fragment j of the group g of 64 columns. It holds columns 16 p + 4 j + m of the group, at 4 p + m:
+  // a lane of the product then has 16 consecutive inputs for 16-byte stores of 16-bit values. Or, for gradients in fp32, which
+  // are stored as such, columns 16 j + 4 p + m: the lanes' 4 consecutive inputs of a fragment lie side by side (4608 x 4096 x
+  // 4096 683 -> 665 us).
   static_assert(kQRows % 16 == 0 || NX == 1, "a work-item's rows have one swizzle");
-  const uint32_t x_place = q_t * TI + ((q_i / 64) ^ swizzle<TI>(q_t)) * 16 + q_i % 64 / 4;
+  constexpr bool kSpread = sizeof(T) == 2;
+  constexpr uint32_t kXStep = kSpread ? kGroups64 * 16 : 4;
+  const uint32_t q_c = q_i / 16;
+  const uint32_t x_place = q_t * TI + ((kSpread ? q_c / 4 : q_c % 4 * kGroups64 + q_c / 4) ^ swizzle<TI>(q_t)) * 16 + (kSpread ? q_c % 4 * 4 : 0);
   // In two steps, as their instructions hide behind products of different halves of a stage.
   Out4 packed[NX][4];
   auto convert_x = [&](const Staged& v, uint32_t j, uint32_t f) __attribute__((always_inline)) {
@@ -223,7 +245,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
     for (uint32_t m = 0; m < 4; ++m) packed[j][f][m] = (E)x[m];
   };
   auto put_x = [&](short* stage, uint32_t j, uint32_t f) __attribute__((always_inline)) {
-    *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kGroups64 * 16) + j * kQRows * TI) = packed[j][f];
+    *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kXStep) + j * kQRows * TI) = packed[j][f];
   };
   static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
   const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
@@ -322,28 +344,37 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
     s = s == 2 ? 0 : s + 1;
   }
 
-  // lane: output l % 16 of each fragment of outputs, 16 consecutive inputs
-  const uint32_t i = i0 + wi * (TI / WI) + lane / 16 * 16;
-  const uint32_t count = i < a.cols ? a.cols - i : 0;
+  // lane: output l % 16 of each fragment of outputs
   float* sums = a.partials;
   if (sums != nullptr) sums += split * ((uint64_t)a.out * a.cols + (a.dbias != nullptr ? a.out : 0));
+  const uint32_t part = lane / 16, first = i0 + wi * (TI / WI);
 #pragma unroll
   for (uint32_t f = 0; f < FO; ++f) {
     const uint32_t o = o0 + wo * (TO / WO) + f * 16 + lane % 16;
     if (o >= a.out) continue;
-    float v[2][8];
+    // neighbouring sums, of inputs i on
+    auto store = [&](const auto& v, uint32_t i) __attribute__((always_inline)) {
+      constexpr uint32_t N = sizeof(v) / 4;
+      const uint32_t n = i < a.cols ? a.cols - i : 0;
+      if (sums != nullptr) return store_run<float, N>(sums + (uint64_t)o * a.cols + i, v, n);
+      const uint64_t at = o * a.dw_ld + i;
+      if (a.out_dtype == SH_DTYPE_BF16) store_run<__bf16, N>(static_cast<__bf16*>(a.dweight) + at, v, n);
+      else if (a.out_dtype == SH_DTYPE_F16) store_run<_Float16, N>(static_cast<_Float16*>(a.dweight) + at, v, n);
+      else store_run<float, N>(static_cast<float*>(a.dweight) + at, v, n);
+    };
+    if constexpr (kSpread) {
 #pragma unroll
-    for (uint32_t j = 0; j < 16; ++j) v[j / 8][j % 8] = acc[f][j / 4][j % 4];
+      for (uint32_t h = 0; h < 2; ++h) {
+        float v[8];
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-      const uint32_t n = count > h * 8 ? count - h * 8 : 0;
-      if (sums != nullptr) {
-        Values8<float>::store(sums + (uint64_t)o * a.cols + i + h * 8, v[h], n);
-      } else {
-        const uint64_t at = o * a.dw_ld + i + h * 8;
-        if (a.out_dtype == SH_DTYPE_BF16) Values8<__bf16>::store(static_cast<__bf16*>(a.dweight) + at, v[h], n);
-        else if (a.out_dtype == SH_DTYPE_F16) Values8<_Float16>::store(static_cast<_Float16*>(a.dweight) + at, v[h], n);
-        else Values8<float>::store(static_cast<float*>(a.dweight) + at, v[h], n);
+        for (uint32_t j = 0; j < 8; ++j) v[j] = acc[f][h * 2 + j / 4][j % 4];
+        store(v, first + part * 16 + h * 8);
+      }
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < FI; ++j) {
+        const float v[4] = {acc[f][j][0], acc[f][j][1], acc[f][j][2], acc[f][j][3]};
+        store(v, first + j * 16 + part * 4);
       }
     }
   }
@@ -379,12 +410,15 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
     weight_grad<T, TO, TI, WO, WI, STEP>(a, lds);                                                                 \
   }
 SH_WEIGHT_GRAD(bf16, __bf16, 32, 128, 2, 2, 128)
+SH_WEIGHT_GRAD(bf16, __bf16, 64, 128, 4, 2, 64)
 SH_WEIGHT_GRAD(bf16, __bf16, 128, 128, 4, 2, 64)
 SH_WEIGHT_GRAD(bf16, __bf16, 256, 256, 2, 4, 32)
 SH_WEIGHT_GRAD(f16, _Float16, 32, 128, 2, 2, 128)
+SH_WEIGHT_GRAD(f16, _Float16, 64, 128, 4, 2, 64)
 SH_WEIGHT_GRAD(f16, _Float16, 128, 128, 4, 2, 64)
 SH_WEIGHT_GRAD(f16, _Float16, 256, 256, 2, 4, 32)
 SH_WEIGHT_GRAD(f32, float, 32, 128, 2, 2, 64)
+SH_WEIGHT_GRAD(f32, float, 64, 128, 2, 2, 32)
 SH_WEIGHT_GRAD(f32, float, 128, 128, 2, 2, 32)
 
 // dweight and dbias from the sums of the splits, in their order: four values a work-item, then the biases.

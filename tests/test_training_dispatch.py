@@ -56,7 +56,7 @@ def test_sizes_of_the_act8_tests_reach_every_kernel(launched):
 
 def test_sizes_of_the_weight_gradient_tests_reach_every_kernel(launched):
     reached(launched, [f"grad {t} {o} {i} {code} 1" for t, o, i in test_weight_grad_act8_gpu.SIZES for code in DTYPE_CODES.values()],
-            "sh_weight_grad_", 9)
+            "sh_weight_grad_", 12)
 
 
 def test_kernels_are_of_the_type_that_is_asked_for(launched):

@@ -19,7 +19,8 @@ pytestmark = pytest.mark.gpu
 
 SIZES = [  # tokens, out, in
     (1, 1, 1), (1, 8, 32), (2, 7, 31), (31, 32, 33), (32, 33, 64), (33, 64, 65), (77, 65, 257), (128, 16, 1155), (129, 256, 256),
-    (1013, 40, 500), (200, 1000, 1155), (4096, 32, 1024), (300, 257, 129), (70, 3000, 2100), (520, 4100, 4130),
+    (1013, 40, 500), (200, 1000, 1155), (4096, 32, 1024), (300, 257, 129), (70, 3000, 2100), (520, 4100, 4130), (300, 1900, 1899),
+    (8000, 1001, 1155), (900, 257, 300),
 ]
 
 
