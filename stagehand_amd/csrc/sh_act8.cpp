@@ -22,7 +22,7 @@ int check_kept(const sh_act8* k, const char* who) {
   if (k == nullptr) return sh::fail(SH_ERR_INVALID, "%s: kept is NULL", who);
   if (k->cols == 0 || k->cols > SH_ACT8_MAX_COLS)
     return sh::fail(SH_ERR_INVALID, "%s: cols %u is not in 1 .. %u", who, k->cols, SH_ACT8_MAX_COLS);
-  if ((uint64_t)k->tokens * groups_of(k->cols) * (SH_ACT8_GROUP / 8) > 0xFFFFFFFFull - sh::kAct8Threads * sh::kAct8Chunks)
+  if ((uint64_t)k->tokens * groups_of(k->cols) * (SH_ACT8_GROUP / 8) > 0xFFFFFFFFull - sh::kAct8Threads)
     return sh::fail(SH_ERR_INVALID, "%s: %u tokens of %u values are too many for one launch", who, k->tokens, k->cols);
   if (k->tokens > 0 && (k->q == nullptr || k->exponent == nullptr))
     return sh::fail(SH_ERR_INVALID, "%s: q or exponent is NULL", who);
@@ -58,7 +58,7 @@ int launch_act8(const sh_act8* k, void* x, uint64_t x_ld, uint32_t dtype, bool b
   a.magic = sh::udiv_magic(a.row_chunks);
   a.tokens = k->tokens;
   a.cols = k->cols;
-  constexpr uint32_t per = sh::kAct8Threads * sh::kAct8Chunks;
+  constexpr uint32_t per = sh::kAct8Threads;
   void* args[] = {(void*)&a};
   return sh::launch_kernel((sh::KernelId)(sh::kKernAct8QuantizeBf16 + (dtype - SH_DTYPE_BF16) * 2 + back), (a.chunks + per - 1) / per,
                            sh::kAct8Threads, stream, args, who);

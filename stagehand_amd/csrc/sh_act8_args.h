@@ -19,7 +19,6 @@ struct Act8Args {
 };
 
 constexpr uint32_t kAct8Threads = 256;
-constexpr uint32_t kAct8Chunks = 1;  // that a work-item takes
 
 struct WeightGradArgs {
   const void* dy;

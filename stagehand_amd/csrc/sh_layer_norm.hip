@@ -4,11 +4,19 @@
 // With n = (x - mean) r, r = (var + eps)^(-1/2), and a gain w (1 + w when modulated): y = n w + b. For a gradient dy,
 // with g = dy w: dx = r (g - mean(g) - n mean(g n)), dw = sum of dy n and db = sum of dy over the tokens that share w, b.
 //
-// Bound by HBM: each value is read once and written once (backward: x and dy read, dx written). A team of wavefronts
-// holds a row in registers, so mean and variance take two passes over registers and one over memory: the variance is a
-// sum of squares of differences, not a difference of sums. The forward leaves mean and r of each token for the backward
-// pass. The gradients of w and b are summed in registers over a workgroup's tokens and joined by a second kernel,
-// always in the same order.
+// Bound by HBM: each value is read once and written once (backward: x and dy read, dx written). A team holds a row in
+// registers, so mean and variance take two passes over registers and one over memory: the variance is a sum of squares of
+// differences, not a difference of sums. The next row is on its way while one is worked on. The forward leaves mean and r
+// of each token for the backward pass. The gradients of w and b are summed in registers over a workgroup's tokens and
+// joined by a second kernel, always in the same order; every workgroup's sums are written and read once more, so there are
+// few workgroups.
+//
+// Measured: forward 2 x 8192 tokens x 4096 bf16 46 us (5.9 TB/s), keeping the input as well 69 us (4.9), 4608 x 4096 16 us (4.6),
+// 65536 x 256 14 us (4.9), 8192 x 16384 102 us (5.3); backward 84 us (4.8 TB/s), from the kept input 69 us (4.9), of which the
+// joining kernel takes 5; a large copy 5.2 TB/s by torch, 6.6 by this library's kernel. Two chunks a work-item against one:
+// 46 and 54 us; 1024 work-items a compute unit against 2048 and 512: 46, 49 and 53 us. Not kept: one or two rows for each of
+// many short workgroups, which stream copies faster (73 us: their start, weights and barriers come with every row), two teams
+// with joined sums in a workgroup of the backward pass (92 us), shuffles through LDS for a wavefront's sums.
 
 #include <hip/hip_runtime.h>
 
