@@ -159,7 +159,7 @@ def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False,
     if out > MAX_OUT:
         raise ValueError(f"dy must have at most {MAX_OUT} features, got {out}")
     rows, tokens, ld = _token_rows(dy, "dy")
-    if tokens > 1 and ld > MAX_OUT:
+    if tokens > 1 and not out <= ld <= MAX_OUT:  # rows that share memory, as of a sum's gradient, or lie too far apart
         rows, ld = rows.contiguous(), out
     elif tokens <= 1:
         ld = out

@@ -38,7 +38,8 @@ int check_values(const void* x, const char* name, uint32_t dtype, uint32_t token
   return SH_OK;
 }
 
-int check_out_rows(uint64_t ld, uint32_t rows, uint32_t cols, const char* name, const char* who) {
+// Rows of more than one do not overlap.
+int check_apart(uint64_t ld, uint32_t rows, uint32_t cols, const char* name, const char* who) {
   if (rows > 1 && ld < cols)
     return sh::fail(SH_ERR_INVALID, "%s: %s %llu is less than the %u values of a row", who, name, (unsigned long long)ld, cols);
   return SH_OK;
@@ -118,7 +119,7 @@ extern "C" int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype
   sh::clear_error();
   if (int st = check_kept(kept, who)) return st;
   if (int st = check_values(out, "out", dtype, kept->tokens, who)) return st;
-  if (int st = check_out_rows(out_ld, kept->tokens, kept->cols, "out_ld", who)) return st;
+  if (int st = check_apart(out_ld, kept->tokens, kept->cols, "out_ld", who)) return st;
   return launch_act8(kept, out, out_ld, dtype, true, (hipStream_t)stream, who);
 }
 
@@ -142,8 +143,10 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   if (out_features > SH_WEIGHT_GRAD_MAX_OUT || dy_ld > SH_WEIGHT_GRAD_MAX_OUT)
     return sh::fail(SH_ERR_INVALID, "%s: out_features %u or dy_ld %llu is more than %u", who, out_features, (unsigned long long)dy_ld,
                     SH_WEIGHT_GRAD_MAX_OUT);
+  // the kernels read up to a word past the end of a row that another one follows
+  if (int st = check_apart(dy_ld, kept->tokens, out_features, "dy_ld", who)) return st;
   if (int st = check_values(dweight, "dweight", out_dtype, out_features, who)) return st;
-  if (int st = check_out_rows(dw_ld, out_features, kept->cols, "dw_ld", who)) return st;
+  if (int st = check_apart(dw_ld, out_features, kept->cols, "dw_ld", who)) return st;
   if (misaligned(dbias, dtype_bytes(out_dtype))) return sh::fail(SH_ERR_INVALID, "%s: dbias is not aligned to its type", who);
   if (out_features == 0) return SH_OK;
   const GradPlan p = plan_of(kept, out_features, dtype, dbias != nullptr);

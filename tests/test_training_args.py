@@ -215,3 +215,10 @@ def test_host_tensors_are_refused():
                  lambda: layer_norm.layer_norm(x, stream=5), lambda: act8.checkpoint_act8(torch.sin, x.clone().requires_grad_())):
         with pytest.raises(ValueError, match="device"):
             call()
+
+
+def test_gradients_whose_rows_overlap_are_refused():
+    need = ctypes.c_uint64()
+    assert _native.lib().sh_weight_grad_act8_workspace(kept(tokens=4096), 1, 33, 1, ctypes.byref(need)) == _native.SH_OK
+    for ld in (0, 1, 32):
+        refused("sh_weight_grad_act8", P, 1, ld, 33, kept(tokens=4096), P, 3, 64, P, P, need.value, 0, match="dy_ld")

@@ -87,3 +87,20 @@ def test_layers_without_tokens():
     x = torch.empty(0, 3, 64, device="cuda", requires_grad=True)
     dx, dw, db = torch.autograd.grad(linear_act8(x, w, b), (x, w, b), torch.empty(0, 3, 8, device="cuda"))
     assert dx.shape == x.shape and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens, out", [(5, 33), (40, 1), (77, 1155), (1013, 301), (300, 64)])
+def test_gradients_expanded_over_tokens(dtype, tokens, out):
+    """A sum over the tokens sends back one row for all of them: the same gradients as from a copy of it for each."""
+    x = torch.randn(tokens, 96, device="cuda", dtype=dtype)
+    w, b = (torch.randn(s, device="cuda", dtype=dtype, requires_grad=True) for s in ((out, 96), (out,)))
+    row = torch.randn(out, device="cuda", dtype=dtype)
+    y = linear_act8(x, w, b)
+    got = torch.autograd.grad(y.sum(0), (w, b), row, retain_graph=True)
+    want = torch.autograd.grad(y, (w, b), row.expand(tokens, out).contiguous())
+    for g, e in zip(got, want):
+        assert torch.equal(g, e)
+    dy = row.expand(tokens, out)
+    for g, e in zip(weight_grad_act8(dy, quantize_activation(x), bias=True), want):
+        assert torch.equal(g, e)
