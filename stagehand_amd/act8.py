@@ -197,7 +197,8 @@ class _LinearAct8(torch.autograd.Function):
         want_x, want_weight, want_bias = ctx.needs_input_grad[:3]
         dx = dw = db = None
         if want_x:  # in two dims: a plain product, whatever dy's strides
-            dx = (dy.reshape(-1, dy.shape[-1]) @ weight).view(*dy.shape[:-1], weight.shape[1])
+            tokens = math.prod(dy.shape[:-1])
+            dx = (dy.reshape(tokens, dy.shape[-1]) @ weight).view(*dy.shape[:-1], weight.shape[1])
         if want_weight:
             dw, db = weight_grad_act8(dy, Activation8(q, exponent, *ctx.rest), bias=want_bias)
         elif want_bias:

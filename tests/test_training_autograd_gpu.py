@@ -104,3 +104,12 @@ def test_gradients_expanded_over_tokens(dtype, tokens, out):
     dy = row.expand(tokens, out)
     for g, e in zip(weight_grad_act8(dy, quantize_activation(x), bias=True), want):
         assert torch.equal(g, e)
+
+
+def test_layers_without_outputs():
+    for shape in ((64,), (5, 64), (2, 3, 64), (0, 64)):
+        x = torch.randn(shape, device="cuda", requires_grad=True)
+        w, b = torch.empty(0, 64, device="cuda", requires_grad=True), torch.empty(0, device="cuda", requires_grad=True)
+        y = linear_act8(x, w, b)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+        assert dx.shape == x.shape and not dx.any() and dw.shape == w.shape and db.shape == b.shape
