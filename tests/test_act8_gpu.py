@@ -5,6 +5,7 @@ import act8_oracle as oracle
 import pytest
 import torch
 from act8_oracle import DTYPES, activations
+from side_stream import side_stream
 
 from stagehand_amd.act8 import Activation8, quantize_activation
 
@@ -118,7 +119,7 @@ def test_offsets_past_32_bits():
 def test_another_stream_and_a_captured_graph():
     x = activations(300, 1155, dtype=torch.bfloat16)
     want = oracle.kept_values(x)
-    side = torch.cuda.Stream()
+    side = side_stream()
     side.wait_stream(torch.cuda.current_stream())
     kept = quantize_activation(x, stream=side)
     y = kept.dequantize(stream=side.cuda_stream)

@@ -13,6 +13,7 @@ import act8_oracle as oracle
 import pytest
 import torch
 from act8_oracle import DTYPES, ROUND, TINY, activations
+from side_stream import side_stream
 
 from stagehand_amd.act8 import quantize_activation
 from stagehand_amd.layer_norm import layer_norm
@@ -327,7 +328,7 @@ def test_offsets_past_32_bits(keep8):
 def test_another_stream_and_a_captured_graph(n, keep8):
     x, w, bias, dy = make(2, 600, n, torch.bfloat16, True)
     want = layer_norm(x, w, bias, modulate=True)
-    side = torch.cuda.Stream()
+    side = side_stream()
     side.wait_stream(torch.cuda.current_stream())
     got = layer_norm(x, w, bias, modulate=True, stream=side)
     side.synchronize()

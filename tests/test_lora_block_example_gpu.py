@@ -11,6 +11,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from side_stream import side_stream
 
 from stagehand_amd.act8 import quantize_activation
 
@@ -67,7 +68,7 @@ def test_a_captured_step_replays():
     def run():
         return torch.autograd.grad(block(leaf, vec, True), (leaf, *params), dy)
 
-    side = torch.cuda.Stream()
+    side = side_stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         run()

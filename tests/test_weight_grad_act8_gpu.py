@@ -11,6 +11,7 @@ import act8_oracle as oracle
 import pytest
 import torch
 from act8_oracle import DTYPES, ROUND, TINY, activations
+from side_stream import side_stream
 from torch.nn import functional as F
 
 from stagehand_amd.act8 import checkpoint_act8, linear_act8, quantize_activation, weight_grad_act8
@@ -171,7 +172,7 @@ def test_another_stream_and_a_captured_graph():
     dy, x = make(3000, 48, 300, torch.bfloat16)
     kept = quantize_activation(x)
     want = weight_grad_act8(dy, kept, bias=True)
-    side = torch.cuda.Stream()
+    side = side_stream()
     side.wait_stream(torch.cuda.current_stream())
     got = weight_grad_act8(dy, kept, bias=True, stream=side)
     side.synchronize()
