@@ -11,7 +11,7 @@
 //
 // Bound by the matrix cores in large products, at the clock that their power allows, and by the instructions that turn
 // bytes into 16-bit values, which every tile of outputs does again: 16384 x 16384 x 4096 (tokens x outputs x inputs) 1.86 to
-// 1.90 ms, 1160 to 1180 TFLOP/s (the installed library 1.83 ms, on a bf16 input); 4608 x 4096 x 4096 146 us. Small ones by
+// 1.99 ms, 1100 to 1180 TFLOP/s (the installed library 1.83 ms, on a bf16 input); 4608 x 4096 x 4096 138 to 146 us. Small ones by
 // the latency of their first loads and steps (1024^3 12.7 us), adapters of rank 32 by both and the joining of parts (4096
 // x 32 x 4096 13.8 us for 17 MB). What it took, at 16384 x 16384 x 4096:
 // - Three stages in LDS and fragments that are read ahead, over a barrier in the middle of a stage (2493 -> 2131 us).
