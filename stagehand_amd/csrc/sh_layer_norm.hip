@@ -5,11 +5,12 @@
 // with g = dy w: dx = r (g - mean(g) - n mean(g n)), dw = sum of dy n and db = sum of dy over the tokens that share w, b.
 //
 // Bound by HBM: each value is read once and written once (backward: x and dy read, dx written). A team holds a row in
-// registers, so mean and variance take two passes over registers and one over memory: the variance is a sum of squares of
-// differences, not a difference of sums. The next row is on its way while one is worked on. The forward leaves mean and r
-// of each token for the backward pass. The gradients of w and b are summed in registers over a workgroup's tokens and
-// joined by a second kernel, always in the same order; every workgroup's sums are written and read once more, so there are
-// few workgroups.
+// registers, so mean and variance take two passes over registers and one over memory: differences from a first mean, whose
+// own mean corrects both. A first mean alone is off by the roundings of the sum and of the division, which r, up to eps^(-1/2),
+// multiplies: rows of 1155 times 1000 had norms of 0.03 in the place of 0. The next row is on its way while one is worked on.
+// The forward leaves mean and r of each token for the backward pass. The gradients of w and b are summed in registers over a
+// workgroup's tokens and joined by a second kernel, always in the same order; every workgroup's sums are written and read once
+// more, so there are few workgroups.
 //
 // Measured: forward 2 x 8192 tokens x 4096 bf16 46 us (5.9 TB/s), keeping the input as well 69 us (4.9), 4608 x 4096 16 us (4.6),
 // 65536 x 256 14 us (4.9), 8192 x 16384 102 us (5.3); backward 84 us (4.8 TB/s), from the kept input 69 us (4.9), of which the
@@ -68,17 +69,19 @@ struct TeamSum {
       if (threadIdx.x < 2 * N * kMostWaves && threadIdx.x % kMostWaves >= blockDim.x / 64) (&slots[0][0][0])[threadIdx.x] = 0.0f;
     }
   }
-  __device__ __forceinline__ void operator()(float (&v)[N]) {
+  template <uint32_t M>
+  __device__ __forceinline__ void operator()(float (&v)[M]) {
+    static_assert(M <= N, "a slot for each sum");
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) v[i] = group_sum(v[i], TEAM ? 64 : lanes);
+    for (uint32_t i = 0; i < M; ++i) v[i] = group_sum(v[i], TEAM ? 64 : lanes);
     if constexpr (TEAM) {
       if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (uint32_t i = 0; i < N; ++i) slots[turn][i][threadIdx.x / 64] = v[i];
+        for (uint32_t i = 0; i < M; ++i) slots[turn][i][threadIdx.x / 64] = v[i];
       }
       __syncthreads();
 #pragma unroll
-      for (uint32_t i = 0; i < N; ++i) {
+      for (uint32_t i = 0; i < M; ++i) {
         v[i] = 0.0f;
 #pragma unroll
         for (uint32_t w = 0; w < kMostWaves; ++w) v[i] += slots[turn][i][w];
@@ -149,8 +152,8 @@ template <typename T, bool TEAM, uint32_t C>
 __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
   const sh_layer_norm_args& a = ka.a;
   const Mine<TEAM, C> m(ka);
-  __shared__ alignas(16) float slots[2][1][kMostWaves];
-  TeamSum<TEAM, 1> team_sum(slots, ka.lanes);
+  __shared__ alignas(16) float slots[2][2][kMostWaves];
+  TeamSum<TEAM, 2> team_sum(slots, ka.lanes);
   const float rcols = 1.0f / (float)a.cols;
   const uint32_t row_chunks = (a.cols + SH_ACT8_GROUP - 1) / SH_ACT8_GROUP * (SH_ACT8_GROUP / 8);
   typename Values8<T>::Vec next[C];
@@ -190,24 +193,28 @@ __device__ __forceinline__ void forward(const sh::LayerNormKernelArgs& ka) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) sum[0] += v[j][i];
     team_sum(sum);
-    const float mean = sum[0] * rcols;
-    sum[0] = 0.0f;
+    // Differences from the product sum * rcols as it is, which the mean below starts from too: neither rounds it.
+    float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
-        v[j][i] = i < m.count(j) ? v[j][i] - mean : 0.0f;
-        sum[0] = __builtin_fmaf(v[j][i], v[j][i], sum[0]);
+        v[j][i] = i < m.count(j) ? __builtin_fmaf(sum[0], -rcols, v[j][i]) : 0.0f;
+        sums[0] += v[j][i];
+        sums[1] = __builtin_fmaf(v[j][i], v[j][i], sums[1]);
       }
     }
-    team_sum(sum);
-    const float r = 1.0f / __builtin_sqrtf(sum[0] * rcols + a.eps);
+    team_sum(sums);
+    const float off = sums[0] * rcols, mean = __builtin_fmaf(sum[0], rcols, off);
+    float var = __builtin_fmaf(off, -off, sums[1] * rcols);
+    if (var < 0.0f) var = 0.0f;  // and a NaN stays one
+    const float r = 1.0f / __builtin_sqrtf(var + a.eps), shift = -off * r;
     T* y = static_cast<T*>(a.y.data) + token.at(a.y);
 #pragma unroll
     for (uint32_t j = 0; j < C; ++j) {
       float out[8];
 #pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) out[i] = __builtin_fmaf(v[j][i] * r, w[j][i], b[j][i]);
+      for (uint32_t i = 0; i < 8; ++i) out[i] = __builtin_fmaf(__builtin_fmaf(v[j][i], r, shift), w[j][i], b[j][i]);
       Values8<T>::store(y + m.col(j), out, m.count(j));
     }
     if (a.stats != nullptr && m.item == 0) {

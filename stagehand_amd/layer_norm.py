@@ -6,7 +6,9 @@ For every token (the last dim of ``x``)::
     y = n * weight + bias                   # n * (1 + weight) + bias when `modulate`
 
 ``var`` is the mean of the squared differences. Statistics, products and the gradients' sums are held in fp32; outputs
-and gradients are rounded once.
+and gradients are rounded once. A mean far above the spread costs the output nothing; the backward pass takes the mean
+rounded to fp32: there ``n`` is off by up to ``2**-24 * |mean| / sqrt(var + eps)``. The sum of a row and that of its squared
+differences have to be numbers of fp32: values beyond 1e17, and where ``eps`` is 0 spreads below 1e-19, are outside it.
 
 Everything runs on the caller's current torch stream unless ``stream`` is given. There is no CPU path.
 """
