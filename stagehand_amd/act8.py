@@ -212,8 +212,8 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
 
     The output and the gradients of ``x`` and ``bias`` are those of an ordinary Linear, the gradient of ``weight`` that of one
     whose input were ``kept.dequantize()``. Layers with one input share what is kept of it: ``kept`` is
-    ``quantize_activation(x.detach())``, made once. Nothing is kept when ``weight`` needs no gradient. Under autocast,
-    inputs are cast as for an ordinary Linear (``kept`` then holds the cast input)."""
+    ``quantize_activation(x.detach())``, made once. Nothing is kept when ``weight`` needs no gradient, or without grad mode.
+    Under autocast, inputs are cast as for an ordinary Linear (``kept`` then holds the cast input)."""
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         with torch.autocast("cuda", enabled=False):
@@ -233,6 +233,8 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
         if kept.dtype != x.dtype or kept.features != x.shape[-1] or torch.Size(kept.shape) != x.shape[:-1]:
             raise ValueError(f"kept is of a {kept.dtype} {(*kept.shape, kept.features)} activation, x is {x.dtype} {tuple(x.shape)}")
         check_device(kept.q, x.device, "kept.q")
+    if not torch.is_grad_enabled():  # a Function's needs_input_grad does not look at this
+        return F.linear(x, weight, bias)
     return _LinearAct8.apply(x, weight, bias, kept)
 
 
