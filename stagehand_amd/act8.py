@@ -196,13 +196,13 @@ class _LinearAct8(torch.autograd.Function):
         weight, q, exponent = ctx.saved_tensors
         want_x, want_weight, want_bias = ctx.needs_input_grad[:3]
         dx = dw = db = None
+        rows = math.prod(dy.shape[:-1]), dy.shape[-1]
         if want_x:  # in two dims: a plain product, whatever dy's strides
-            tokens = math.prod(dy.shape[:-1])
-            dx = (dy.reshape(tokens, dy.shape[-1]) @ weight).view(*dy.shape[:-1], weight.shape[1])
+            dx = (dy.reshape(rows) @ weight).view(*dy.shape[:-1], weight.shape[1])
         if want_weight:
             dw, db = weight_grad_act8(dy, Activation8(q, exponent, *ctx.rest), bias=want_bias)
         elif want_bias:
-            db = dy.sum(tuple(range(dy.dim() - 1)))
+            db = dy.reshape(rows).sum(0)  # also of one token without leading dims
         return dx, dw, db, None
 
 
