@@ -230,6 +230,9 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
     Under autocast, inputs are cast as for an ordinary Linear (``kept`` then holds the cast input)."""
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
+        for what, t in (("x", x), ("weight", weight), ("bias", bias)):
+            if t is not None and t.dtype not in DTYPE_CODES:  # autocast leaves these as they are
+                raise ValueError(f"{what} must be of type bfloat16, float16 or float32, got {t.dtype}")
         with torch.autocast("cuda", enabled=False):
             return linear_act8(x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype), kept)
     check_device(x, None, "x")
