@@ -164,7 +164,8 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   a.dweight = dweight;
   a.dbias = dbias;
   a.partials = p.splits > 1 ? static_cast<float*>(workspace) : nullptr;
-  a.dy_ld = dy_ld;
+  // rows past the last of a part lie behind its end only at a distance of a row's values, also where there is one row
+  a.dy_ld = kept->tokens > 1 ? dy_ld : out_features;
   a.dw_ld = dw_ld;
   a.tokens = kept->tokens;
   a.out = out_features;
