@@ -257,7 +257,7 @@ def linear_act8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
 
 def checkpoint_act8(function: Callable[..., Any], x: torch.Tensor, *args: Any, **kwargs: Any) -> Any:
     """``function(x, *args, **kwargs)``, of which only ``x`` is kept for the backward pass, in 8 bits: the backward pass
-    recomputes the rest from ``quantize_activation(x).dequantize()``.
+    recomputes the rest from ``quantize_activation(x).dequantize()``, whose dims lie in memory in the order of those of ``x``.
 
     As ``torch.utils.checkpoint.checkpoint`` without reentrance, to which it leaves the recomputation (random state and
     autocast are restored); ``args`` and ``kwargs`` are kept as they are. ``function`` must not write to ``x``. The
@@ -269,11 +269,16 @@ def checkpoint_act8(function: Callable[..., Any], x: torch.Tensor, *args: Any, *
     check_no_tangent("checkpoint_act8", x)
     kept = quantize_activation(x.detach())
     needs_grad, first = x.requires_grad, [x]
+    strides = None if x.is_contiguous() else torch.empty_like(x, device="meta").stride()  # dense, dims in the order of x's
 
     def run(q: torch.Tensor, *rest: Any) -> Any:
         # the forward pass runs on x itself, a recomputation on what is kept of it
-        again = first[0] if first else kept.dequantize().requires_grad_(needs_grad)
-        return function(again, *rest, **kwargs)
+        if first:
+            return function(first[0], *rest, **kwargs)
+        again = kept.dequantize()
+        if strides is not None and again.stride() != strides:  # views that x's order of dims allows stay views
+            again = torch.empty_strided(again.shape, strides, dtype=again.dtype, device=again.device).copy_(again)
+        return function(again.requires_grad_(needs_grad), *rest, **kwargs)
 
     try:
         return checkpoint(run, kept.q, *args, use_reentrant=False)  # q tells it the device
