@@ -853,8 +853,10 @@ int sh_act8_dequantize(const sh_act8* kept, void* out, uint32_t dtype, uint64_t 
  * out_dtype. dy is tokens x out_features in `dtype` (rows dy_ld elements apart
  * that do not overlap, out_features and dy_ld at most SH_WEIGHT_GRAD_MAX_OUT),
  * the type that the kept activation had: values kept of bf16 or fp32 need not
- * be fp16 numbers. fp32 gradients are multiplied with all their bits. dbias may be NULL. The workspace (16-byte aligned device
- * memory, in use until the call's kernels have run) holds at least
+ * be fp16 numbers. fp32 gradients are multiplied with all their bits from
+ * 2^-110 on; of smaller ones, what lies under 2^-133 is cut (dbias keeps it).
+ * dbias may be NULL. The workspace (16-byte aligned device memory, in use
+ * until the call's kernels have run) holds at least
  * sh_weight_grad_act8_workspace bytes, for `bias` as dbias is given. */
 int sh_weight_grad_act8_workspace(const sh_act8* kept, uint32_t dtype, uint32_t out_features, uint32_t bias,
                                   uint64_t* bytes);

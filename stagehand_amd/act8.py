@@ -137,7 +137,8 @@ def weight_grad_act8(dy: torch.Tensor, kept: Activation8, *, bias: bool = False,
     ``dweight[o, i] = sum dy[..., o] * kept[..., i]``, ``dbias[o] = sum dy[..., o]`` (None without ``bias``).
 
     ``dy`` has the kept activation's type and leading dims. The products are summed in float32 in a fixed order and
-    rounded once to ``out_dtype`` (default: the type of ``dy``); a float32 ``dy`` is multiplied with all its bits."""
+    rounded once to ``out_dtype`` (default: the type of ``dy``). A float32 ``dy`` is multiplied with all its bits from ``2**-110``
+    on; of smaller values, what lies under ``2**-133`` is cut in ``dweight``."""
     if stream is not None:
         with on_stream(stream, kept.q):
             return weight_grad_act8(dy, kept, bias=bias, out_dtype=out_dtype)

@@ -4,7 +4,8 @@
 //   dW[o][i] = sum over the tokens t of dy[t][o] x^[t][i],  db[o] = sum over t of dy[t][o]
 //
 // x^ is exact in the 16-bit types (7 significant bits), so the matrix cores multiply the very numbers that were kept, and
-// sum in fp32. A gradient in fp32 goes in as three bf16 parts that add up to its 24 bits, each multiplied by itself.
+// sum in fp32. A gradient in fp32 goes in as three bf16 parts that add up to its 24 bits, each multiplied by itself; below
+// 2^-110 they lose what lies under 2^-133, the least number of bf16.
 //
 // Both operands lie with the tokens, over which is summed, in their slow direction. Tiles go through LDS as they lie, x^
 // in 16 bits, and the transposing LDS reads give the lanes what a fragment needs.
@@ -230,7 +231,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
         for (uint32_t part = 0; part < kParts; ++part) {
           Out8 out;
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits; all of an infinity
+          for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits, as far as bf16 has them; all of an infinity
             const float head = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xFFFF0000u);
             out[i] = (E)head;
             rest[i] = rest[i] == head ? 0.0f : rest[i] - head;
