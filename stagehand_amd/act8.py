@@ -33,7 +33,7 @@ from torch.autograd.graph import increment_version
 from torch.nn import functional as F
 
 from stagehand_amd import _native
-from stagehand_amd.int8 import DTYPE_CODES, _output, _token_rows, check_device, check_no_grad, check_no_tangent, on_stream
+from stagehand_amd.int8 import DTYPE_CODES, _output, _token_rows, check_device, check_no_tangent, on_stream
 from stagehand_amd.unpack import current_stream_handle
 
 __all__ = ["Activation8", "quantize_activation", "weight_grad_act8", "linear_act8", "checkpoint_act8"]

@@ -172,7 +172,6 @@ extern "C" int sh_weight_grad_act8(const void* dy, uint32_t dtype, uint64_t dy_l
   a.cols = kept->cols;
   a.splits = p.splits;
   a.split_tokens = p.split_tokens;
-  a.dtype = dtype;
   a.out_dtype = out_dtype;
   static_assert(sh::kKernWeightGradJoin - sh::kKernWeightGradBf1632x128 == 3 * sh::kGradTileCount - 1, "one kernel per type and tile");
   void* args[] = {(void*)&a};

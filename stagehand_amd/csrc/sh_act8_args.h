@@ -32,7 +32,7 @@ struct WeightGradArgs {
   uint32_t tokens, out, cols;
   uint32_t splits;        // parts of the tokens, each summed by workgroups of its own
   uint32_t split_tokens;  // tokens of a part, a multiple of the tile's step
-  uint32_t dtype, out_dtype;
+  uint32_t out_dtype;
 };
 
 // Tiles of outputs x inputs of dweight. For gradients of 16 and of 32 bits: the work-items, the tokens that are staged at a

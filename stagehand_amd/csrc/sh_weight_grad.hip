@@ -132,7 +132,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   constexpr uint32_t kThreads = WO * WI * 64, FO = TO / WO / 16, FI = TI / WI / 16;
   static_assert(FI == 4, "a wavefront's inputs are one group of 64 permuted ones");
   constexpr uint32_t kDy = kStep * TO, kStage = kParts * kDy + kStep * TI, kGroups64 = TI / 64;
-  constexpr uint32_t ND = (kDy / 8 + kThreads - 1) / kThreads, NX = (kStep * TI / 16 + kThreads - 1) / kThreads;
+  constexpr uint32_t ND = kDy / 8 / kThreads, NX = kStep * TI / 16 / kThreads;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wo = wave / WI, wi = wave % WI;
 
@@ -218,26 +218,23 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
       for (uint32_t i = 0; i < 8; ++i) bias[i] += (float)v.dy[j][i];
   };
   auto put_dy = [&](const Staged& v, short* stage, uint32_t j) __attribute__((always_inline)) {
-    if (kDy / 8 < kThreads && threadIdx.x >= kDy / 8) return;
-    {
-      short* at = stage + dy_place + j * kDyRows * TO;
-      if constexpr (kParts == 1) {
-        *reinterpret_cast<typename Values8<T>::Vec*>(at) = v.dy[j];
-      } else {
-        float rest[8];
+    short* at = stage + dy_place + j * kDyRows * TO;
+    if constexpr (kParts == 1) {
+      *reinterpret_cast<typename Values8<T>::Vec*>(at) = v.dy[j];
+    } else {
+      float rest[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) rest[i] = v.dy[j][i];
+      for (uint32_t i = 0; i < 8; ++i) rest[i] = v.dy[j][i];
 #pragma unroll
-        for (uint32_t part = 0; part < kParts; ++part) {
-          Out8 out;
+      for (uint32_t part = 0; part < kParts; ++part) {
+        Out8 out;
 #pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits, as far as bf16 has them; all of an infinity
-            const float head = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xFFFF0000u);
-            out[i] = (E)head;
-            rest[i] = rest[i] == head ? 0.0f : rest[i] - head;
-          }
-          *reinterpret_cast<Out8*>(at + part * kDy) = out;
+        for (uint32_t i = 0; i < 8; ++i) {  // the next 8 significant bits, as far as bf16 has them; all of an infinity
+          const float head = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[i]) & 0xFFFF0000u);
+          out[i] = (E)head;
+          rest[i] = rest[i] == head ? 0.0f : rest[i] - head;
         }
+        *reinterpret_cast<Out8*>(at + part * kDy) = out;
       }
     }
   };
@@ -262,7 +259,7 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   auto put_x = [&](short* stage, uint32_t j, uint32_t f) __attribute__((always_inline)) {
     *reinterpret_cast<Out4*>(stage + kParts * kDy + (x_place ^ f * kXStep) + j * kQRows * TI) = packed[j][f];
   };
-  static_assert(kStep * TI / 16 % kThreads == 0, "every work-item stages inputs");
+  static_assert(kStep * TI / 16 % kThreads == 0 && kDy / 8 % kThreads == 0, "every work-item stages inputs and gradients");
   const uint32_t x_read = read_place<TI>() ^ wi * 16, dy_read = read_place<TO>() ^ wo * FO * 16;
   // Fragment j of x^, of the stage's tokens 32 k .. 32 k + 31.
   auto read_x = [&](const short* stage, uint32_t k, uint32_t j) __attribute__((always_inline)) {
@@ -397,18 +394,15 @@ __device__ __forceinline__ void weight_grad(const sh::WeightGradArgs& a, short* 
   // an output's sums, in their order
   __syncthreads();  // the stages are not read any more
   float* sum = reinterpret_cast<float*>(lds);
-  if (kDy / 8 >= kThreads || threadIdx.x < kDy / 8) {
 #pragma unroll
-    for (uint32_t k = 0; k < 8; ++k) sum[dy_t * TO + dy_o + k] = bias[k];
-  }
+  for (uint32_t k = 0; k < 8; ++k) sum[dy_t * TO + dy_o + k] = bias[k];
   __syncthreads();
-  constexpr uint32_t kSums = kDyRows < kStep ? kDyRows : kStep;  // work-items that staged an output
   for (uint32_t k = threadIdx.x; k < TO; k += kThreads) {
     const uint32_t o = o0 + k;
     if (o >= a.out) continue;
     float v = 0.0f;
 #pragma unroll
-    for (uint32_t r = 0; r < kSums; ++r) v += sum[r * TO + k];
+    for (uint32_t r = 0; r < kDyRows; ++r) v += sum[r * TO + k];
     if (sums != nullptr) sums[(uint64_t)a.out * a.cols + o] = v;
     else if (a.out_dtype == SH_DTYPE_BF16) static_cast<__bf16*>(a.dbias)[o] = (__bf16)v;
     else if (a.out_dtype == SH_DTYPE_F16) static_cast<_Float16*>(a.dbias)[o] = (_Float16)v;
