@@ -76,10 +76,18 @@ constexpr uint32_t kComputeUnits = 256;
 
 // The tile, and into how many parts the tokens are split, of the least estimated time: rounds of workgroups over the
 // compute units, one on each, times the steps of a part; and the parts' sums, written and read once at 3.5 TB/s, with a launch of
-// 3 us. Around the switches, times in us (tile, parts):
-//   1013 x 1000 x 1155    128x128 1: 19   2: 22   256x256 1: 39     4096 x 2048 x 2048   128x128 1: 61   256x256 1: 113   4: 66
-//   16384 x 1024 x 1024   128x128 1: 190  4: 68   256x256 4: 124    4608 x 4096 x 4096   256x256 1: 145  128x128 1: 297
-//   4096 x 32 x 4096      32x128 4: 17    8: 14   16: 21
+// 3 us. Around the switches, times in us (tile, parts), * where the estimate leads:
+//   1013 x 1000 x 1155    *64x128 1: 16  2: 23   128x128 1: 18  2: 21   256x256 1: 40
+//   1013 x 2000 x 1155    64x128 1: 22   *128x128 1: 18  2: 34   256x256 1: 41
+//   4096 x 1024 x 2048    *64x128 1: 46  2: 44   128x128 1: 51  2: 39   256x256 4: 53
+//   4096 x 2048 x 2048    64x128 1: 66   *128x128 1: 52  2: 72   256x256 1: 115  4: 64
+//   16384 x 1024 x 1024   128x128 1: 190  *4: 61   256x256 4: 124
+//   4608 x 4096 x 4096    *256x256 1: 145   128x128 1: 297     fp32: 64x128 1: 578   *128x128 1: 669
+//   16384 x 64 x 4096     32x128 4: 44  8: 47   64x128 4: 50  *8: 31   128x128 8: 33
+//   4096 x 32 x 4096      32x128 4: 17  *8: 13   64x128 8: 14
+//   512 x 1024 x 1024     *32x128 1: 9  2: 20   64x128 1: 9   128x128 1: 10
+// The estimates are off by up to a sixth, and two workgroups of 64 x 128 fit a compute unit, which the rounds do not count: 4096 x
+// 1024 x 2048 and the fp32 row go past the shortest time.
 GradPlan plan_of(const sh_act8* k, uint32_t out, uint32_t dtype, bool bias) {
   const bool wide = dtype == SH_DTYPE_F32;
   const uint64_t sums = (uint64_t)out * k->cols + (bias ? out : 0);

@@ -79,6 +79,8 @@ sh::LayerNormKernelArgs kernel_args(const sh_layer_norm_args* a, bool backward) 
   const uint32_t useful = (ka.tokens + teams - 1) / teams;
   uint32_t per_group;
   if (!backward) {
+    // Work-items a compute unit, times in us. 65536 x 256: 1024 15.1, 1536 14.5, 2048 14.9; x 512 26.2, 24.6, 25.9. Longer rows, 2 x
+    // 8192 x 4096: 512 53, 1024 46, 2048 49.
     per_group = kComputeUnits * ((shape.chunks == 1 ? 1536 : 1024) / threads) / groups;
   } else {
     // Every workgroup leaves a set of sums, that is written and read once more: 16 MB of them at most, and no team has fewer

@@ -12,12 +12,14 @@
 // workgroup's tokens and joined by a second kernel, always in the same order; every workgroup's sums are written and read once
 // more, so there are few workgroups.
 //
-// Measured: forward 2 x 8192 tokens x 4096 bf16 46 us (5.9 TB/s), keeping the input as well 69 us (4.9), 4608 x 4096 16 us (4.6),
-// 65536 x 256 14 us (4.9), 8192 x 16384 102 us (5.3); backward 84 us (4.8 TB/s), from the kept input 69 us (4.9), of which the
-// joining kernel takes 5; a large copy 5.2 TB/s by torch, 6.6 by this library's kernel. Two chunks a work-item against one:
-// 46 and 54 us; 1024 work-items a compute unit against 2048 and 512: 46, 49 and 53 us. Not kept: one or two rows for each of
-// many short workgroups, which stream copies faster (73 us: their start, weights and barriers come with every row), two teams
-// with joined sums in a workgroup of the backward pass (87 against 84 us; 3 x 1013 x 1155 20 against 21), shuffles through LDS for a wavefront's sums.
+// Measured: forward 2 x 8192 tokens x 4096 bf16 46 us (5.9 TB/s), keeping the input as well 66-70 us (4.9), fp32 100 us (5.4),
+// 4608 x 4096 15 us (5.0; 0.5 us of it the correction of the mean), 65536 x 256 14.5 us (4.6), 8192 x 16384 102 us (5.3);
+// backward with the joining kernel, 2 x 8192 x 4096 86-89 us (4.6 TB/s), from the kept input 72-74 (4.6), fp32 157-164 (5.0) and
+// 124-127; 8192 x 16384, whose rows load nothing ahead, 169-175 (4.7) and 142-153, 8 of them the joining; a large copy 5.2 TB/s
+// by torch, 6.6 by this library's kernel. Two chunks a work-item against one: 46 and 54 us; 1024 work-items a compute unit against
+// 2048 and 512: 46, 49 and 53 us. Not kept: one or two rows for each of many short workgroups, which stream copies faster (73 us:
+// their start, weights and barriers come with every row), two teams with joined sums in a workgroup of the backward pass (87
+// against 84 us; 3 x 1013 x 1155 20 against 21), shuffles through LDS for a wavefront's sums.
 
 #include <hip/hip_runtime.h>
 
