@@ -14,7 +14,7 @@
 // instructions that turn bytes into 16-bit values, which every tile of outputs does again, LDS and the barriers, at the clock
 // that their power allows. 16384 x 16384 x 4096 (tokens x outputs x inputs) takes 1.86 to 2.04 ms, 1080 to 1180 TFLOP/s, 4608 x
 // 4096 x 4096 133 to 146 us; reading the input back in 16 bits and a product of the installed library 1.87 ms and 144 us on a
-// box where these took 1.98 ms and 142 us: what is gained at that size is the input's memory. Small ones are bound by the
+// card where these took 1.98 ms and 142 us: what is gained at that size is the input's memory. Small ones are bound by the
 // latency of their first loads and steps (1024^3 12.8 us), adapters of rank 32 by both and the joining of parts (4096 x 32 x 4096
 // 13.9 us for 17 MB; 4096 x 4096 x 32, of whose tiles three quarters hold no inputs, 15). fp32 gradients have four wavefronts a
 // workgroup, one or two a SIMD: 4608 x 4096 x 4096 669 us, 231 TFLOP/s. What it took, at 16384 x 16384 x 4096:
